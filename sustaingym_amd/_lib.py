@@ -133,6 +133,40 @@ BAT_SIGNATURES = {
     'bat_read_metrics': (_i32, [_vp, _vp]),
 }
 
+class LearnerRows(C.Structure):
+    _fields_ = [('logits', C.c_void_p), ('outer', C.c_int64), ('inner', C.c_int64), ('levels', C.c_int64),
+                ('stride_outer', C.c_int64), ('stride_inner', C.c_int64), ('mask', C.c_void_p), ('mask_outer', C.c_int64),
+                ('mask_inner', C.c_int64), ('mask_level', C.c_int32), ('dtype', C.c_int32)]
+
+
+class LearnerSeq(C.Structure):
+    _fields_ = [('steps', C.c_int64), ('batch', C.c_int64), ('channels', C.c_int64), ('reverse', C.c_int32),
+                ('dtype', C.c_int32)]
+
+
+class LearnerView(C.Structure):
+    _fields_ = [('data', C.c_void_p), ('st', C.c_int64), ('sb', C.c_int64), ('sc', C.c_int64)]
+
+
+LEARNER_MAX_TOP = 64
+
+# Every symbol include/learner_ops.h declares
+_i64, _rows, _seq, _view = C.c_int64, C.POINTER(LearnerRows), C.POINTER(LearnerSeq), C.POINTER(LearnerView)
+LEARNER_SIGNATURES = {
+    'lrn_last_error': (C.c_char_p, []),
+    'lrn_choose_workspace': (_i64, [_rows]),
+    'lrn_choose': (_i32, [_i32, _vp, _rows, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64]),
+    'lrn_score_workspace': (_i64, [_rows, _i32]),
+    'lrn_score': (_i32, [_i32, _vp, _rows, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64]),
+    'lrn_score_backward_needs_stat': (_i32, [_rows]),
+    'lrn_score_backward': (_i32, [_i32, _vp, _rows, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
+    'lrn_scan_workspace': (_i64, [_seq]),
+    'lrn_scan': (_i32, [_i32, _vp, _seq, _view, _view, C.c_double, _view, _vp, _view, _vp, _vp, _i64]),
+    'lrn_scan_backward': (_i32, [_i32, _vp, _seq, _view, C.c_double, _view, _vp, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
+    'lrn_advantages_workspace': (_i64, [_seq]),
+    'lrn_advantages': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, C.c_double, C.c_double, _vp, _vp, _vp, _i64]),
+}
+
 _lib = None
 
 
@@ -156,7 +190,7 @@ def load() -> C.CDLL:
         lib = C.CDLL(LIB_PATH)
     except OSError as exc:  # e.g. libamdhip64 missing
         raise EngineLibraryError(f'cannot load {LIB_PATH}: {exc}') from exc
-    for name, (res, args) in list(SIGNATURES.items()) + list(BAT_SIGNATURES.items()):
+    for name, (res, args) in [*SIGNATURES.items(), *BAT_SIGNATURES.items(), *LEARNER_SIGNATURES.items()]:
         try:
             fn = getattr(lib, name)
         except AttributeError as exc:

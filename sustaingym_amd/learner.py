@@ -1,0 +1,418 @@
+"""What a learner computes next to the engine, on the device tensors that the vector environments hand out
+(include/learner_ops.h; hand-written gfx950 kernels in the same library).
+
+    choose_levels(logits, noise, mask)          -> LevelChoice    the levels that ``step`` takes, from a policy's logits
+    level_logprobs(logits, levels, mask, top)   -> LevelScores    log probabilities of levels that were played (differentiable)
+    gated_scan(x, gate, initial, resets)        -> (h, final)     h_t = gate_t h_{t-1} + x_t over a trajectory (differentiable)
+    advantages(rewards, values, ends, ...)      -> Advantages     generalised advantages and value targets
+
+A *level* is a choice of :class:`DiscreteActionWrapper` (or any other index into a row of logits); a row is one decision, so
+a batch of N environments with n stations and K levels is ``logits[N, n, K]``.
+
+Every call runs on the current torch stream of its tensors' device, does not synchronise, and may be captured into a graph.
+Tensors of any strides are taken as they are where the last dimension of logits and noise is dense; anything else is copied
+first.  Wrong arguments raise ``ValueError`` before anything is launched.  There is no CPU form: CPU tensors are refused.
+
+To capture a backward pass, ask for it with ``torch.autograd.grad`` inside the capture, on a forward pass of the same capture.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SEQ_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
+MAX_TOP = _lib.LEARNER_MAX_TOP
+
+
+class LevelChoice(NamedTuple):
+    levels: torch.Tensor         # int64 [...]
+    logprobs: torch.Tensor       # float32 [...]
+    entropy: torch.Tensor        # float32 [...]
+
+
+class LevelScores(NamedTuple):
+    logprobs: torch.Tensor               # float32 [...]
+    entropy: torch.Tensor                # float32 [...]
+    top_logprobs: torch.Tensor | None    # float32 [..., top]
+    top_levels: torch.Tensor | None      # int64 [..., top]
+
+
+class Advantages(NamedTuple):
+    advantages: torch.Tensor     # float32 [T, N]
+    targets: torch.Tensor        # float32 [T, N]
+
+
+def _check(rc: int, what: str) -> None:
+    if rc != 0:
+        raise _lib.EngineLibraryError(f'{what} failed with code {rc}: {_lib.load().lrn_last_error().decode("utf-8", "replace")}')
+
+
+def _need(ok: bool, text: str) -> None:
+    if not ok:
+        raise ValueError(text)
+
+
+def _on_device(name: str, t, device=None) -> None:
+    _need(isinstance(t, torch.Tensor), f'{name}: a tensor is needed, not {type(t).__name__}')
+    _need(t.is_cuda, f'{name}: a CUDA tensor is needed (there is no CPU form)')
+    _need(device is None or t.device == device, f'{name}: on {t.device}, the first argument is on {device}')
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _workspace(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---- rows of logits --------------------------------------------------------------------------------------------------
+
+def _folded(shape, strides):
+    """Leading dimensions as (outer, inner) with two strides for each of ``strides``; None if they do not fold that far."""
+    dims: list[list] = []
+    for i, n in enumerate(shape):
+        if n == 1:
+            continue
+        s = [st[i] for st in strides]
+        if dims and all(p == n * q for p, q in zip(dims[-1][1], s)):
+            dims[-1] = [dims[-1][0] * n, s]
+        else:
+            dims.append([n, s])
+    if len(dims) > 2:
+        return None
+    while len(dims) < 2:
+        dims.insert(0, [1, [0] * len(strides)])
+    return dims[0][0], dims[1][0], list(zip(dims[0][1], dims[1][1]))
+
+
+class _Rows:
+    """logits (and mask, noise) laid out for the C call; keeps the tensors that its pointers belong to alive."""
+
+    __slots__ = ('struct', 'keep', 'noise', 'noise_strides')
+
+    def __init__(self, logits, mask, noise=None):
+        lead, K = logits.shape[:-1], logits.shape[-1]
+        if logits.stride(-1) != 1 and K > 1:
+            logits = logits.contiguous()
+        mask_level = 1
+        if mask is not None:
+            if mask.shape != logits.shape:
+                mask = mask.expand(logits.shape)
+            mask_level = mask.stride(-1)
+            if mask_level not in (0, 1):
+                mask = mask.contiguous()
+                mask_level = 1 if K > 1 else 0
+        if noise is not None:
+            if noise.shape != logits.shape:
+                noise = noise.expand(logits.shape)
+            if noise.stride(-1) != 1 and K > 1:
+                noise = noise.contiguous()
+        n = math.prod(lead)
+        if logits.is_contiguous() and (mask is None or mask.is_contiguous()) and (noise is None or noise.is_contiguous()):
+            outer, inner, strides = 1, n, [(0, K)] * 3
+        elif n == 0:
+            outer, inner, strides = 0, 0, [(0, 0)] * 3
+        else:
+            there = [t for t in (logits, mask, noise) if t is not None]
+            folded = _folded(lead, [t.stride()[:-1] for t in there])
+            if folded is None:
+                logits = logits.contiguous()
+                mask = None if mask is None else mask.contiguous()
+                noise = None if noise is None else noise.contiguous()
+                mask_level = 1
+                folded = 1, n, [(0, K)] * 3
+            outer, inner, strides = folded
+            strides = list(strides)
+            if mask is None:
+                strides.insert(1, (0, 0))
+            if noise is None:
+                strides.append((0, 0))
+        self.struct = _lib.LearnerRows(logits.data_ptr(), outer, inner, K, strides[0][0], strides[0][1], _ptr(mask),
+                                       strides[1][0], strides[1][1], mask_level, _ROW_TYPES[logits.dtype])
+        self.keep = (logits, mask, noise)
+        self.noise, self.noise_strides = noise, strides[2]
+
+
+def _check_rows(logits, mask, noise=None):
+    _on_device('logits', logits)
+    _need(logits.dtype in _ROW_TYPES, f'logits: float32, bfloat16 or float16, not {logits.dtype}')
+    _need(logits.dim() >= 1 and 1 <= logits.shape[-1] < 2 ** 30, f'logits: [..., levels], got {tuple(logits.shape)}')
+    for name, t, kinds in (('mask', mask, (torch.bool,)), ('noise', noise, (torch.float32,))):
+        if t is None:
+            continue
+        _on_device(name, t, logits.device)
+        _need(t.dtype in kinds, f'{name}: {kinds[0]}, not {t.dtype}')
+        if t.shape != logits.shape:
+            try:
+                ok = torch.broadcast_shapes(t.shape, logits.shape) == logits.shape
+            except RuntimeError:
+                ok = False
+            _need(ok, f'{name}: {tuple(t.shape)} does not broadcast to the logits\' {tuple(logits.shape)}')
+
+
+def choose_levels(logits, noise=None, mask=None) -> LevelChoice:
+    """One level for every row: the allowed one with the largest ``logits + noise`` (the lowest index among equals).
+
+    logits: ``[..., K]`` float32 / bfloat16 / float16.
+    noise: float32, broadcastable to the logits; with Gumbel noise (``-log(-log(u))``) the level is a sample of
+        ``softmax(logits)`` over the allowed levels, without noise it is the most probable one.
+    mask: bool, broadcastable to the logits, True = allowed (``mask[N, n, 1]``: stations without a car).
+
+    Returns int64 levels — what ``EVChargingVectorEnv(discrete_bins=K).step`` takes — with their log probabilities and the
+    entropy of every row (of the logits without noise; float32).  A row without an allowed level gives level 0, log
+    probability 0 and entropy 0.  No gradient flows: a learner asks :func:`level_logprobs` for the same levels."""
+    _check_rows(logits, mask, noise)
+    logits = logits.detach()
+    lib, device, shape = _lib.load(), logits.device, logits.shape[:-1]
+    levels = torch.empty(shape, dtype=torch.int64, device=device)
+    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    rows = _Rows(logits, mask, noise)
+    ref = C.byref(rows.struct)
+    nbytes = lib.lrn_choose_workspace(ref)
+    ws = _workspace(nbytes, device)
+    _check(lib.lrn_choose(device.index, _stream(device), ref, _ptr(rows.noise), rows.noise_strides[0], rows.noise_strides[1],
+                          levels.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(), _ptr(ws), nbytes), 'choose_levels')
+    return LevelChoice(levels, logprobs, entropy)
+
+
+def _score(rows, levels, shape, device, top, want_stat):
+    lib = _lib.load()
+    ref = C.byref(rows.struct)
+    logprobs = torch.empty(shape, dtype=torch.float32, device=device)
+    entropy = torch.empty(shape, dtype=torch.float32, device=device)
+    stat = torch.empty((*shape, 2), dtype=torch.float32, device=device) if want_stat else None
+    tl = torch.empty((*shape, top), dtype=torch.float32, device=device) if top else None
+    ti = torch.empty((*shape, top), dtype=torch.int64, device=device) if top else None
+    nbytes = lib.lrn_score_workspace(ref, top)
+    ws = _workspace(nbytes, device)
+    _check(lib.lrn_score(device.index, _stream(device), ref, levels.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
+                         _ptr(stat), top, _ptr(tl), _ptr(ti), _ptr(ws), nbytes), 'level_logprobs')
+    return logprobs, entropy, stat, tl, ti
+
+
+def _row_gradient(g):
+    """A per-row gradient and its element stride: one value for all rows (a sum's gradient) is not spread out."""
+    if g is None:
+        return None, 0
+    if all(s == 0 or n == 1 for n, s in zip(g.shape, g.stride())):
+        return g, 0
+    return g.contiguous(), 1
+
+
+class _LevelLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, levels, mask, top):
+        rows = _Rows(logits, mask)
+        needs = bool(_lib.load().lrn_score_backward_needs_stat(C.byref(rows.struct)))
+        logprobs, entropy, stat, tl, ti = _score(rows, levels, logits.shape[:-1], logits.device, top, needs)
+        ctx.save_for_backward(logits, levels, mask, stat, entropy if needs else None)
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(tl, ti)
+        return logprobs, entropy, tl, ti
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, *_):
+        logits, levels, mask, stat, entropy = ctx.saved_tensors
+        rows = _Rows(logits, mask)
+        g_logprobs, s_lp = _row_gradient(g_logprobs)
+        g_entropy, s_h = _row_gradient(g_entropy)
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _check(_lib.load().lrn_score_backward(logits.device.index, _stream(logits.device), C.byref(rows.struct),
+                                              levels.data_ptr(), _ptr(stat), _ptr(entropy), _ptr(g_logprobs), s_lp,
+                                              _ptr(g_entropy), s_h, grad.data_ptr()), 'level_logprobs backward')
+        return grad, None, None, None
+
+
+def level_logprobs(logits, levels, mask=None, top: int = 0) -> LevelScores:
+    """Log probabilities of given levels under ``softmax(logits)`` over the allowed levels, entropies, and alternatives.
+
+    logits: ``[..., K]`` float32 / bfloat16 / float16; gradients of ``logprobs`` and ``entropy`` flow to them.
+    levels: int64 or int32 ``[...]``; a negative level marks a padded row (log probability 0, no gradient through it).  A level
+        that the mask forbids has log probability -inf; one ``>= K`` gives NaN (levels are not looked at on the host).
+    mask: bool, broadcastable to the logits, True = allowed; what masked places hold is never used.  A row that the mask leaves
+        empty has log probability 0, entropy 0 and gradient 0.
+    top: 0 .. min(K, 64): the most probable levels of each row in falling order (the lowest index first among equals) with their
+        log probabilities, ``[..., top]``; behind the last allowed one -1 and -inf.  No gradient flows through these.
+
+    Log probabilities, entropies and all sums are float32 whatever the logits' type; the gradient has the logits' type."""
+    _check_rows(logits, mask)
+    _on_device('levels', levels, logits.device)
+    _need(levels.dtype in (torch.int64, torch.int32), f'levels: int64 or int32, not {levels.dtype}')
+    _need(levels.shape == logits.shape[:-1], f'levels: {tuple(levels.shape)}, the logits have rows {tuple(logits.shape[:-1])}')
+    top = int(top)
+    _need(0 <= top <= min(MAX_TOP, logits.shape[-1]), f'top: 0 .. {min(MAX_TOP, logits.shape[-1])}, got {top}')
+    if levels.dtype != torch.int64 or not levels.is_contiguous():
+        levels = levels.to(torch.int64).contiguous()
+    if logits.requires_grad and torch.is_grad_enabled():
+        return LevelScores(*_LevelLogprobs.apply(logits, levels, mask, top))
+    rows = _Rows(logits.detach(), mask)
+    logprobs, entropy, _, tl, ti = _score(rows, levels, logits.shape[:-1], logits.device, top, False)
+    return LevelScores(logprobs, entropy, tl, ti)
+
+
+# ---- recurrences -----------------------------------------------------------------------------------------------------
+
+def _view(t, dim):
+    """(time, batch, channel) strides of a tensor whose time dimension is ``dim``."""
+    if t is None:
+        return None
+    st = t.stride()
+    if t.dim() == 1:
+        return _lib.LearnerView(t.data_ptr(), st[0], 0, 0)
+    return _lib.LearnerView(t.data_ptr(), st[dim], st[1 - dim], st[2] if t.dim() > 2 else 0)
+
+
+def _ref(v):
+    return None if v is None else C.byref(v)
+
+
+def _sequence(shape, dim, reverse, dtype):
+    return _lib.LearnerSeq(shape[dim], shape[1 - dim] if len(shape) > 1 else 1, shape[2] if len(shape) > 2 else 1,
+                           int(reverse), _SEQ_TYPES[dtype])
+
+
+def _state_type(dtype):
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
+def _scan(x, gate, gate_const, initial, resets, dim, reverse):
+    lib, device = _lib.load(), x.device
+    h = torch.empty(x.shape, dtype=x.dtype, device=device)
+    final = torch.empty([n for i, n in enumerate(x.shape) if i != dim], dtype=_state_type(x.dtype), device=device)
+    seq = _sequence(x.shape, dim, reverse, x.dtype)
+    ref = C.byref(seq)
+    nbytes = lib.lrn_scan_workspace(ref)
+    ws = _workspace(nbytes, device)
+    _check(lib.lrn_scan(device.index, _stream(device), ref, _ref(_view(x, dim)), _ref(_view(gate, dim)), gate_const,
+                        _ref(_view(resets, dim)), _ptr(initial), _ref(_view(h, dim)), final.data_ptr(), _ptr(ws), nbytes),
+           'gated_scan')
+    return h, final
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, initial, resets, gate_const, dim, reverse):
+        h, final = _scan(x, gate, gate_const, initial, resets, dim, reverse)
+        # The gate's gradient needs the states; where they were rounded to 16 bits, so is their share of it (half a step of h),
+        # for what reading x and walking forward again would cost.
+        ctx.save_for_backward(gate, resets, initial, h if ctx.needs_input_grad[1] else None)
+        ctx.args = (gate_const, dim, reverse, x.shape, x.dtype, x.device)
+        ctx.set_materialize_grads(False)
+        return h, final
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_h, g_final):
+        gate, resets, initial, h = ctx.saved_tensors
+        gate_const, dim, reverse, shape, dtype, device = ctx.args
+        want_x, want_gate, want_initial = ctx.needs_input_grad[:3]
+        if g_h is None and g_final is None:
+            return (None,) * 7
+        lib = _lib.load()
+        g_final = None if g_final is None else g_final.contiguous()
+        gx = torch.empty(shape, dtype=dtype, device=device) if want_x else None
+        gg = torch.empty(shape, dtype=dtype, device=device) if want_gate else None
+        gi = torch.empty(initial.shape, dtype=initial.dtype, device=device) if want_initial else None
+        seq = _sequence(shape, dim, reverse, dtype)
+        ref = C.byref(seq)
+        nbytes = lib.lrn_scan_workspace(ref)
+        ws = _workspace(nbytes, device)
+        _check(lib.lrn_scan_backward(device.index, _stream(device), ref, _ref(_view(gate, dim)), gate_const,
+                                     _ref(_view(resets, dim)), _ptr(initial), _ref(_view(h, dim)), _ref(_view(g_h, dim)),
+                                     _ptr(g_final), _ref(_view(gx, dim)), _ref(_view(gg, dim)), _ptr(gi), _ptr(ws), nbytes),
+               'gated_scan backward')
+        return gx, gg, gi, None, None, None, None
+
+
+def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool = False):
+    """``h_t = gate_t * h_{t-1} + x_t`` along ``dim``; returns ``(h, final)``.
+
+    x: ``[T]``, ``[T, N]`` or ``[T, N, C]`` (``dim=0``), ``[N, T]`` or ``[N, T, C]`` (``dim=1``); float32, bfloat16, float16 or
+        float64.  T may be 0 (``final`` is the initial state) or 1 (one step of a policy's state).
+    gate: a tensor of x's type, broadcastable to x, or a number (discounted returns: ``gated_scan(rewards, gamma,
+        resets=ends, reverse=True)``).
+    initial: the state before the first step, x's shape without ``dim`` (float32; float64 for float64 x); None = 0.
+    resets: bool, x's first two dimensions: the sequence starts anew at this step, ``h_t = x_t`` — nothing from before enters,
+        not even a NaN.  Forward, that is the step AFTER an episode's end; with ``reverse`` the step of the end itself.
+    reverse: from the last step to the first (``h_t = gate_t * h_{t+1} + x_t``).
+
+    ``h`` has x's type and is contiguous; ``final`` is the last state of the walk in the state's own type, what a following
+    call takes as ``initial``.  Differentiable in x, gate and initial."""
+    _on_device('x', x)
+    _need(x.dtype in _SEQ_TYPES, f'x: float32, bfloat16, float16 or float64, not {x.dtype}')
+    _need(1 <= x.dim() <= 3, f'x: one to three dimensions, got {tuple(x.shape)}')
+    _need(dim in (0, 1) and dim < x.dim(), f'dim: 0 or 1 of {tuple(x.shape)}, got {dim}')
+    const = 0.0
+    if isinstance(gate, torch.Tensor):
+        _on_device('gate', gate, x.device)
+        _need(gate.dtype == x.dtype, f'gate: {gate.dtype}, x is {x.dtype}')
+        if gate.shape != x.shape:
+            try:
+                ok = torch.broadcast_shapes(gate.shape, x.shape) == x.shape
+            except RuntimeError:
+                ok = False
+            _need(ok, f'gate: {tuple(gate.shape)} does not broadcast to x\'s {tuple(x.shape)}')
+            gate = gate.expand(x.shape)
+    else:
+        _need(isinstance(gate, (int, float)), f'gate: a tensor or a number, not {type(gate).__name__}')
+        const, gate = float(gate), None
+    if initial is not None:
+        _on_device('initial', initial, x.device)
+        shape = tuple(n for i, n in enumerate(x.shape) if i != dim)
+        _need(tuple(initial.shape) == shape, f'initial: {tuple(initial.shape)} instead of {shape}')
+        _need(initial.dtype == _state_type(x.dtype), f'initial: {_state_type(x.dtype)}, not {initial.dtype}')
+        initial = initial.contiguous()
+    if resets is not None:
+        _on_device('resets', resets, x.device)
+        _need(resets.dtype == torch.bool, f'resets: torch.bool, not {resets.dtype}')
+        _need(resets.shape == x.shape[:2], f'resets: {tuple(resets.shape)} instead of {tuple(x.shape[:2])}')
+    reverse = bool(reverse)
+    if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad)
+                                    or (initial is not None and initial.requires_grad)):
+        return _GatedScan.apply(x, gate, initial, resets, const, dim, reverse)
+    return _scan(x.detach(), gate, const, initial, resets, dim, reverse)
+
+
+def advantages(rewards, values, ends, last_values, gamma: float = 0.99, lam: float = 0.95) -> Advantages:
+    """Generalised advantages ``A_t = d_t + gamma lam (1 - end_t) A_{t+1}``, ``d_t = r_t + gamma (1 - end_t) V_{t+1} - V_t``, and
+    the value targets ``A_t + V_t`` of a trajectory.
+
+    rewards: ``[T, N]`` (or ``[T]``) float64, as the engines write them, or float32; values: float32, the same shape;
+    ends: bool, the same shape, True where the episode ended with that step; last_values: float32 ``[N]``, the value of the
+    state behind the last step.  Float32 results; the arithmetic is float64 where the rewards are.  No gradient flows."""
+    _on_device('rewards', rewards)
+    device, shape = rewards.device, rewards.shape
+    _need(rewards.dtype in (torch.float64, torch.float32), f'rewards: float64 or float32, not {rewards.dtype}')
+    _need(1 <= rewards.dim() <= 2, f'rewards: [T, N] or [T], got {tuple(shape)}')
+    for name, t, kind, want in (('values', values, torch.float32, shape), ('ends', ends, torch.bool, shape),
+                                ('last_values', last_values, torch.float32, shape[1:])):
+        _on_device(name, t, device)
+        _need(t.dtype == kind, f'{name}: {kind}, not {t.dtype}')
+        _need(t.shape == want, f'{name}: {tuple(t.shape)} instead of {tuple(want)}')
+    lib = _lib.load()
+    adv = torch.empty(shape, dtype=torch.float32, device=device)
+    tgt = torch.empty(shape, dtype=torch.float32, device=device)
+    seq = _sequence(shape, 0, True, rewards.dtype)
+    ref = C.byref(seq)
+    nbytes = lib.lrn_advantages_workspace(ref)
+    ws = _workspace(nbytes, device)
+    last_values = last_values.detach().contiguous()
+    _check(lib.lrn_advantages(device.index, _stream(device), ref, _ref(_view(rewards, 0)), _ref(_view(values, 0)), _ref(_view(ends, 0)),
+                              last_values.data_ptr(), float(gamma), float(lam), adv.data_ptr(), tgt.data_ptr(), _ptr(ws), nbytes),
+           'advantages')
+    return Advantages(adv, tgt)

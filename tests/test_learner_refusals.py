@@ -1,0 +1,143 @@
+"""Arguments that the learner's operators refuse before anything is launched: the Python checks, and the C-ABI's own."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+from sustaingym_amd import _lib, learner
+
+
+def learner_symbols():
+    text = open(os.path.join(os.path.dirname(_lib.HEADER_PATH), 'learner_ops.h')).read()
+    text = re.sub(r'/\*.*?\*/', '', text, flags=re.S)
+    return sorted(set(re.findall(r'\b(lrn_[a-z_0-9]+)\s*\(', text)))
+
+
+def test_header_binding_and_library_agree():
+    lib = _lib.load()
+    assert sorted(_lib.LEARNER_SIGNATURES) == learner_symbols()
+    assert all(hasattr(lib, name) for name in learner_symbols())
+    text = open(os.path.join(os.path.dirname(_lib.HEADER_PATH), 'learner_ops.h')).read()
+    assert int(re.search(r'#define\s+LRN_MAX_TOP\s+(\d+)', text).group(1)) == _lib.LEARNER_MAX_TOP == learner.MAX_TOP
+
+
+def test_cpu_tensors_are_refused():
+    z = torch.zeros(4, 5)
+    for call in (lambda: learner.choose_levels(z), lambda: learner.level_logprobs(z, torch.zeros(4, dtype=torch.int64)),
+                 lambda: learner.gated_scan(z, 0.5), lambda: learner.advantages(z, z, z > 0, z[0])):
+        with pytest.raises(ValueError, match='no CPU form'):
+            call()
+    with pytest.raises(ValueError, match='a tensor is needed'):
+        learner.choose_levels([1.0, 2.0])
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """The checks behind the device check, on CPU tensors."""
+    monkeypatch.setattr(learner, '_on_device', lambda name, t, device=None: None)
+
+
+def refused(match, call):
+    with pytest.raises(ValueError, match=match):
+        call()
+
+
+def test_row_arguments(anywhere):
+    z, l = torch.zeros(4, 3, 5), torch.zeros(4, 3, dtype=torch.int64)
+    refused('logits: float32', lambda: learner.choose_levels(z.double()))
+    refused('logits: \\[..., levels\\]', lambda: learner.choose_levels(torch.zeros(())))
+    refused('logits: \\[..., levels\\]', lambda: learner.choose_levels(torch.zeros(3, 0)))
+    refused('noise: torch.float32', lambda: learner.choose_levels(z, z.double()))
+    refused('noise: .* does not broadcast', lambda: learner.choose_levels(z, torch.zeros(4, 3, 4)))
+    refused('noise: .* does not broadcast', lambda: learner.choose_levels(z, torch.zeros(2, 4, 3, 5)))
+    refused('mask: torch.bool', lambda: learner.choose_levels(z, None, z))
+    refused('mask: .* does not broadcast', lambda: learner.level_logprobs(z, l, torch.ones(4, 2, 1, dtype=torch.bool)))
+    refused('levels: int64', lambda: learner.level_logprobs(z, l.float()))
+    refused('levels: \\(4,\\)', lambda: learner.level_logprobs(z, l[:, 0]))
+    refused('top: 0 .. 5, got 6', lambda: learner.level_logprobs(z, l, None, 6))
+    refused('top: 0 .. 64, got 65', lambda: learner.level_logprobs(torch.zeros(4, 100), l[:, 0], None, 65))
+    refused('top: 0', lambda: learner.level_logprobs(z, l, None, -1))
+
+
+def test_sequence_arguments(anywhere):
+    x = torch.zeros(6, 4, 3)
+    refused('x: float32', lambda: learner.gated_scan(x.long(), 0.5))
+    refused('x: one to three', lambda: learner.gated_scan(x[None], 0.5))
+    refused('dim: 0 or 1', lambda: learner.gated_scan(x, 0.5, dim=2))
+    refused('dim: 0 or 1', lambda: learner.gated_scan(x[:, 0, 0], 0.5, dim=1))
+    refused('gate: torch.float64, x is torch.float32', lambda: learner.gated_scan(x, x.double()))
+    refused('gate: .* does not broadcast', lambda: learner.gated_scan(x, torch.zeros(6, 4, 2)))
+    refused('gate: a tensor or a number', lambda: learner.gated_scan(x, 'a'))
+    refused('initial: \\(6, 3\\) instead of \\(4, 3\\)', lambda: learner.gated_scan(x, 0.5, torch.zeros(6, 3)))
+    refused('initial: torch.float32, not torch.float64', lambda: learner.gated_scan(x, 0.5, torch.zeros(4, 3).double()))
+    refused('initial: torch.float64', lambda: learner.gated_scan(x.double(), 0.5, torch.zeros(4, 3)))
+    refused('resets: torch.bool', lambda: learner.gated_scan(x, 0.5, None, torch.zeros(6, 4)))
+    refused('resets: \\(4, 6\\) instead', lambda: learner.gated_scan(x, 0.5, None, torch.zeros(4, 6, dtype=torch.bool)))
+    r, e = torch.zeros(6, 4), torch.zeros(6, 4, dtype=torch.bool)
+    refused('rewards: float64 or float32', lambda: learner.advantages(r.half(), r, e, r[0]))
+    refused('rewards: \\[T, N\\]', lambda: learner.advantages(x, x, x > 0, x[0]))
+    refused('values: torch.float32', lambda: learner.advantages(r, r.double(), e, r[0]))
+    refused('ends: torch.bool', lambda: learner.advantages(r, r, r, r[0]))
+    refused('last_values: \\(6,\\) instead of \\(4,\\)', lambda: learner.advantages(r, r, e, r[:, 0]))
+
+
+def test_strides_fold():
+    f = learner._folded
+    assert f((4, 6), [(30, 5)]) == (1, 24, [(0, 5)])
+    assert f((4, 6), [(60, 5), (0, 5)]) == (4, 6, [(60, 5), (0, 5)])
+    assert f((4, 1, 6), [(60, 7, 5)]) == (4, 6, [(60, 5)])
+    assert f((2, 3, 4), [(100, 30, 5)]) is None
+    assert f((), [()]) == (1, 1, [(0, 0)])
+    assert f((2, 3, 4), [(60, 20, 5), (0, 0, 0)]) == (1, 24, [(0, 5), (0, 0)])
+
+
+def test_the_c_abi_refuses():
+    """Every refusal comes before the device is touched, so it is the same without one."""
+    lib = _lib.load()
+    one = C.c_void_p(64)            # never dereferenced by a refused call
+
+    def rows(**kw):
+        base = dict(logits=64, outer=1, inner=4, levels=5, stride_outer=0, stride_inner=5, mask=None, mask_outer=0, mask_inner=0, mask_level=0, dtype=0)
+        return C.byref(_lib.LearnerRows(**{**base, **kw}))
+
+    def text():
+        return lib.lrn_last_error().decode()
+
+    for kw in (dict(levels=0), dict(levels=2 ** 30), dict(outer=-1), dict(inner=-1), dict(dtype=3), dict(dtype=-1), dict(mask_level=2), dict(logits=None)):
+        assert lib.lrn_choose(0, None, rows(**kw), None, 0, 0, one, one, one, None, 0) == -1 and 'rows' in text()
+        assert lib.lrn_score(0, None, rows(**kw), one, one, one, None, 0, None, None, None, 0) == -1
+        assert lib.lrn_score_backward(0, None, rows(**kw), one, one, one, None, 0, None, 0, one) == -1
+    assert lib.lrn_choose(0, None, None, None, 0, 0, one, one, one, None, 0) == -1
+    assert lib.lrn_choose(0, None, rows(), None, 0, 0, None, one, one, None, 0) == -1 and 'null output' in text()
+    for top in (-1, 6, 65):
+        assert lib.lrn_score(0, None, rows(), one, one, one, None, top, one, one, None, 0) == -1 and 'top' in text()
+    assert lib.lrn_score(0, None, rows(), one, one, one, None, 2, None, one, None, 0) == -1
+    assert lib.lrn_score_backward(0, None, rows(levels=3001, stride_inner=3001), one, one, one, one, 2, None, 0, one) == -1 and 'strides' in text()
+    big = rows(levels=200000, stride_inner=200000)
+    need = lib.lrn_score_workspace(big, 5)
+    if need:
+        assert lib.lrn_score(0, None, big, one, one, one, None, 5, one, one, one, need - 1) == -1 and 'workspace' in text()
+        assert lib.lrn_score(0, None, big, one, one, one, None, 5, one, one, None, need) == -1
+    need = lib.lrn_choose_workspace(big)
+    if need:
+        assert lib.lrn_choose(0, None, big, None, 0, 0, one, one, one, one, need - 1) == -1 and 'workspace' in text()
+
+    def seq(**kw):
+        return C.byref(_lib.LearnerSeq(**{**dict(steps=4, batch=2, channels=3, reverse=0, dtype=0), **kw}))
+
+    v = C.byref(_lib.LearnerView(64, 6, 3, 1))
+    for kw in (dict(steps=-1), dict(batch=-1), dict(channels=-1), dict(dtype=4), dict(dtype=-1)):
+        assert lib.lrn_scan(0, None, seq(**kw), v, None, 0.5, None, None, v, None, None, 0) == -1
+        assert lib.lrn_scan_backward(0, None, seq(**kw), None, 0.5, None, None, None, v, None, v, None, None, None, 0) == -1
+    assert lib.lrn_scan(0, None, seq(), None, None, 0.5, None, None, v, None, None, 0) == -1
+    assert lib.lrn_scan(0, None, seq(), v, None, 0.5, None, None, None, None, None, 0) == -1
+    assert lib.lrn_scan_backward(0, None, seq(), v, 0.0, None, None, None, v, None, v, v, None, None, 0) == -1 and 'null h' in text()
+    long = seq(steps=10 ** 6, batch=1, channels=1)
+    need = lib.lrn_scan_workspace(long)
+    if need:
+        assert lib.lrn_scan(0, None, long, v, None, 0.5, None, None, v, None, one, need - 1) == -1 and 'workspace' in text()
+    assert lib.lrn_advantages(0, None, seq(), v, v, v, one, 0.9, 0.9, one, one, None, 0) == -1 and 'channels' in text()
+    assert lib.lrn_advantages(0, None, seq(channels=1, dtype=1), v, v, v, one, 0.9, 0.9, one, one, None, 0) == -1 and 'dtype' in text()
+    assert lib.lrn_advantages(0, None, seq(channels=1), v, v, None, one, 0.9, 0.9, one, one, None, 0) == -1
