@@ -20,6 +20,7 @@ struct Rows {
     int64_t rows, inner;
     int64_t so, si, mo, mi;
     int32_t levels, mask_level;
+    uint32_t per_level;          // ceil(2^32 / levels): e / levels = e per_level >> 32 for e < 2^16, levels <= 1024
 };
 
 struct Sums {
@@ -84,9 +85,17 @@ struct TopList {
     }
 };
 
-__device__ __forceinline__ int64_t row_base(const Rows& R, int64_t r) { return (r / R.inner) * R.so + (r % R.inner) * R.si; }
+// row r = (o, i)
+__device__ __forceinline__ void split(const Rows& R, int64_t r, int64_t& o, int64_t& i) {
+    if ((uint64_t)R.rows <= 0xffffffffu) { o = (uint32_t)r / (uint32_t)R.inner; i = (uint32_t)r - (uint32_t)o * (uint32_t)R.inner; }
+    else { o = r / R.inner; i = r - o * R.inner; }
+}
+__device__ __forceinline__ int64_t row_base(const Rows& R, int64_t r) { int64_t o, i; split(R, r, o, i); return o * R.so + i * R.si; }
 __device__ __forceinline__ const uint8_t* row_mask(const Rows& R, int64_t r) {
-    return R.mask ? R.mask + (r / R.inner) * R.mo + (r % R.inner) * R.mi : nullptr;
+    if (!R.mask) return nullptr;
+    int64_t o, i;
+    split(R, r, o, i);
+    return R.mask + o * R.mo + i * R.mi;
 }
 
 __device__ __forceinline__ void wave_join(Sums& a) {
@@ -200,6 +209,261 @@ __global__ __launch_bounds__(256) void score_backward_kernel(Rows R, BackIn I, T
     }
 }
 
+// ---- rows of up to 1024 levels: G lanes to a row -----------------------------------------------------------------------
+//
+// A workgroup takes 256 / G rows.  Their logits are one run of memory (FLAT): 16-byte loads by all lanes bring it, whatever
+// the rows' length, and the rows are picked out of LDS, where they sit an odd number of words apart (no two lanes of a
+// half-wavefront on one bank).  A lane holds E levels of its row in registers, so that the maximum comes first and every
+// weight is computed once; the group's sums go through DPP.  The backward pass computes the row's maximum and sums again from
+// the logits that it has to read anyway: cheaper than 12 bytes a row of saved statistics.  Rows at other strides, broadcast
+// masks and unaligned starts are read a row at a time by the row's own lanes (not FLAT).
+
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL> __device__ __forceinline__ int dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+
+// f(v) for the partner lanes: neighbours, pairs, quads and half rows of 16 by DPP (each step's partner holds the other half's
+// result, mirrored where the hardware has no exchange), 16 and 32 lanes apart by a lane exchange.
+template <int G, class F> __device__ __forceinline__ void over_group(F&& f) {
+    if constexpr (G >= 2) f([](auto v) { return dpp<0xB1>(v); });
+    if constexpr (G >= 4) f([](auto v) { return dpp<0x4E>(v); });
+    if constexpr (G >= 8) f([](auto v) { return dpp<0x141>(v); });
+    if constexpr (G >= 16) f([](auto v) { return dpp<0x140>(v); });
+    if constexpr (G >= 32) f([](auto v) { return __shfl_xor(v, 16); });
+    if constexpr (G >= 64) f([](auto v) { return __shfl_xor(v, 32); });
+}
+
+// What a group knows of its row: the levels g, g + G, ... are z[0], z[1], ... of lane g (-inf behind the row and where masked).
+template <int G, int E>
+__device__ __forceinline__ Sums group_sums(const float (&z)[E], float (&e)[E]) {
+    Sums a;
+    a.m = z[0];
+#pragma unroll
+    for (int k = 1; k < E; k++) a.m = fmaxf(a.m, z[k]);
+    over_group<G>([&](auto from) { a.m = fmaxf(a.m, from(a.m)); });
+    a.s = a.t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        const float d = z[k] - a.m;
+        e[k] = z[k] == kNegInf ? 0.0f : fast_exp(d);
+        a.s += e[k];
+        a.t += e[k] > 0.0f ? e[k] * d : 0.0f;
+    }
+    over_group<G>([&](auto from) { a.s += from(a.s); a.t += from(a.t); });
+    finish(a);
+    return a;
+}
+
+template <int G, int E> constexpr int kTile = 256 / G * (G * E + 1);
+
+// The tile's logits (and noise) into LDS as float32; masked ones as -inf.
+template <class T, int G, int E, bool FLAT, bool NOISE>
+__device__ __forceinline__ void load_tile(const Rows& R, const ChooseOut* C, int64_t r0, int rows, float* z, float* nz) {
+    const int K = R.levels, pitch = K | 1, tid = threadIdx.x;
+    if constexpr (FLAT) {
+        constexpr int VE = 16 / sizeof(T);
+        const int n = rows * K;
+        const T* src = (const T*)R.logits + r0 * K;
+        const uint8_t* mk = R.mask ? R.mask + r0 * K : nullptr;
+        const float* ns = NOISE && C->noise ? C->noise + r0 * K : nullptr;
+        for (int e0 = tid * VE; e0 < n; e0 += 256 * VE) {
+            int row = __umulhi((uint32_t)e0, R.per_level), col = e0 - row * K;
+            T v[VE];
+            uint8_t b[VE];
+            float w[VE];
+            const bool whole = e0 + VE <= n;
+            if (whole) {
+                *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + e0);
+                if (mk) {
+                    if constexpr (VE == 8) *reinterpret_cast<uint2*>(b) = *reinterpret_cast<const uint2*>(mk + e0);
+                    else *reinterpret_cast<uint32_t*>(b) = *reinterpret_cast<const uint32_t*>(mk + e0);
+                }
+                if (NOISE && ns) {
+#pragma unroll
+                    for (int k = 0; k < VE; k += 4) *reinterpret_cast<float4*>(w + k) = *reinterpret_cast<const float4*>(ns + e0 + k);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < VE; k++)
+                    if (e0 + k < n) { v[k] = src[e0 + k]; if (mk) b[k] = mk[e0 + k]; if (NOISE && ns) w[k] = ns[e0 + k]; }
+            }
+#pragma unroll
+            for (int k = 0; k < VE; k++) {
+                if (whole || e0 + k < n) {
+                    z[row * pitch + col] = mk && !b[k] ? kNegInf : to_f32(v[k]);
+                    if (NOISE && ns) nz[row * pitch + col] = w[k];
+                }
+                if (++col == K) { col = 0; row++; }
+            }
+        }
+    } else {
+        const int row = tid / G, g = tid % G;
+        if (row < rows) {
+            int64_t o, i;
+            split(R, r0 + row, o, i);
+            const T* src = (const T*)R.logits + o * R.so + i * R.si;
+            const uint8_t* mk = R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
+            const float* ns = NOISE && C->noise ? C->noise + o * C->no + i * C->ni : nullptr;
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const int j = g + G * k;
+                if (j < K) {
+                    z[row * pitch + j] = mk && !mk[j * R.mask_level] ? kNegInf : to_f32(src[j]);
+                    if (NOISE && ns) nz[row * pitch + j] = ns[j];
+                }
+            }
+        }
+    }
+    __syncthreads();
+}
+
+template <class T, int G, int E, bool FLAT>
+__global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) {
+    __shared__ float zs[kTile<G, E>], ns[kTile<G, E>];
+    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
+    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels;
+    load_tile<T, G, E, FLAT, true>(R, &O, r0, rows, zs, ns);
+    const int row = threadIdx.x / G, g = threadIdx.x % G;
+    if (row >= rows) return;                    // whole groups: no lane of a group leaves alone
+    const float* mine = zs + row * (K | 1);
+    const float* noise = ns + row * (K | 1);
+    float z[E], e[E];
+    Best b;
+    b.clear();
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        const int j = g + G * k;
+        z[k] = j < K ? mine[j] : kNegInf;
+        if (z[k] != kNegInf) b.add(O.noise ? z[k] + noise[j] : z[k], j);
+    }
+    const Sums a = group_sums<G, E>(z, e);
+    over_group<G>([&](auto from) { b.add(from(b.v), from(b.j)); });
+    if (g == 0) {
+        const bool some = a.s != 0.0f, found = b.j < K;
+        const float logs = logf(a.s);
+        O.level[r0 + row] = some && found ? b.j : 0;
+        O.logprob[r0 + row] = !some ? 0.0f : found ? mine[b.j] - a.m - logs : __builtin_nanf("");
+        O.entropy[r0 + row] = entropy_of(a, logs);
+    }
+}
+
+template <class T, int G, int E, bool FLAT>
+__global__ __launch_bounds__(256) void group_score_kernel(Rows R, ScoreOut O) {
+    __shared__ float zs[kTile<G, E>];
+    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
+    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels;
+    load_tile<T, G, E, FLAT, false>(R, nullptr, r0, rows, zs, nullptr);
+    const int row = threadIdx.x / G, g = threadIdx.x % G;
+    if (row >= rows) return;
+    const int64_t r = r0 + row;
+    const float* mine = zs + row * (K | 1);
+    const int64_t l = g == 0 ? O.level[r] : 0;
+    float z[E], e[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) z[k] = g + G * k < K ? mine[g + G * k] : kNegInf;
+    const Sums a = group_sums<G, E>(z, e);
+    const float logs = logf(a.s);
+    if (g == 0) {
+        O.logprob[r] = l >= K ? __builtin_nanf("") : l < 0 || a.s == 0.0f ? 0.0f : mine[l] - a.m - logs;
+        O.entropy[r] = entropy_of(a, logs);
+        if (O.stat) { O.stat[2 * r] = a.m; O.stat[2 * r + 1] = a.s; }
+    }
+    for (int n = 0; n < O.top; n++) {           // the best of what is left, O.top times
+        Best b;
+        b.clear();
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (z[k] > kNegInf) b.add(z[k], g + G * k);
+        over_group<G>([&](auto from) { b.add(from(b.v), from(b.j)); });
+#pragma unroll
+        for (int k = 0; k < E; k++)
+            if (g + G * k == b.j) z[k] = kNegInf;
+        if (g == 0) {
+            const bool some = b.j < K;
+            O.top_logprob[r * O.top + n] = some ? b.v - a.m - logs : a.s == a.s ? kNegInf : a.s;
+            O.top_level[r * O.top + n] = some ? b.j : -1;
+        }
+    }
+}
+
+template <class T, int G, int E, bool FLAT>
+__global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T* grad, bool aligned) {
+    __shared__ float zs[kTile<G, E>];
+    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
+    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels, pitch = K | 1;
+    load_tile<T, G, E, FLAT, false>(R, nullptr, r0, rows, zs, nullptr);
+    const int row = threadIdx.x / G, g = threadIdx.x % G;
+    if (row < rows) {
+        const int64_t r = r0 + row;
+        float* mine = zs + row * pitch;
+        const int64_t l = I.level[r];
+        const float gl = I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f, gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f;
+        float z[E], e[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) z[k] = g + G * k < K ? mine[g + G * k] : kNegInf;
+        const Sums a = group_sums<G, E>(z, e);
+        const float logs = logf(a.s), inv = 1.0f / a.s, H = entropy_of(a, logs);
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const int j = g + G * k;
+            const float p = e[k] * inv;
+            float d = (j == l ? gl : 0.0f) - p * (gl + gh * (e[k] > 0.0f ? z[k] - a.m - logs + H : 0.0f));
+            if (z[k] == kNegInf) d = 0.0f;
+            if (l >= K) d = __builtin_nanf("");
+            if (j < K) mine[j] = d;
+        }
+    }
+    __syncthreads();
+    constexpr int VE = 16 / sizeof(T);
+    const int n = rows * K;
+    T* out = grad + r0 * K;
+    for (int e0 = threadIdx.x * VE; e0 < n; e0 += 256 * VE) {
+        int at = __umulhi((uint32_t)e0, R.per_level), col = e0 - at * K;
+        T v[VE];
+#pragma unroll
+        for (int k = 0; k < VE; k++) {
+            v[k] = e0 + k < n ? (T)zs[at * pitch + col] : (T)0.0f;
+            if (++col == K) { col = 0; at++; }
+        }
+        if (aligned && e0 + VE <= n) *reinterpret_cast<uint4*>(out + e0) = *reinterpret_cast<const uint4*>(v);
+        else {
+#pragma unroll
+            for (int k = 0; k < VE; k++)
+                if (e0 + k < n) out[e0 + k] = v[k];
+        }
+    }
+}
+
+// 8 levels to a lane fill the registers of a full set of wavefronts; up to 1024 levels a wavefront is one row.
+constexpr int kGroupLevels = 1024;
+#define BY_LEVELS(K, call)                                                          \
+    do {                                                                            \
+        if ((K) <= 4) { constexpr int G = 1, E = 4; call; }                         \
+        else if ((K) <= 8) { constexpr int G = 1, E = 8; call; }                    \
+        else if ((K) <= 16) { constexpr int G = 2, E = 8; call; }                   \
+        else if ((K) <= 32) { constexpr int G = 4, E = 8; call; }                   \
+        else if ((K) <= 64) { constexpr int G = 8, E = 8; call; }                   \
+        else if ((K) <= 128) { constexpr int G = 16, E = 8; call; }                 \
+        else if ((K) <= 256) { constexpr int G = 32, E = 8; call; }                 \
+        else if ((K) <= 512) { constexpr int G = 64, E = 8; call; }                 \
+        else { constexpr int G = 64, E = 16; call; }                                \
+    } while (0)
+
+int group_rows(int64_t K) { int g = 256; BY_LEVELS(K, (g = 256 / G, (void)E)); return g; }
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Whether the rows (and mask, noise) are one dense run whose tiles start on 16 bytes (the mask's on 8, float32: 4).
+bool flat(const Rows& R, int64_t size, const float* noise, int64_t no, int64_t ni) {
+    const int64_t K = R.levels, per = group_rows(K) * K;
+    const bool one = R.rows == R.inner;
+    auto dense = [&](int64_t o, int64_t i) { return (R.inner == 1 || i == K) && (one || o == K * R.inner); };
+    if (!dense(R.so, R.si) || !aligned16(R.logits) || (per * size) % 16) return false;
+    if (R.mask && (R.mask_level != 1 || !dense(R.mo, R.mi) || ((uintptr_t)R.mask & 7) || per % 8)) return false;
+    return !noise || (dense(no, ni) && aligned16(noise) && per % 4 == 0);
+}
+
 int checked(const lrn_rows* in, Rows* out) {
     if (!in) return fail(-1, "rows: null");
     if (in->outer < 0 || in->inner < 0 || in->levels < 1 || in->levels > 0x3fffffff)
@@ -215,6 +479,15 @@ int checked(const lrn_rows* in, Rows* out) {
     out->mo = in->mask_outer; out->mi = in->mask_inner;
     out->levels = (int32_t)in->levels;
     out->mask_level = in->mask_level;
+    out->per_level = (uint32_t)((0xffffffffull + in->levels) / in->levels);
+    return 0;
+}
+
+int64_t size_of(int dtype) { return dtype == LRN_F32 ? 4 : 2; }
+int tiles(const Rows& R, unsigned* grid) {
+    const int64_t n = cdiv(R.rows, group_rows(R.levels));
+    if (n > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
+    *grid = (unsigned)n;
     return 0;
 }
 
@@ -246,6 +519,17 @@ int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const flo
     if (!level_out || !logprob_out || !entropy_out) return fail(-1, "lrn_choose: null output");
     LRN_ON_DEVICE(device);
     const ChooseOut O{noise, noise_outer, noise_inner, level_out, logprob_out, entropy_out};
+    if (R.levels <= kGroupLevels) {
+        unsigned grid;
+        if (int rc = tiles(R, &grid)) return rc;
+        hipStream_t stream = (hipStream_t)hip_stream;
+        if (flat(R, size_of(rows->dtype), noise, noise_outer, noise_inner))
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, O))))
+        else
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, O))))
+        LRN_LAUNCHED("lrn_choose");
+        return 0;
+    }
     BY_TYPE(rows->dtype, (choose_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, O)));
     LRN_LAUNCHED("lrn_choose");
     return 0;
@@ -262,12 +546,23 @@ int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int6
     if (!level || !logprob_out || !entropy_out || (top && (!top_logprob_out || !top_level_out))) return fail(-1, "lrn_score: null argument");
     LRN_ON_DEVICE(device);
     const ScoreOut O{level, logprob_out, entropy_out, stat_out, top, top_logprob_out, top_level_out};
+    if (R.levels <= kGroupLevels) {
+        unsigned grid;
+        if (int rc = tiles(R, &grid)) return rc;
+        hipStream_t stream = (hipStream_t)hip_stream;
+        if (flat(R, size_of(rows->dtype), nullptr, 0, 0))
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, O))))
+        else
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, O))))
+        LRN_LAUNCHED("lrn_score");
+        return 0;
+    }
     BY_TYPE(rows->dtype, (score_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, O)));
     LRN_LAUNCHED("lrn_score");
     return 0;
 }
 
-int lrn_score_backward_needs_stat(const lrn_rows*) { return 1; }
+int lrn_score_backward_needs_stat(const lrn_rows* rows) { return rows && rows->levels > kGroupLevels; }
 
 int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, const int64_t* level, const float* stat,
                        const float* entropy, const float* g_logprob, int32_t g_logprob_stride, const float* g_entropy,
@@ -275,10 +570,23 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
     Rows R;
     if (int rc = checked(rows, &R)) return rc;
     if (!R.rows) return 0;
-    if (!level || !stat || !entropy || !grad_out) return fail(-1, "lrn_score_backward: null argument");
+    const bool again = R.levels <= kGroupLevels;
+    if (!level || !grad_out || (!again && (!stat || !entropy))) return fail(-1, "lrn_score_backward: null argument");
     if ((g_logprob_stride & ~1) || (g_entropy_stride & ~1)) return fail(-1, "lrn_score_backward: gradient strides are 0 or 1");
     LRN_ON_DEVICE(device);
     const BackIn I{level, stat, entropy, g_logprob, g_entropy, g_logprob_stride, g_entropy_stride};
+    if (again) {
+        unsigned grid;
+        if (int rc = tiles(R, &grid)) return rc;
+        hipStream_t stream = (hipStream_t)hip_stream;
+        const bool out16 = aligned16(grad_out) && (group_rows(R.levels) * (int64_t)R.levels * size_of(rows->dtype)) % 16 == 0;
+        if (flat(R, size_of(rows->dtype), nullptr, 0, 0))
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out, out16))))
+        else
+            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out, out16))))
+        LRN_LAUNCHED("lrn_score_backward");
+        return 0;
+    }
     BY_TYPE(rows->dtype, (score_backward_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, I, (T*)grad_out)));
     LRN_LAUNCHED("lrn_score_backward");
     return 0;
