@@ -3,6 +3,9 @@
 // One pass over a row with the running maximum m, s = sum exp(z - m) and t = sum exp(z - m) (z - m): when the maximum moves
 // from m to m', c = exp(m - m') rescales s' = c s and t' = c (t + s (m - m')).  log s and t / s are all that the log
 // probability and the entropy need.  Sums are float32 whatever the logits' type.
+#include <algorithm>
+#include <type_traits>
+
 #include "lrn_common.h"
 
 namespace lrn {
@@ -26,19 +29,6 @@ struct Rows {
 struct Sums {
     float m, s, t;
     __device__ __forceinline__ void clear() { m = kNegInf; s = 0.0f; t = 0.0f; }
-    // one more logit (not -inf)
-    __device__ __forceinline__ void add(float z) {
-        if (z > m) {
-            const float d = m - z, c = s > 0.0f ? fast_exp(d) : 0.0f;
-            t = s > 0.0f ? c * (t + s * d) : 0.0f;
-            s = c * s + 1.0f;
-            m = z;
-        } else {
-            const float d = z - m, e = fast_exp(d);
-            s += e;
-            t += e > 0.0f ? e * d : (d != d ? d : 0.0f);
-        }
-    }
     // A part without an allowed logit has s = 0 and says nothing; NaN stays NaN.
     __device__ __forceinline__ void join(const Sums& o) {
         if (o.s == 0.0f) return;
@@ -98,18 +88,6 @@ __device__ __forceinline__ const uint8_t* row_mask(const Rows& R, int64_t r) {
     return R.mask + o * R.mo + i * R.mi;
 }
 
-__device__ __forceinline__ void wave_join(Sums& a) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        Sums b{__shfl_xor(a.m, o), __shfl_xor(a.s, o), __shfl_xor(a.t, o)};
-        a.join(b);
-    }
-}
-__device__ __forceinline__ void wave_join(Best& a) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) a.add(__shfl_xor(a.v, o), __shfl_xor(a.j, o));
-}
-
 // +inf among the allowed logits: no distribution
 __device__ __forceinline__ void finish(Sums& a) { if (a.m == -kNegInf) a.s = __builtin_nanf(""); }
 __device__ __forceinline__ float entropy_of(const Sums& a, float logs) { return a.s != 0.0f ? logs - a.t / a.s : 0.0f; }
@@ -117,97 +95,7 @@ __device__ __forceinline__ float entropy_of(const Sums& a, float logs) { return 
 struct ChooseOut { const float* noise; int64_t no, ni; int64_t* level; float* logprob; float* entropy; };
 struct ScoreOut { const int64_t* level; float* logprob; float* entropy; float* stat; int top; float* top_logprob; int64_t* top_level; };
 
-// A wavefront to a row.
-template <class T>
-__global__ __launch_bounds__(256) void choose_kernel(Rows R, ChooseOut O) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R.rows; r += (int64_t)gridDim.x * 4) {
-        const T* z = (const T*)R.logits + row_base(R, r);
-        const uint8_t* mk = row_mask(R, r);
-        const float* nz = O.noise ? O.noise + (r / R.inner) * O.no + (r % R.inner) * O.ni : nullptr;
-        Sums a; a.clear();
-        Best b; b.clear();
-        float zb = 0.0f;
-        for (int j = lane; j < R.levels; j += 64) {
-            const float v = mk && !mk[(int64_t)j * R.mask_level] ? kNegInf : to_f32(z[j]);
-            if (v == kNegInf) continue;
-            a.add(v);
-            b.add(nz ? v + nz[j] : v, j);
-        }
-        wave_join(a);
-        wave_join(b);
-        finish(a);
-        if (lane == 0) {
-            const bool some = a.s != 0.0f;
-            const int at = b.j < R.levels ? b.j : 0;
-            const float logs = logf(a.s);
-            zb = to_f32(z[at]);
-            O.level[r] = some ? at : 0;
-            O.logprob[r] = some ? (b.j < R.levels ? zb - a.m - logs : __builtin_nanf("")) : 0.0f;
-            O.entropy[r] = entropy_of(a, logs);
-        }
-    }
-}
-
-template <class T>
-__global__ __launch_bounds__(256) void score_kernel(Rows R, ScoreOut O) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R.rows; r += (int64_t)gridDim.x * 4) {
-        const T* z = (const T*)R.logits + row_base(R, r);
-        const uint8_t* mk = row_mask(R, r);
-        Sums a; a.clear();
-        TopList list; list.clear();
-        for (int j0 = 0; j0 < R.levels; j0 += 64) {
-            const int j = j0 + lane;
-            float v = kNegInf;
-            if (j < R.levels && !(mk && !mk[(int64_t)j * R.mask_level])) v = to_f32(z[j]);
-            if (v != kNegInf) a.add(v);
-            if (O.top) list.offer(v, j, O.top, lane);
-        }
-        wave_join(a);
-        finish(a);
-        const float logs = logf(a.s);
-        if (lane == 0) {
-            const int64_t l = O.level[r];
-            float lp = 0.0f;
-            if (l >= R.levels) lp = __builtin_nanf("");
-            else if (l >= 0 && a.s != 0.0f) lp = (mk && !mk[l * R.mask_level]) ? kNegInf + 0.0f * a.s : to_f32(z[l]) - a.m - logs;
-            O.logprob[r] = lp;
-            O.entropy[r] = entropy_of(a, logs);
-            if (O.stat) { O.stat[2 * r] = a.m; O.stat[2 * r + 1] = a.s; }
-        }
-        if (lane < O.top) {
-            const bool some = list.v > kNegInf;
-            O.top_logprob[r * O.top + lane] = some ? list.v - a.m - logs : (a.s == a.s ? kNegInf : a.s);
-            O.top_level[r * O.top + lane] = some ? list.j : -1;
-        }
-    }
-}
-
 struct BackIn { const int64_t* level; const float* stat; const float* entropy; const float* g_lp; const float* g_h; int g_lp_stride, g_h_stride; };
-
-template <class T>
-__global__ __launch_bounds__(256) void score_backward_kernel(Rows R, BackIn I, T* grad) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < R.rows; r += (int64_t)gridDim.x * 4) {
-        const T* z = (const T*)R.logits + row_base(R, r);
-        const uint8_t* mk = row_mask(R, r);
-        const float m = I.stat[2 * r], s = I.stat[2 * r + 1], H = I.entropy[r];
-        const int64_t l = I.level[r];
-        const float g = I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f, gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f;
-        const float logs = logf(s), inv = 1.0f / s;
-        for (int j = lane; j < R.levels; j += 64) {
-            const float v = mk && !mk[(int64_t)j * R.mask_level] ? kNegInf : to_f32(z[j]);
-            float d = 0.0f;
-            if (v != kNegInf && s != 0.0f) {
-                const float e = fast_exp(v - m), p = e * inv;
-                d = (j == l ? g : 0.0f) - p * (g + gh * (e > 0.0f ? v - m - logs + H : 0.0f));
-                if (l >= R.levels) d = __builtin_nanf("");
-            }
-            grad[r * R.levels + j] = (T)d;
-        }
-    }
-}
 
 // ---- rows of up to 1024 levels: G lanes to a row -----------------------------------------------------------------------
 //
@@ -464,6 +352,259 @@ bool flat(const Rows& R, int64_t size, const float* noise, int64_t no, int64_t n
     return !noise || (dense(no, ni) && aligned16(noise) && per % 4 == 0);
 }
 
+// ---- longer rows: a workgroup to a row, or to a part of one -----------------------------------------------------------
+//
+// Every lane walks 16-byte pieces of the row (at any alignment: the hardware takes a vector load at its element's) with a
+// running maximum and sums of its own, rescaled when a piece raises the maximum; the lanes join at the end.  Where there are
+// too few rows to fill the GPU a row is cut into up to 64 parts, whose sums, best level and best alternatives go through the
+// workspace to a second launch, a wavefront to a row.
+
+template <class T> struct Piece {
+    static constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+struct Mask8 { typedef uint8_t vec __attribute__((ext_vector_type(8), aligned(1))); };
+struct Mask4 { typedef uint8_t vec __attribute__((ext_vector_type(4), aligned(1))); };
+
+// The levels e0 .. of a row into z (-inf where masked or behind `end`).
+template <class T, int N = Piece<T>::N>
+__device__ __forceinline__ void load_piece(const T* src, const uint8_t* mk, int mask_level, int e0, int end, float (&z)[N]) {
+    if (e0 + N <= end) {
+        const typename Piece<T>::vec v = *reinterpret_cast<const typename Piece<T>::vec*>(src + e0);
+#pragma unroll
+        for (int k = 0; k < N; k++) z[k] = to_f32(v[k]);
+        if (mk && mask_level) {
+            using M = std::conditional_t<N == 8, Mask8, Mask4>;
+            const typename M::vec b = *reinterpret_cast<const typename M::vec*>(mk + e0);
+#pragma unroll
+            for (int k = 0; k < N; k++) z[k] = b[k] ? z[k] : kNegInf;
+        } else if (mk) {
+            const bool on = mk[0];
+#pragma unroll
+            for (int k = 0; k < N; k++) z[k] = on ? z[k] : kNegInf;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k++) z[k] = e0 + k < end && !(mk && !mk[(e0 + k) * (int64_t)mask_level]) ? to_f32(src[e0 + k]) : kNegInf;
+    }
+}
+
+template <int N> __device__ __forceinline__ void add_piece(Sums& a, const float (&z)[N]) {
+    float top = z[0];
+#pragma unroll
+    for (int k = 1; k < N; k++) top = fmaxf(top, z[k]);
+    if (top > a.m) {
+        const float d = a.m - top, c = fast_exp(d);              // a.m = -inf: c = 0, and s = t = 0
+        a.t = c > 0.0f ? c * (a.t + a.s * d) : 0.0f;
+        a.s = c * a.s;
+        a.m = top;
+    }
+    if (a.m == kNegInf) {                                        // nothing allowed so far, or NaN
+#pragma unroll
+        for (int k = 0; k < N; k++)
+            if (z[k] != z[k]) a.s = z[k];
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const float d = z[k] - a.m, e = fast_exp(d);
+        a.s += e;
+        a.t += e * fmaxf(d, -3.0e38f);                           // a masked level: 0 times a number
+    }
+}
+
+__device__ __forceinline__ void wave_join(Sums& a) {
+    over_group<64>([&](auto from) { a.join(Sums{from(a.m), from(a.s), from(a.t)}); });
+}
+
+struct Part { float m, s, t, v; int j; };
+
+struct Cut {
+    int parts, length;           // levels of a part
+    Part* part;                  // [rows][parts], parts > 1
+    float* top_v;                // [rows][parts][top]
+    int* top_j;
+};
+
+// The row's outputs, from its joined sums; called by one whole wavefront.
+template <class T> __device__ __forceinline__ void put_choice(const Rows& R, const ChooseOut& O, int64_t r, const Sums& a, const Best& b, int lane) {
+    if (lane) return;
+    const bool some = a.s != 0.0f, found = b.j < R.levels;
+    const float logs = logf(a.s);
+    O.level[r] = some && found ? b.j : 0;
+    O.logprob[r] = !some ? 0.0f : found ? to_f32(((const T*)R.logits + row_base(R, r))[b.j]) - a.m - logs : __builtin_nanf("");
+    O.entropy[r] = entropy_of(a, logs);
+}
+template <class T> __device__ __forceinline__ void put_score(const Rows& R, const ScoreOut& O, int64_t r, const Sums& a, const TopList& list, int lane) {
+    const float logs = logf(a.s);
+    if (lane == 0) {
+        const int64_t l = O.level[r];
+        float lp = 0.0f;
+        if (l >= R.levels) lp = __builtin_nanf("");
+        else if (l >= 0 && a.s != 0.0f) {
+            const uint8_t* mk = row_mask(R, r);
+            lp = (mk && !mk[l * R.mask_level] ? kNegInf : to_f32(((const T*)R.logits + row_base(R, r))[l])) - a.m - logs;
+        }
+        O.logprob[r] = lp;
+        O.entropy[r] = entropy_of(a, logs);
+        if (O.stat) { O.stat[2 * r] = a.m; O.stat[2 * r + 1] = a.s; }
+    }
+    if (lane < O.top) {
+        const bool some = list.v > kNegInf;
+        O.top_logprob[r * O.top + lane] = some ? list.v - a.m - logs : a.s == a.s ? kNegInf : a.s;
+        O.top_level[r * O.top + lane] = some ? list.j : -1;
+    }
+}
+
+template <class T, bool CHOOSE>
+__global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut O, Cut cut) {
+    constexpr int N = Piece<T>::N;
+    __shared__ Part waves[4];
+    __shared__ float list_v[3 * LRN_MAX_TOP];
+    __shared__ int list_j[3 * LRN_MAX_TOP];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = cut.parts > 1 ? (int64_t)blockIdx.x / cut.parts : blockIdx.x;
+    const int p = cut.parts > 1 ? (int)(blockIdx.x - r * cut.parts) : 0;
+    const int begin = p * cut.length, end = min(begin + cut.length, R.levels);
+    int64_t o, i;
+    split(R, r, o, i);
+    const T* src = (const T*)R.logits + o * R.so + i * R.si;
+    const uint8_t* mk = R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
+    const float* ns = CHOOSE && C.noise ? C.noise + o * C.no + i * C.ni : nullptr;
+    Sums a;
+    a.clear();
+    Best b;
+    b.clear();
+    TopList list;
+    list.clear();
+    const int top = CHOOSE ? 0 : O.top;
+    // all lanes of a wavefront go round together: the list of alternatives is the wavefront's
+    for (int e0 = begin + tid * N; e0 - lane * N < end; e0 += 256 * N) {
+        float z[N];
+        load_piece<T>(src, mk, R.mask_level, e0, end, z);
+        add_piece(a, z);
+        if constexpr (CHOOSE) {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (z[k] != kNegInf) b.add(ns ? z[k] + ns[e0 + k] : z[k], e0 + k);
+        } else if (top) {
+            float best = z[0];
+#pragma unroll
+            for (int k = 1; k < N; k++) best = fmaxf(best, z[k]);
+            if (__ballot(best >= __shfl(list.v, top - 1) && best > kNegInf)) {
+#pragma unroll
+                for (int k = 0; k < N; k++) list.offer(z[k], e0 + k, top, lane);
+            }
+        }
+    }
+    wave_join(a);
+    if constexpr (CHOOSE) over_group<64>([&](auto from) { b.add(from(b.v), from(b.j)); });
+    if (lane == 0) waves[wave] = Part{a.m, a.s, a.t, b.v, b.j};
+    if (top && wave && lane < top) { list_v[(wave - 1) * LRN_MAX_TOP + lane] = list.v; list_j[(wave - 1) * LRN_MAX_TOP + lane] = list.j; }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < 4; w++) {
+        a.join(Sums{waves[w].m, waves[w].s, waves[w].t});
+        if constexpr (CHOOSE) b.add(waves[w].v, waves[w].j);
+        else if (top) list.offer(lane < top ? list_v[(w - 1) * LRN_MAX_TOP + lane] : kNegInf, lane < top ? list_j[(w - 1) * LRN_MAX_TOP + lane] : 0, top, lane);
+    }
+    if (cut.parts == 1) {
+        finish(a);
+        if constexpr (CHOOSE) put_choice<T>(R, C, r, a, b, lane);
+        else put_score<T>(R, O, r, a, list, lane);
+    } else {
+        if (lane == 0) cut.part[blockIdx.x] = Part{a.m, a.s, a.t, b.v, b.j};
+        if (lane < top) { cut.top_v[(int64_t)blockIdx.x * top + lane] = list.v; cut.top_j[(int64_t)blockIdx.x * top + lane] = list.j; }
+    }
+}
+
+template <class T, bool CHOOSE>
+__global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut O, Cut cut) {
+    const int lane = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    Part mine{kNegInf, 0.0f, 0.0f, kNegInf, 0x7fffffff};
+    if (lane < cut.parts) mine = cut.part[r * cut.parts + lane];
+    Sums a{mine.m, mine.s, mine.t};
+    Best b{mine.v, mine.j};
+    TopList list;
+    list.clear();
+    wave_join(a);
+    finish(a);
+    if constexpr (CHOOSE) {
+        over_group<64>([&](auto from) { b.add(from(b.v), from(b.j)); });
+        put_choice<T>(R, C, r, a, b, lane);
+    } else {
+        const int top = O.top, n = cut.parts * top;
+        for (int k0 = 0; k0 < n; k0 += 64) {
+            const int k = k0 + lane;
+            list.offer(k < n ? cut.top_v[r * n + k] : kNegInf, k < n ? cut.top_j[r * n + k] : 0, top, lane);
+        }
+        put_score<T>(R, O, r, a, list, lane);
+    }
+}
+
+// One piece of 16 bytes after the other, with the row's statistics: bound by memory.
+constexpr int kBackPieces = 4;       // pieces a lane
+template <class T>
+__global__ __launch_bounds__(256) void wide_backward_kernel(Rows R, BackIn I, T* grad, int parts) {
+    constexpr int N = Piece<T>::N;
+    const int64_t r = blockIdx.x / (unsigned)parts;
+    const int begin = (int)(blockIdx.x - r * parts) * (256 * N * kBackPieces), end = min(begin + 256 * N * kBackPieces, R.levels);
+    int64_t o, i;
+    split(R, r, o, i);
+    const T* src = (const T*)R.logits + o * R.so + i * R.si;
+    const uint8_t* mk = R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
+    T* out = grad + r * R.levels;
+    const float m = I.stat[2 * r], s = I.stat[2 * r + 1], H = I.entropy[r];
+    const int64_t l = I.level[r];
+    float g = I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f;
+    const float gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f, inv = s != 0.0f ? 1.0f / s : 0.0f;
+    const float lift = s != 0.0f ? H - logf(s) : 0.0f;           // log p + H = z - m + lift
+    if (l >= R.levels) g = __builtin_nanf("");
+#pragma unroll
+    for (int n = 0; n < kBackPieces; n++) {
+        const int e0 = begin + (n * 256 + (int)threadIdx.x) * N;
+        if (e0 >= end) return;
+        float z[N];
+        load_piece<T>(src, mk, R.mask_level, e0, end, z);
+        typename Piece<T>::vec v;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float w = z[k] - m, e = fast_exp(w), p = e * inv;
+            float d = -p * (g + gh * (e > 0.0f ? w + lift : 0.0f));
+            if (e0 + k == l) d += g;
+            v[k] = (T)(z[k] == kNegInf ? 0.0f : d);
+        }
+        if (e0 + N <= end) *reinterpret_cast<typename Piece<T>::vec*>(out + e0) = v;
+        else {
+#pragma unroll
+            for (int k = 0; k < N; k++)
+                if (e0 + k < end) out[e0 + k] = v[k];
+        }
+    }
+}
+
+// Parts of a row: enough workgroups for four a compute unit, parts of 4096 levels at least (a part's fixed cost, its joins, is
+// about that of 2000 levels), at most one for each lane of the joining wavefront.
+Cut cut_of(const Rows& R, int top, void* workspace) {
+    Cut c{};
+    int64_t parts = std::min<int64_t>({cdiv(1024, R.rows), cdiv(R.levels, 4096), 64});
+    c.length = (int)(cdiv(cdiv(R.levels, parts), 2048) * 2048);
+    c.parts = (int)cdiv(R.levels, c.length);
+    if (c.parts > 1) {
+        c.part = (Part*)workspace;
+        c.top_v = (float*)(c.part + R.rows * c.parts);
+        c.top_j = (int*)(c.top_v + R.rows * c.parts * top);
+    }
+    return c;
+}
+int64_t cut_bytes(const Rows& R, int top) {
+    if (R.levels <= kGroupLevels || R.rows <= 0) return 0;
+    const Cut c = cut_of(R, top, nullptr);
+    return c.parts > 1 ? R.rows * c.parts * (int64_t)(sizeof(Part) + 8 * top) : 0;
+}
+
 int checked(const lrn_rows* in, Rows* out) {
     if (!in) return fail(-1, "rows: null");
     if (in->outer < 0 || in->inner < 0 || in->levels < 1 || in->levels > 0x3fffffff)
@@ -491,7 +632,19 @@ int tiles(const Rows& R, unsigned* grid) {
     return 0;
 }
 
-unsigned grid_for(int64_t rows) { const int64_t g = cdiv(rows, 4); return (unsigned)(g < 65536 ? g : 65536); }
+int check_workspace(int64_t need, const void* workspace, int64_t bytes, const char* who) {
+    if (need && (!workspace || bytes < need)) return fail(-1, "%s: a workspace of %lld bytes is needed, got %lld", who, (long long)need, (long long)bytes);
+    return 0;
+}
+
+template <class T, bool CHOOSE> int launch_wide(const Rows& R, const ChooseOut& C, const ScoreOut& O, int top, void* workspace, hipStream_t stream, const char* who) {
+    const Cut cut = cut_of(R, top, workspace);
+    if (R.rows * cut.parts > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
+    wide_kernel<T, CHOOSE><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
+    if (cut.parts > 1) join_kernel<T, CHOOSE><<<(unsigned)R.rows, 64, 0, stream>>>(R, C, O, cut);
+    LRN_LAUNCHED(who);
+    return 0;
+}
 
 }  // namespace
 }  // namespace lrn
@@ -509,14 +662,18 @@ extern "C" {
 
 const char* lrn_last_error(void) { return error_text(); }
 
-int64_t lrn_choose_workspace(const lrn_rows*) { return 0; }
+int64_t lrn_choose_workspace(const lrn_rows* rows) {
+    Rows R;
+    return rows && checked(rows, &R) == 0 ? cut_bytes(R, 0) : 0;
+}
 
 int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const float* noise, int64_t noise_outer,
-               int64_t noise_inner, int64_t* level_out, float* logprob_out, float* entropy_out, void*, int64_t) {
+               int64_t noise_inner, int64_t* level_out, float* logprob_out, float* entropy_out, void* workspace, int64_t workspace_bytes) {
     Rows R;
     if (int rc = checked(rows, &R)) return rc;
     if (!R.rows) return 0;
     if (!level_out || !logprob_out || !entropy_out) return fail(-1, "lrn_choose: null output");
+    if (int rc = check_workspace(cut_bytes(R, 0), workspace, workspace_bytes, "lrn_choose")) return rc;
     LRN_ON_DEVICE(device);
     const ChooseOut O{noise, noise_outer, noise_inner, level_out, logprob_out, entropy_out};
     if (R.levels <= kGroupLevels) {
@@ -530,20 +687,23 @@ int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const flo
         LRN_LAUNCHED("lrn_choose");
         return 0;
     }
-    BY_TYPE(rows->dtype, (choose_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, O)));
-    LRN_LAUNCHED("lrn_choose");
-    return 0;
+    BY_TYPE(rows->dtype, return (launch_wide<T, true>(R, O, ScoreOut{}, 0, workspace, (hipStream_t)hip_stream, "lrn_choose")));
 }
 
-int64_t lrn_score_workspace(const lrn_rows*, int32_t) { return 0; }
+int64_t lrn_score_workspace(const lrn_rows* rows, int32_t top) {
+    Rows R;
+    return rows && top >= 0 && top <= LRN_MAX_TOP && checked(rows, &R) == 0 ? cut_bytes(R, top) : 0;
+}
 
 int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int64_t* level, float* logprob_out,
-              float* entropy_out, float* stat_out, int32_t top, float* top_logprob_out, int64_t* top_level_out, void*, int64_t) {
+              float* entropy_out, float* stat_out, int32_t top, float* top_logprob_out, int64_t* top_level_out, void* workspace,
+              int64_t workspace_bytes) {
     Rows R;
     if (int rc = checked(rows, &R)) return rc;
     if (top < 0 || top > LRN_MAX_TOP || top > R.levels) return fail(-1, "lrn_score: top %d of %d levels (at most %d)", top, R.levels, LRN_MAX_TOP);
     if (!R.rows) return 0;
     if (!level || !logprob_out || !entropy_out || (top && (!top_logprob_out || !top_level_out))) return fail(-1, "lrn_score: null argument");
+    if (int rc = check_workspace(cut_bytes(R, top), workspace, workspace_bytes, "lrn_score")) return rc;
     LRN_ON_DEVICE(device);
     const ScoreOut O{level, logprob_out, entropy_out, stat_out, top, top_logprob_out, top_level_out};
     if (R.levels <= kGroupLevels) {
@@ -557,9 +717,7 @@ int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int6
         LRN_LAUNCHED("lrn_score");
         return 0;
     }
-    BY_TYPE(rows->dtype, (score_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, O)));
-    LRN_LAUNCHED("lrn_score");
-    return 0;
+    BY_TYPE(rows->dtype, return (launch_wide<T, false>(R, ChooseOut{}, O, top, workspace, (hipStream_t)hip_stream, "lrn_score")));
 }
 
 int lrn_score_backward_needs_stat(const lrn_rows* rows) { return rows && rows->levels > kGroupLevels; }
@@ -587,7 +745,9 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
         LRN_LAUNCHED("lrn_score_backward");
         return 0;
     }
-    BY_TYPE(rows->dtype, (score_backward_kernel<T><<<grid_for(R.rows), 256, 0, (hipStream_t)hip_stream>>>(R, I, (T*)grad_out)));
+    const int64_t parts = cdiv(R.levels, 256 * kBackPieces * 16 / size_of(rows->dtype));
+    if (R.rows * parts > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
+    BY_TYPE(rows->dtype, (wide_backward_kernel<T><<<(unsigned)(R.rows * parts), 256, 0, (hipStream_t)hip_stream>>>(R, I, (T*)grad_out, (int)parts)));
     LRN_LAUNCHED("lrn_score_backward");
     return 0;
 }

@@ -66,7 +66,8 @@ def _on_device(name: str, t, device=None) -> None:
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream's handle (``torch.cuda.current_stream(device).cuda_stream`` without the object: 0.1 us instead of 2)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _workspace(nbytes: int, device):
