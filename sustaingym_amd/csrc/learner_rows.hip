@@ -48,32 +48,56 @@ struct Best {
     __device__ __forceinline__ void add(float x, int i) { if (x > v || (x == v && i < j)) { v = x; j = i; } }
 };
 
-// The 64 best of what a wavefront has seen, lane i the i-th (falling, the lowest index first among equals).
+__device__ __forceinline__ float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// The 64 best of what a wavefront has seen, lane i the i-th (falling, the lowest index first among equals).  Candidates go in
+// one at a time: k (1 + log(n / k)) of n values do.  What an insertion costs is latency, so nothing in it goes through LDS: the
+// candidate and the bound are scalars (v_readlane), the entries behind it move up by one lane with a whole-wavefront shift.
 struct TopList {
     float v;
     int j;
-    __device__ __forceinline__ void clear() { v = kNegInf; j = 0x7fffffff; }
-    __device__ __forceinline__ void insert(float x, int i, int lane) {
-        const bool ahead = v > x || (v == x && j < i);
-        const int at = __popcll(__ballot(ahead));
-        const float pv = __shfl_up(v, 1);
-        const int pj = __shfl_up(j, 1);
-        if (lane > at) { v = pv; j = pj; }
-        if (lane == at) { v = x; j = i; }
-    }
-    // every lane offers one candidate; only those ahead of the top-th entry are put in, one after the other
+    float floor;                 // `top` values of at least this are known to come
+    float bound;                 // what a candidate has to be ahead of: the top-th entry, or the floor until there is one
+    int bound_j;
+    __device__ __forceinline__ void clear(float at_least = kNegInf) { v = kNegInf; bound = floor = at_least; j = bound_j = 0x7fffffff; }
+    // every lane offers one candidate (-inf: none)
     __device__ __forceinline__ void offer(float x, int i, int top, int lane) {
         for (;;) {
-            const float bound = __shfl(v, top - 1);
-            const int bound_j = __shfl(j, top - 1);
             const unsigned long long some = __ballot(x > bound || (x == bound && x > kNegInf && i < bound_j));
             if (!some) return;
             const int src = __ffsll((long long)some) - 1;
-            insert(__shfl(x, src), __shfl(i, src), lane);
+            const float cv = lane_of(x, src);
+            const int cj = lane_of(i, src);
+            const int at = __popcll(__ballot(v > cv || (v == cv && j < cj)));
+            const float pv = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x138, 0xf, 0xf, true));
+            const int pj = __builtin_amdgcn_update_dpp(0, j, 0x138, 0xf, 0xf, true);
+            v = lane > at ? pv : lane == at ? cv : v;
+            j = lane > at ? pj : lane == at ? cj : j;
+            const float last = lane_of(v, top - 1);
+            if (last >= floor) { bound = last; bound_j = lane_of(j, top - 1); }
             if (lane == src) x = kNegInf;
         }
     }
 };
+
+// The `count`-th largest of 256 values (four a lane) by halving the ordered bit patterns.
+__device__ __forceinline__ float nth_of_256(const float (&v)[4], int count) {
+    uint32_t key[4], at = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, v[k]);
+        key[k] = u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
+    }
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        const uint32_t t = at | bit;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) n += __popcll(__ballot(key[k] >= t));
+        if (n >= count) at = t;
+    }
+    return __builtin_bit_cast(float, at & 0x80000000u ? at ^ 0x80000000u : ~at);
+}
 
 // row r = (o, i)
 __device__ __forceinline__ void split(const Rows& R, int64_t r, int64_t& o, int64_t& i) {
@@ -389,6 +413,44 @@ __device__ __forceinline__ void load_piece(const T* src, const uint8_t* mk, int 
     }
 }
 
+// f(z, e0) for every piece of a lane; kAhead pieces are asked for before the first is used.
+constexpr int kAhead = 4;
+template <class T, bool MASK, class F>
+__device__ __forceinline__ void over_pieces(const T* src, const uint8_t* mk, int mask_level, int begin, int end, F&& f) {
+    constexpr int N = Piece<T>::N, STEP = 256 * N;
+    using V = typename Piece<T>::vec;
+    using M = typename std::conditional_t<N == 8, Mask8, Mask4>::vec;
+    int base = begin;
+    for (; base + kAhead * STEP <= end; base += kAhead * STEP) {
+        const int e0 = base + (int)threadIdx.x * N;
+        V v[kAhead];
+        M b[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) v[u] = *reinterpret_cast<const V*>(src + e0 + u * STEP);
+        if (MASK && mask_level) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) b[u] = *reinterpret_cast<const M*>(mk + e0 + u * STEP);
+        } else if (MASK) {
+            const uint8_t on = mk[0];
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) b[u] = on;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; u++) {
+            float z[N];
+#pragma unroll
+            for (int k = 0; k < N; k++) z[k] = !MASK || b[u][k] ? to_f32(v[u][k]) : kNegInf;
+            f(z, e0 + u * STEP);
+        }
+    }
+    for (; base < end; base += STEP) {
+        const int e0 = base + (int)threadIdx.x * N;
+        float z[N];
+        load_piece<T>(src, mk, mask_level, e0, end, z);
+        f(z, e0);
+    }
+}
+
 template <int N> __device__ __forceinline__ void add_piece(Sums& a, const float (&z)[N]) {
     float top = z[0];
 #pragma unroll
@@ -456,10 +518,11 @@ template <class T> __device__ __forceinline__ void put_score(const Rows& R, cons
     }
 }
 
-template <class T, bool CHOOSE>
+template <class T, bool CHOOSE, bool MASK>
 __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut O, Cut cut) {
     constexpr int N = Piece<T>::N;
     __shared__ Part waves[4];
+    __shared__ float maxima[256];
     __shared__ float list_v[3 * LRN_MAX_TOP];
     __shared__ int list_j[3 * LRN_MAX_TOP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -469,7 +532,7 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
     int64_t o, i;
     split(R, r, o, i);
     const T* src = (const T*)R.logits + o * R.so + i * R.si;
-    const uint8_t* mk = R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
+    const uint8_t* mk = MASK ? R.mask + o * R.mo + i * R.mi : nullptr;
     const float* ns = CHOOSE && C.noise ? C.noise + o * C.no + i * C.ni : nullptr;
     Sums a;
     a.clear();
@@ -478,24 +541,29 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
     TopList list;
     list.clear();
     const int top = CHOOSE ? 0 : O.top;
-    // all lanes of a wavefront go round together: the list of alternatives is the wavefront's
-    for (int e0 = begin + tid * N; e0 - lane * N < end; e0 += 256 * N) {
-        float z[N];
-        load_piece<T>(src, mk, R.mask_level, e0, end, z);
+    over_pieces<T, MASK>(src, mk, R.mask_level, begin, end, [&](const float (&z)[N], int e0) {
         add_piece(a, z);
         if constexpr (CHOOSE) {
 #pragma unroll
             for (int k = 0; k < N; k++)
                 if (z[k] != kNegInf) b.add(ns ? z[k] + ns[e0 + k] : z[k], e0 + k);
-        } else if (top) {
+        }
+    });
+    if (top) {
+        // The top-th largest of the 256 lanes' maxima is at most the row's: a second walk (the part is in the caches) has
+        // little more than `top` candidates left to put in order.
+        maxima[tid] = a.m;
+        __syncthreads();
+        list.clear(nth_of_256({maxima[lane], maxima[lane + 64], maxima[lane + 128], maxima[lane + 192]}, top));
+        over_pieces<T, MASK>(src, mk, R.mask_level, begin, end, [&](const float (&z)[N], int e0) {      // (whole wavefronts)
             float best = z[0];
 #pragma unroll
             for (int k = 1; k < N; k++) best = fmaxf(best, z[k]);
-            if (__ballot(best >= __shfl(list.v, top - 1) && best > kNegInf)) {
+            if (__ballot(best >= list.bound && best > kNegInf)) {
 #pragma unroll
                 for (int k = 0; k < N; k++) list.offer(z[k], e0 + k, top, lane);
             }
-        }
+        });
     }
     wave_join(a);
     if constexpr (CHOOSE) over_group<64>([&](auto from) { b.add(from(b.v), from(b.j)); });
@@ -535,10 +603,23 @@ __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut 
         over_group<64>([&](auto from) { b.add(from(b.v), from(b.j)); });
         put_choice<T>(R, C, r, a, b, lane);
     } else {
+        // The parts' best first, then their second best, ...: 64 candidates hold one of each part, and where none of them
+        // gets in, nothing that follows does.
         const int top = O.top, n = cut.parts * top;
+        auto fetch = [&](int k, float& v, int& j) {
+            const int64_t from = r * n + (k % cut.parts) * top + k / cut.parts;
+            v = k < n ? cut.top_v[from] : kNegInf;
+            j = k < n ? cut.top_j[from] : 0x7fffffff;
+        };
+        float v, next_v;
+        int j, next_j;
+        fetch(lane, next_v, next_j);
         for (int k0 = 0; k0 < n; k0 += 64) {
-            const int k = k0 + lane;
-            list.offer(k < n ? cut.top_v[r * n + k] : kNegInf, k < n ? cut.top_j[r * n + k] : 0, top, lane);
+            v = next_v;
+            j = next_j;
+            if (!__ballot(v > list.bound || (v == list.bound && v > kNegInf && j < list.bound_j))) break;
+            fetch(k0 + 64 + lane, next_v, next_j);
+            list.offer(v, j, top, lane);
         }
         put_score<T>(R, O, r, a, list, lane);
     }
@@ -640,7 +721,8 @@ int check_workspace(int64_t need, const void* workspace, int64_t bytes, const ch
 template <class T, bool CHOOSE> int launch_wide(const Rows& R, const ChooseOut& C, const ScoreOut& O, int top, void* workspace, hipStream_t stream, const char* who) {
     const Cut cut = cut_of(R, top, workspace);
     if (R.rows * cut.parts > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
-    wide_kernel<T, CHOOSE><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
+    if (R.mask) wide_kernel<T, CHOOSE, true><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
+    else wide_kernel<T, CHOOSE, false><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
     if (cut.parts > 1) join_kernel<T, CHOOSE><<<(unsigned)R.rows, 64, 0, stream>>>(R, C, O, cut);
     LRN_LAUNCHED(who);
     return 0;
