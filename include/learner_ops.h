@@ -77,7 +77,7 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
  * lrn_scan:  h_t = a_t h_{t-1} + x_t,  t = 0 .. steps-1  (reverse: from the last step to the first; "before" and "last"
  * below are meant in that order).  a_t = gate_t (the type of x, or gate_const where gate is NULL), and exactly 0 where
  * resets (bytes, (time, batch) strides, NULL = none) says that the sequence starts anew: nothing of what came before
- * enters, not even a NaN.  initial [batch][channels] contiguous (NULL = 0) is the state before the first step; final
+ * enters, not even a NaN (nor does it where the gate itself is exactly 0).  initial [batch][channels] contiguous (NULL = 0) is the state before the first step; final
  * (NULL = not wanted) receives the last one.  initial / final are float32, float64 for LRN_F64; the state is carried in
  * those types whatever the type of x and h.  h may not overlap an input.
  */
@@ -106,12 +106,12 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
 /* Generalised advantages of `steps` x `batch` (channels = 1, reverse ignored):
  *   d_t = r_t + gamma (1 - end_t) V_{t+1} - V_t,  A_t = d_t + gamma lam (1 - end_t) A_{t+1},  target_t = A_t + V_t
  * rewards: float64 or float32 (seq->dtype LRN_F64 / LRN_F32), values float32, ends bytes (non-zero: the episode ended with
- * this step), last_values [batch] float32 contiguous = V behind the last step.  Outputs float32, contiguous
- * [steps][batch].  The arithmetic is float64 for float64 rewards. */
+ * this step), last_values [batch] float32 contiguous = V behind the last step.  Outputs float32.  The arithmetic is float64
+ * for float64 rewards. */
 int64_t lrn_advantages_workspace(const lrn_seq* seq);
 int lrn_advantages(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* rewards, const lrn_view* values,
-                   const lrn_view* ends, const float* last_values, double gamma, double lam, float* advantage_out,
-                   float* target_out, void* workspace, int64_t workspace_bytes);
+                   const lrn_view* ends, const float* last_values, double gamma, double lam, const lrn_view* advantage_out,
+                   const lrn_view* target_out, void* workspace, int64_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -291,9 +291,20 @@ def _state_type(dtype):
     return torch.float64 if dtype == torch.float64 else torch.float32
 
 
+def _laid_out(shape, stride, dtype, device):
+    """An output in the layout of the input with these strides (a batch-major trajectory stays one); contiguous where that one
+    has holes or overlaps."""
+    expect = 1
+    for s, n in sorted((s, n) for n, s in zip(shape, stride) if n != 1):
+        if s != expect or n == 0:
+            return torch.empty(shape, dtype=dtype, device=device)
+        expect *= n
+    return torch.empty_strided(shape, stride, dtype=dtype, device=device)
+
+
 def _scan(x, gate, gate_const, initial, resets, dim, reverse):
     lib, device = _lib.load(), x.device
-    h = torch.empty(x.shape, dtype=x.dtype, device=device)
+    h = _laid_out(x.shape, x.stride(), x.dtype, device)
     final = torch.empty([n for i, n in enumerate(x.shape) if i != dim], dtype=_state_type(x.dtype), device=device)
     seq = _sequence(x.shape, dim, reverse, x.dtype)
     ref = C.byref(seq)
@@ -312,7 +323,7 @@ class _GatedScan(torch.autograd.Function):
         # The gate's gradient needs the states; where they were rounded to 16 bits, so is their share of it (half a step of h),
         # for what reading x and walking forward again would cost.
         ctx.save_for_backward(gate, resets, initial, h if ctx.needs_input_grad[1] else None)
-        ctx.args = (gate_const, dim, reverse, x.shape, x.dtype, x.device)
+        ctx.args = (gate_const, dim, reverse, x.shape, x.stride(), x.dtype, x.device)
         ctx.set_materialize_grads(False)
         return h, final
 
@@ -320,14 +331,14 @@ class _GatedScan(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, g_h, g_final):
         gate, resets, initial, h = ctx.saved_tensors
-        gate_const, dim, reverse, shape, dtype, device = ctx.args
+        gate_const, dim, reverse, shape, stride, dtype, device = ctx.args
         want_x, want_gate, want_initial = ctx.needs_input_grad[:3]
         if g_h is None and g_final is None:
             return (None,) * 7
         lib = _lib.load()
         g_final = None if g_final is None else g_final.contiguous()
-        gx = torch.empty(shape, dtype=dtype, device=device) if want_x else None
-        gg = torch.empty(shape, dtype=dtype, device=device) if want_gate else None
+        gx = _laid_out(shape, stride, dtype, device) if want_x else None
+        gg = _laid_out(shape, stride, dtype, device) if want_gate else None
         gi = torch.empty(initial.shape, dtype=initial.dtype, device=device) if want_initial else None
         seq = _sequence(shape, dim, reverse, dtype)
         ref = C.byref(seq)
@@ -352,7 +363,7 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
         not even a NaN.  Forward, that is the step AFTER an episode's end; with ``reverse`` the step of the end itself.
     reverse: from the last step to the first (``h_t = gate_t * h_{t+1} + x_t``).
 
-    ``h`` has x's type and is contiguous; ``final`` is the last state of the walk in the state's own type, what a following
+    ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the state's own type, what a following
     call takes as ``initial``.  Differentiable in x, gate and initial."""
     _on_device('x', x)
     _need(x.dtype in _SEQ_TYPES, f'x: float32, bfloat16, float16 or float64, not {x.dtype}')
@@ -406,14 +417,15 @@ def advantages(rewards, values, ends, last_values, gamma: float = 0.99, lam: flo
         _need(t.dtype == kind, f'{name}: {kind}, not {t.dtype}')
         _need(t.shape == want, f'{name}: {tuple(t.shape)} instead of {tuple(want)}')
     lib = _lib.load()
-    adv = torch.empty(shape, dtype=torch.float32, device=device)
-    tgt = torch.empty(shape, dtype=torch.float32, device=device)
+    adv = _laid_out(shape, rewards.stride(), torch.float32, device)
+    tgt = _laid_out(shape, rewards.stride(), torch.float32, device)
     seq = _sequence(shape, 0, True, rewards.dtype)
     ref = C.byref(seq)
     nbytes = lib.lrn_advantages_workspace(ref)
     ws = _workspace(nbytes, device)
     last_values = last_values.detach().contiguous()
     _check(lib.lrn_advantages(device.index, _stream(device), ref, _ref(_view(rewards, 0)), _ref(_view(values, 0)), _ref(_view(ends, 0)),
-                              last_values.data_ptr(), float(gamma), float(lam), adv.data_ptr(), tgt.data_ptr(), _ptr(ws), nbytes),
+                              last_values.data_ptr(), float(gamma), float(lam), _ref(_view(adv, 0)), _ref(_view(tgt, 0)), _ptr(ws),
+                              nbytes),
            'advantages')
     return Advantages(adv, tgt)

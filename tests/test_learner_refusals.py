@@ -138,6 +138,7 @@ def test_the_c_abi_refuses():
     need = lib.lrn_scan_workspace(long)
     if need:
         assert lib.lrn_scan(0, None, long, v, None, 0.5, None, None, v, None, one, need - 1) == -1 and 'workspace' in text()
-    assert lib.lrn_advantages(0, None, seq(), v, v, v, one, 0.9, 0.9, one, one, None, 0) == -1 and 'channels' in text()
-    assert lib.lrn_advantages(0, None, seq(channels=1, dtype=1), v, v, v, one, 0.9, 0.9, one, one, None, 0) == -1 and 'dtype' in text()
-    assert lib.lrn_advantages(0, None, seq(channels=1), v, v, None, one, 0.9, 0.9, one, one, None, 0) == -1
+    assert lib.lrn_advantages(0, None, seq(), v, v, v, one, 0.9, 0.9, v, v, None, 0) == -1 and 'channels' in text()
+    assert lib.lrn_advantages(0, None, seq(channels=1, dtype=1), v, v, v, one, 0.9, 0.9, v, v, None, 0) == -1 and 'dtype' in text()
+    assert lib.lrn_advantages(0, None, seq(channels=1), v, v, v, one, 0.9, 0.9, v, None, None, 0) == -1
+    assert lib.lrn_advantages(0, None, seq(channels=1), v, v, None, one, 0.9, 0.9, v, v, None, 0) == -1
