@@ -72,7 +72,7 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
 
 /*
  * RECURRENCES over `steps` steps of `batch` sequences of `channels` values each; strides in elements (time, batch,
- * channel), any sign, 0 = broadcast (inputs).
+ * channel): time's of any sign, the others not negative, 0 = broadcast (inputs).
  *
  * lrn_scan:  h_t = a_t h_{t-1} + x_t,  t = 0 .. steps-1  (reverse: from the last step to the first; "before" and "last"
  * below are meant in that order).  a_t = gate_t (the type of x, or gate_const where gate is NULL), and exactly 0 where

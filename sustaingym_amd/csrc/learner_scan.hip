@@ -19,6 +19,8 @@
 //
 // A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.
 #include <algorithm>
+#include <initializer_list>
+#include <type_traits>
 
 #include "lrn_common.h"
 
@@ -40,6 +42,7 @@ struct Seq {
     const void* edge;           // backward: the initial state; advantages: V behind the last step (float32)
     void* final;
     int64_t part;               // steps of a part
+    int64_t tight;              // COLUMNS: tiles of a sequence where a tile may not reach over two (else 0)
     void* pairs;                // [parts][2][cols]
 };
 
@@ -61,246 +64,176 @@ template <class W> struct Pair {
 
 constexpr int L = 8;             // steps of a lane's run
 
-// The elements of one lane's run: L steps of V adjacent columns.
+// One lane's run, L steps of V adjacent columns: as it comes from memory ...
+template <Kind K, class T, int V>
+struct Raw {
+    static constexpr int N = L * V;
+    T x[N];
+    T g[K == ADVANTAGES ? 1 : N];              // SCAN: gate of the step; BACKWARD: of the step before in this order
+    T before[K == BACKWARD ? N : 1];           // the state before the step
+    float v[K == ADVANTAGES ? N + V : 1];      // values of the steps u0 - 1 .. u0 + L - 1
+    uint8_t r[K == BACKWARD ? N + V : N];      // flags of the steps u0 .., BACKWARD: u0 - 1 ..
+};
+// ... and as it acts
 template <Kind K, class T, int V>
 struct Run {
     using W = typename State<T>::type;
-    static constexpr int N = L * V;
-    T x[N];
-    T g[N];                      // SCAN: gate of the step; BACKWARD: of the step before in this order
-    T before[K == BACKWARD ? N : 1];
-    float v[K == ADVANTAGES ? N + V : 1];     // values of the steps u0 - 1 .. u0 + L - 1
-    uint8_t r[N + V];            // SCAN, ADVANTAGES: flags of u0 ..; BACKWARD: of u0 - 1 ..
-
-    // the coefficient and the addend of step i
-    __device__ __forceinline__ W coefficient(const Seq& S, int i, int k) const {
-        const bool cut = r[i * V + k] != 0;
-        if constexpr (K == ADVANTAGES) return cut ? W(0) : (W)S.gate_const;
-        else return cut ? W(0) : (W)g[i * V + k];
-    }
-    __device__ __forceinline__ W addend(const Seq& S, int i, int k) const {
-        const W e = (W)x[i * V + k];
-        if constexpr (K == ADVANTAGES) {
-            const W now = (W)v[(i + 1) * V + k], next = (W)v[i * V + k];
-            return r[i * V + k] ? e - now : e + (W)S.scale * next - now;
-        } else return e;
-    }
+    W a[L * V], x[L * V];
+    std::conditional_t<K == ADVANTAGES, float, W> extra[K == SCAN ? 1 : L * V];    // BACKWARD: d h / d gate; ADVANTAGES: V
 };
 
-// ---- loads and stores --------------------------------------------------------------------------------------------------
+// A lane's V columns in every view: the part of the address that is the same for the wavefront, and the lane's own.
+struct Place {
+    const char *x, *gate, *before, *resets;
+    char *h, *gate_out;
+    uint32_t ox, og, ob, orr, oh, oo;          // bytes
+    uint32_t second;                           // from the first column's flags to the second's
+};
+
+// ---- COLUMNS: loads and stores ------------------------------------------------------------------------------------------
 
 template <class E, int V> struct Vec { typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E)))); };
 
-// V adjacent columns at one step
-template <class E, int V> __device__ __forceinline__ void get(const E* p, E* to) {
-    if constexpr (V == 1) to[0] = p[0];
+template <class E, int V> __device__ __forceinline__ void get(const char* base, uint32_t lane, E* to) {
+    if constexpr (V == 1) to[0] = *reinterpret_cast<const E*>(base + lane);
     else {
-        const typename Vec<E, V>::type w = *reinterpret_cast<const typename Vec<E, V>::type*>(p);
+        const typename Vec<E, V>::type w = *reinterpret_cast<const typename Vec<E, V>::type*>(base + lane);
 #pragma unroll
         for (int k = 0; k < V; k++) to[k] = w[k];
     }
 }
-template <class E, int V> __device__ __forceinline__ void put(E* p, const E* from) {
-    if constexpr (V == 1) p[0] = from[0];
+template <class E, int V> __device__ __forceinline__ void put(char* base, uint32_t lane, const E* from) {
+    if constexpr (V == 1) *reinterpret_cast<E*>(base + lane) = from[0];
     else {
         typename Vec<E, V>::type w;
 #pragma unroll
         for (int k = 0; k < V; k++) w[k] = from[k];
-        *reinterpret_cast<typename Vec<E, V>::type*>(p) = w;
+        *reinterpret_cast<typename Vec<E, V>::type*>(base + lane) = w;
     }
 }
 
-// COLUMNS: E[from .. from + count) of the V columns at p, `fill` outside [lo, hi)
-template <class E, int V, int COUNT>
-__device__ __forceinline__ void get_steps(const void* base, int64_t st, int64_t from, int64_t lo, int64_t hi, E fill, E* to) {
-    const E* p = (const E*)base + from * st;
-    if (from >= lo && from + COUNT <= hi) {
+// COUNT steps from `from`; FULL: all of them lie in [lo, hi), else what does not is left as it is
+template <class E, int V, int COUNT, bool FULL>
+__device__ __forceinline__ void get_steps(const char* base, int64_t st, uint32_t lane, int64_t from, int64_t lo, int64_t hi, E* to) {
+    const char* p = base + from * st * (int64_t)sizeof(E);
 #pragma unroll
-        for (int i = 0; i < COUNT; i++) get<E, V>(p + i * st, to + i * V);
-    } else {
-#pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-#pragma unroll
-            for (int k = 0; k < V; k++) to[i * V + k] = fill;
-            if (from + i >= lo && from + i < hi) get<E, V>(p + i * st, to + i * V);
-        }
-    }
+    for (int i = 0; i < COUNT; i++)
+        if (FULL || (from + i >= lo && from + i < hi)) get<E, V>(p + i * st * (int64_t)sizeof(E), lane, to + i * V);
 }
 
-// RUNS: the same of one column whose steps are adjacent (either way round): 16 bytes at a time
-template <class E, int COUNT>
-__device__ __forceinline__ void get_run(const void* base, int64_t st, int64_t from, int64_t lo, int64_t hi, E fill, E* to) {
-    constexpr int VN = 16 / sizeof(E) < COUNT ? 16 / sizeof(E) : COUNT;
-    if (COUNT % VN == 0 && from >= lo && from + COUNT <= hi && (st == 1 || st == -1)) {
-        const E* p = (const E*)base + (st == 1 ? from : -(from + COUNT - 1));
+// Steps u0 .. u0 + L - 1 as they are in memory.
+template <Kind K, class T, int V, bool FULL, bool APPLYING>
+__device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t q, int64_t u0, int64_t end, Raw<K, T, V>& d) {
+    constexpr int shift = K == BACKWARD ? 1 : 0, COUNT = L + shift;
+    if (P.x) get_steps<T, V, L, FULL>(P.x, S.x.st, P.ox, u0, 0, end, d.x);
+    if constexpr (K != ADVANTAGES)
+        if (P.gate) get_steps<T, V, L, FULL>(P.gate, S.gate.st, P.og, u0 - shift, 0, end, d.g);
+    if (P.resets) {
+        const char* p = P.resets + (u0 - shift) * S.resets.st;
 #pragma unroll
-        for (int j = 0; j < COUNT; j += VN) {
-            const typename Vec<E, VN>::type w = *reinterpret_cast<const typename Vec<E, VN>::type*>(p + j);
+        for (int i = 0; i < COUNT; i++)
+            if (FULL || (u0 - shift + i >= 0 && u0 - shift + i < end)) {
 #pragma unroll
-            for (int k = 0; k < VN; k++) to[j + k] = w[k];
-        }
-        if (st == -1) {
-#pragma unroll
-            for (int j = 0; j < COUNT / 2; j++) { const E t = to[j]; to[j] = to[COUNT - 1 - j]; to[COUNT - 1 - j] = t; }
-        }
-    } else get_steps<E, 1, COUNT>(base, st, from, lo, hi, fill, to);
-}
-template <class E>
-__device__ __forceinline__ void put_run(void* base, int64_t st, int64_t from, int64_t hi, const E* v) {
-    constexpr int VN = 16 / sizeof(E) < L ? 16 / sizeof(E) : L;
-    if (from + L <= hi && (st == 1 || st == -1)) {
-        E* p = (E*)base + (st == 1 ? from : -(from + L - 1));
-#pragma unroll
-        for (int j = 0; j < L; j += VN) {
-            typename Vec<E, VN>::type w;
-#pragma unroll
-            for (int k = 0; k < VN; k++) w[k] = st == 1 ? v[j + k] : v[L - 1 - j - k];
-            *reinterpret_cast<typename Vec<E, VN>::type*>(p + j) = w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < L; i++)
-            if (from + i < hi) ((E*)base)[(from + i) * st] = v[i];
+                for (int k = 0; k < V; k++) d.r[i * V + k] = *reinterpret_cast<const uint8_t*>(p + i * S.resets.st + (P.orr + k * P.second));
+            }
     }
+    if constexpr (K == ADVANTAGES) get_steps<float, V, L + 1, FULL>(P.before, S.before.st, P.ob, u0 - 1, 0, end, d.v);
+    if constexpr (K == BACKWARD && APPLYING)
+        if (P.gate_out) get_steps<T, V, L, FULL>(P.before, S.before.st, P.ob, u0 + 1, 0, S.steps, d.before);
 }
 
-// A lane's V columns: where they start in every view.
-struct Base {
-    const void *x, *gate, *before;
-    const uint8_t* resets;
-    int64_t second;                    // flags of the second column
-    void *h, *gate_out;
-};
-template <class E> __device__ __forceinline__ const void* column(const View& v, int64_t b, int64_t c) { return v.p ? (const void*)((const E*)v.p + b * v.sb + c * v.sc) : nullptr; }
-
-template <Kind K, class T> __device__ __forceinline__ Base base_of(const Seq& S, int64_t q) {
-    int64_t b, c;
-    if ((uint64_t)S.cols <= 0xffffffffu) { b = (uint32_t)q / (uint32_t)S.channels; c = (uint32_t)q - (uint32_t)b * (uint32_t)S.channels; }
-    else { b = q / S.channels; c = q - b * S.channels; }
-    using O = std::conditional_t<K == ADVANTAGES, float, T>;
-    return Base{column<T>(S.x, b, c), column<T>(S.gate, b, c), column<O>(S.before, b, c), (const uint8_t*)column<uint8_t>(S.resets, b, 0),
-                S.channels == 1 ? S.resets.sb : 0, (void*)column<O>(S.h, b, c), (void*)column<O>(S.gate_out, b, c)};
-}
-
-template <Kind K, class T, int V, bool RUNS, bool APPLYING>
-__device__ __forceinline__ void load(const Seq& S, const Base& B, int64_t q, int64_t u0, int64_t end, Run<K, T, V>& d) {
-    constexpr int N = L * V;
-    auto steps = [&](auto fill, auto count, const void* base, int64_t st, int64_t from, int64_t lo, int64_t hi, auto* to) {
-        using E = decltype(fill);
-        if constexpr (RUNS) get_run<E, decltype(count)::value>(base, st, from, lo, hi, fill, to);
-        else get_steps<E, V, decltype(count)::value>(base, st, from, lo, hi, fill, to);
-    };
-    constexpr auto run = std::integral_constant<int, L>{};
-    constexpr int64_t shift = K == BACKWARD ? 1 : 0;
-    if (K == BACKWARD && !B.x) {
+// What the steps do.  Behind the end: a = 1, x = 0, so that a run that is cut short has the pair of what it holds.
+template <Kind K, class T, int V, bool FULL>
+__device__ __forceinline__ void fold(const Seq& S, const Place& P, const Raw<K, T, V>& d, const typename State<T>::type (&edge)[V], int64_t u0, int64_t end,
+                                     Run<K, T, V>& f) {
+    using W = typename State<T>::type;
 #pragma unroll
-        for (int i = 0; i < N; i++) d.x[i] = T(0);
-    } else steps(T(0), run, B.x, S.x.st, u0, 0, end, d.x);
-    if constexpr (K != ADVANTAGES) {
-        if (B.gate) {
-            // behind the end: a coefficient of 1, so that a run that is cut short has the pair of what it holds
-            steps(T(1), run, B.gate, S.gate.st, u0 - shift, 0, end - shift, d.g);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; i++) d.g[i] = (T)S.gate_const;
-        }
-    }
-    // flags, a byte each
-    constexpr int COUNT = K == BACKWARD ? L + 1 : L;
-    if (B.resets) {
-#pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            const int64_t u = u0 - shift + i;
-            const bool in = u >= 0 && u < end;
-#pragma unroll
-            for (int k = 0; k < V; k++) d.r[i * V + k] = in ? B.resets[u * S.resets.st + k * B.second] : 0;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < COUNT * V; i++) d.r[i] = 0;
-    }
-    if constexpr (K == ADVANTAGES) {
-        steps(0.0f, run, B.before, S.before.st, u0, 0, end, d.v + V);
+    for (int i = 0; i < L; i++) {
+        const bool in = FULL || u0 + i < end;
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const int64_t at = RUNS ? 0 : k;
-            d.v[k] = u0 == 0 ? ((const float*)S.edge)[q + k] : u0 <= end ? ((const float*)B.before)[(u0 - 1) * S.before.st + at] : 0.0f;
-        }
-    }
-    if constexpr (K == BACKWARD && APPLYING) {
-        // (the state before the step that is last in this order is the initial one, which is not in h: see walk)
-        if (B.gate_out) steps(T(0), run, B.before, S.before.st, u0 + 1, 0, S.steps, d.before);
-        else {
-#pragma unroll
-            for (int i = 0; i < N; i++) d.before[i] = T(0);
+            const int n = i * V + k;
+            const bool cut = P.resets && d.r[n];
+            W x = P.x ? (W)d.x[n] : W(0), a;
+            if constexpr (K == ADVANTAGES) {
+                const W now = (W)d.v[n + V], next = !FULL && u0 + i == 0 ? edge[k] : (W)d.v[n];
+                x = cut ? x - now : x + (W)S.scale * next - now;
+                a = cut ? W(0) : (W)S.gate_const;
+                f.extra[n] = d.v[n + V];
+            } else {
+                a = P.gate ? (W)d.g[n] : (W)S.gate_const;
+                if (cut) a = W(0);
+            }
+            if constexpr (K == BACKWARD) {
+                if (!FULL && u0 + i == 0) a = W(1);                        // g_final enters as it is
+                W prev = (W)d.before[n];
+                if (!FULL && u0 + i + 1 == S.steps) prev = edge[k];
+                f.extra[n] = P.resets && d.r[n + V] ? W(0) : prev;
+            }
+            f.a[n] = in ? a : W(1);
+            f.x[n] = in ? x : W(0);
         }
     }
 }
 
-// What lies outside the sequence: no coefficient in front of the first step of the backward pass but 1, and a constant gate
-// does not act behind the end.
-template <Kind K, class T, int V>
-__device__ __forceinline__ typename State<T>::type coefficient(const Seq& S, const Run<K, T, V>& d, int64_t u, int64_t end, int i, int k) {
-    using W = typename State<T>::type;
-    if (u + i >= end) return W(1);
-    if constexpr (K == BACKWARD)
-        if (u + i == 0) return W(1);
-    if constexpr (K != ADVANTAGES)
-        if (!S.gate.p) return d.r[i * V + k] ? W(0) : (W)S.gate_const;
-    return d.coefficient(S, i, k);
-}
-
-template <Kind K, class T, int V>
-__device__ __forceinline__ Pair<typename State<T>::type> pair_of(const Seq& S, const Run<K, T, V>& d, int64_t u0, int64_t end, int k) {
+template <Kind K, class T, int V> __device__ __forceinline__ Pair<typename State<T>::type> pair_of(const Run<K, T, V>& f, int k) {
     using W = typename State<T>::type;
     Pair<W> p{W(1), W(0)};
 #pragma unroll
-    for (int i = 0; i < L; i++) p.then(coefficient<K, T, V>(S, d, u0, end, i, k), u0 + i < end ? d.addend(S, i, k) : W(0));
+    for (int i = 0; i < L; i++) p.then(f.a[i * V + k], f.x[i * V + k]);
     return p;
 }
 
-// Walks the run from the state in front of it and writes.
-template <Kind K, class T, int V, bool RUNS>
-__device__ __forceinline__ void walk(const Seq& S, const Base& B, int64_t q, const Run<K, T, V>& d, int64_t u0, int64_t end, typename State<T>::type (&h)[V]) {
+// The outputs of step i from the state behind it.
+template <Kind K, class T, int V, class O> __device__ __forceinline__ O second_of(const Run<K, T, V>& f, int n, typename State<T>::type h) {
     using W = typename State<T>::type;
+    if constexpr (K == BACKWARD) return (O)(h * f.extra[n]);
+    else return (O)(h + (W)f.extra[n]);
+}
+
+// Walks the run from the state in front of it and writes.
+template <Kind K, class T, int V, bool FULL>
+__device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<K, T, V>& f, int64_t u0, int64_t end, typename State<T>::type (&h)[V]) {
     using O = std::conditional_t<K == ADVANTAGES, float, T>;
-    O out[L * V], second[K == SCAN ? 1 : L * V];
+    char* ph = P.h + u0 * S.h.st * (int64_t)sizeof(O);
+    char* po = P.gate_out + u0 * S.gate_out.st * (int64_t)sizeof(O);
 #pragma unroll
     for (int i = 0; i < L; i++) {
+        O out[V], second[V];
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const bool in = u0 + i < end;
-            const W a = coefficient<K, T, V>(S, d, u0, end, i, k);
-            h[k] = step(a, h[k], in ? d.addend(S, i, k) : W(0));
-            out[i * V + k] = (O)h[k];
-            if constexpr (K == BACKWARD) {
-                W prev = (W)d.before[i * V + k];
-                if (u0 + i + 1 == S.steps) prev = S.edge ? ((const W*)S.edge)[q + k] : W(0);
-                second[i * V + k] = (O)(d.r[(i + 1) * V + k] ? W(0) : h[k] * prev);
-            }
-            if constexpr (K == ADVANTAGES) second[i * V + k] = (O)(h[k] + (W)d.v[(i + 1) * V + k]);
-            if (S.final && u0 + i + 1 == S.steps) {
-                W f = h[k];
-                if constexpr (K == BACKWARD) {         // through the coefficient of the step itself
-                    const W own = d.r[(i + 1) * V + k] ? W(0) : B.gate ? (W)((const T*)B.gate)[(S.steps - 1) * S.gate.st + k] : (W)S.gate_const;
-                    f = own == W(0) ? W(0) : own * h[k];
-                }
-                ((W*)S.final)[q + k] = f;
-            }
+            h[k] = step(f.a[i * V + k], h[k], f.x[i * V + k]);
+            out[k] = (O)h[k];
+            if constexpr (K != SCAN) second[k] = second_of<K, T, V, O>(f, i * V + k, h[k]);
+        }
+        if (FULL || u0 + i < end) {
+            if (P.h) put<O, V>(ph + i * S.h.st * (int64_t)sizeof(O), P.oh, out);
+            if constexpr (K != SCAN)
+                if (P.gate_out) put<O, V>(po + i * S.gate_out.st * (int64_t)sizeof(O), P.oo, second);
         }
     }
-    auto write = [&](void* base, int64_t st, const O* v) {
-        if (!base) return;
-        if constexpr (RUNS) put_run<O>(base, st, u0, end, v);
-        else {
-            O* p = (O*)base + u0 * st;
-#pragma unroll
-            for (int i = 0; i < L; i++)
-                if (u0 + i < end) put<O, V>(p + i * st, v + i * V);
-        }
-    };
-    write(B.h, S.h.st, out);
-    if constexpr (K != SCAN) write(B.gate_out, S.gate_out.st, second);
+}
+
+// Whether the turn of `length` steps from u lies inside in every respect: its own steps, the one before and the one behind.
+template <Kind K> __device__ __forceinline__ bool inside(const Seq& S, int64_t u, int64_t length, int64_t end) {
+    return u + length <= end && (K == SCAN || u > 0) && (K != BACKWARD || u + length < S.steps);
+}
+
+template <class E> __device__ __forceinline__ const char* uniform_part(const View& v, int64_t b) { return v.p ? (const char*)v.p + b * v.sb * (int64_t)sizeof(E) : nullptr; }
+template <class E> __device__ __forceinline__ uint32_t lane_part(const View& v, int64_t b, int64_t c) { return (uint32_t)((b * v.sb + c * v.sc) * (int64_t)sizeof(E)); }
+
+// Column q = (b, c) seen from sequence b0.
+template <Kind K, class T> __device__ __forceinline__ Place place_of(const Seq& S, int64_t b0, int64_t b, int64_t c) {
+    using O = std::conditional_t<K == ADVANTAGES, float, T>;
+    Place P;
+    P.x = uniform_part<T>(S.x, b0); P.ox = lane_part<T>(S.x, b - b0, c);
+    P.gate = uniform_part<T>(S.gate, b0); P.og = lane_part<T>(S.gate, b - b0, c);
+    P.before = uniform_part<O>(S.before, b0); P.ob = lane_part<O>(S.before, b - b0, c);
+    P.resets = uniform_part<uint8_t>(S.resets, b0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
+    P.h = (char*)uniform_part<O>(S.h, b0); P.oh = lane_part<O>(S.h, b - b0, c);
+    P.gate_out = (char*)uniform_part<O>(S.gate_out, b0); P.oo = lane_part<O>(S.gate_out, b - b0, c);
+    P.second = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
+    return P;
 }
 
 // The pair of parts [from, to) of column q.
@@ -320,29 +253,69 @@ template <class W> __device__ __forceinline__ Pair<W> joined_parts(const Seq& S,
 template <Kind K, class W> __device__ __forceinline__ W first_state(const Seq& S, int64_t q) {
     return K == ADVANTAGES || !S.initial ? W(0) : ((const W*)S.initial)[q];
 }
+template <Kind K, class W> __device__ __forceinline__ W edge_of(const Seq& S, int64_t q) {
+    if constexpr (K == BACKWARD) return S.edge ? ((const W*)S.edge)[q] : W(0);
+    else if constexpr (K == ADVANTAGES) return (W)((const float*)S.edge)[q];
+    else return W(0);
+}
+// The state behind the last step to `final`; the backward pass goes through the last step's own coefficient.
+template <Kind K, class T, class W> __device__ __forceinline__ void put_final(const Seq& S, int64_t b, int64_t c, int64_t q, W h) {
+    if (!S.final) return;
+    if (K == BACKWARD && S.steps > 0) {
+        const bool cut = S.resets.p && ((const uint8_t*)S.resets.p)[(S.steps - 1) * S.resets.st + b * S.resets.sb];
+        W own = (W)S.gate_const;
+        if (S.gate.p) own = (W)((const T*)S.gate.p)[(S.steps - 1) * S.gate.st + b * S.gate.sb + c * S.gate.sc];
+        h = step(cut ? W(0) : own, h, W(0));
+    }
+    ((W*)S.final)[q] = h;
+}
 
 // ---- COLUMNS: 64 V columns to a wavefront, WT wavefronts of a workgroup one behind the other in time -----------------------
 
-template <Kind K, class T, int V, int WT, Phase P>
+template <Kind K, class T, int V, int WT, Phase PH>
 __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S) {
     using W = typename State<T>::type;
     constexpr int WC = WT == 1 ? 4 : 1;               // tiles of columns to a workgroup
+    constexpr int64_t TURN = WT * L;
     __shared__ W pa[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1], ph[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wt = WT > 1 ? wave : 0;
-    int64_t q = ((int64_t)blockIdx.x * WC + (WT > 1 ? 0 : wave)) * 64 * V + lane * V;
-    const bool there = q < S.cols;
-    if (!there) q = 0;                                // (goes along to the barriers, reads column 0, writes nothing)
-    const int64_t part = P == WHOLE ? 0 : blockIdx.y;
-    const int64_t begin = part * S.part, end = P == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Base B = base_of<K, T>(S, q);
-    W carry[V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
+    const int64_t tile = (int64_t)blockIdx.x * WC + (WT > 1 ? 0 : wave);
+    int64_t b0, b, c, q;
+    bool there;
+    if (S.tight) {                                    // a tile has columns of one sequence
+        b0 = b = tile / S.tight;
+        c = (tile - b * S.tight) * 64 * V + lane * V;
+        there = c < S.channels && b < S.cols / S.channels;
+        q = b * S.channels + c;
+    } else {
+        q = tile * 64 * V + lane * V;
+        there = q < S.cols;
+        b0 = tile * 64 * V / S.channels;
+        b = q / S.channels;
+        c = q - b * S.channels;
+    }
+    // (a lane without a column goes along to the barriers, reads the tile's first column and writes nothing)
+    if (!there) { b = b0; c = S.tight ? 0 : tile * 64 * V - b0 * S.channels; q = b * S.channels + c; }
+    if (q >= S.cols) return;                          // WT = 1: a whole wavefront behind the last tile
+    const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
+    const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
+    const Place P = place_of<K, T>(S, b0, b, c);
+    W carry[V], edge[V];
     Pair<W> all[V];
 #pragma unroll
     for (int k = 0; k < V; k++) {
         carry[k] = first_state<K, W>(S, q + k);
+        edge[k] = edge_of<K, W>(S, q + k);
         all[k] = Pair<W>{W(1), W(0)};
     }
-    if constexpr (P == APPLY) {
+    Raw<K, T, V> raw;
+    bool full = inside<K>(S, begin, TURN, end);
+    auto fetch = [&](int64_t u0) {
+        if (full) load<K, T, V, true, PH != PAIRS>(S, P, q, u0, end, raw);
+        else load<K, T, V, false, PH != PAIRS>(S, P, q, u0, end, raw);
+    };
+    fetch(begin + wt * L);
+    if constexpr (PH == APPLY) {
         // what came before this part: a wavefront joins its share of the parts, the workgroup the wavefronts'
         const int64_t share = (part + WT - 1) / WT, from = min(wt * share, part), to = min(from + share, part);
 #pragma unroll
@@ -357,37 +330,32 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
 #pragma unroll
             for (int w = 0; w < WT; w++) carry[k] = step(pa[1][w][lane * V + k], carry[k], ph[1][w][lane * V + k]);
     }
-    if (P != PAIRS && S.steps == 0 && S.final && there && wt == 0) {
-#pragma unroll
-        for (int k = 0; k < V; k++) ((W*)S.final)[q + k] = carry[k];
-    }
-    Run<K, T, V> next;
-    load<K, T, V, false, P != PAIRS>(S, B, q, begin + wt * L, end, next);
     int turn = 0;
-    for (int64_t u = begin; u < end; u += WT * L, turn ^= 1) {
+    for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
         const int64_t u0 = u + wt * L;
-        const Run<K, T, V> d = next;
-        if (u + WT * L < end) load<K, T, V, false, P != PAIRS>(S, B, q, u0 + WT * L, end, next);
+        Run<K, T, V> f;
+        const bool now_full = full;
+        if (now_full) fold<K, T, V, true>(S, P, raw, edge, u0, end, f);
+        else fold<K, T, V, false>(S, P, raw, edge, u0, end, f);
+        if (u + TURN < end) {                         // the next turn is on its way while this one is worked on
+            full = inside<K>(S, u + TURN, TURN, end);
+            fetch(u0 + TURN);
+        }
         W mine[V];
         if constexpr (WT > 1) {
-            Pair<W> p[V];
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                p[k] = pair_of<K, T, V>(S, d, u0, end, k);
-                pa[turn][wt][lane * V + k] = p[k].a;
-                ph[turn][wt][lane * V + k] = p[k].h;
+                const Pair<W> p = pair_of<K, T, V>(f, k);
+                pa[turn][wt][lane * V + k] = p.a;
+                ph[turn][wt][lane * V + k] = p.h;
             }
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < V; k++) {
-                if constexpr (P == PAIRS) {
+                if constexpr (PH == PAIRS) {
                     if (wt == 0) {
 #pragma unroll
-                        for (int w = 0; w < WT; w++) {
-                            Pair<W> o{pa[turn][w][lane * V + k], ph[turn][w][lane * V + k]};
-                            o.after(all[k]);
-                            all[k] = o;
-                        }
+                        for (int w = 0; w < WT; w++) all[k].then(pa[turn][w][lane * V + k], ph[turn][w][lane * V + k]);
                     }
                 } else {
 #pragma unroll
@@ -399,73 +367,159 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                if constexpr (P == PAIRS) {
-                    Pair<W> o = pair_of<K, T, V>(S, d, u0, end, k);
-                    o.after(all[k]);
-                    all[k] = o;
-                } else mine[k] = carry[k];
-            }
+            for (int k = 0; k < V; k++) mine[k] = carry[k];
         }
-        if constexpr (P != PAIRS) {
-            if (there && u0 < end) walk<K, T, V, false>(S, B, q, d, u0, end, mine);
+        if constexpr (PH != PAIRS) {
+            if (there) {
+                if (now_full) walk<K, T, V, true>(S, P, f, u0, end, mine);
+                else walk<K, T, V, false>(S, P, f, u0, end, mine);
+            }
             if constexpr (WT == 1) {
 #pragma unroll
                 for (int k = 0; k < V; k++) carry[k] = mine[k];
             }
         }
     }
-    if (P == PAIRS && there && wt == 0) {
+    if (!there || wt) return;
+    if constexpr (PH == PAIRS) {
         W* pairs = (W*)S.pairs + 2 * part * S.cols + q;
 #pragma unroll
         for (int k = 0; k < V; k++) { pairs[k] = all[k].a; pairs[S.cols + k] = all[k].h; }
+    } else if (end == S.steps) {
+#pragma unroll
+        for (int k = 0; k < V; k++) put_final<K, T, W>(S, S.channels == 1 ? b + k : b, S.channels == 1 ? c : c + k, q + k, carry[k]);
     }
 }
 
 // ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column -----------------------------------------------
 
-template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
+// COUNT adjacent steps from `from`, 16 bytes at a time where time has a stride of 1 or -1 and all of them are there
+template <class E, int COUNT, bool FULL>
+__device__ __forceinline__ void get_run(const char* base, int64_t st, int64_t from, int64_t lo, int64_t hi, E* to) {
+    constexpr int VN = (int)(16 / sizeof(E)) < COUNT ? (int)(16 / sizeof(E)) : COUNT;
+    if (FULL && (st == 1 || st == -1)) {
+        const E* p = (const E*)base + (st == 1 ? from : -(from + COUNT - 1));
+#pragma unroll
+        for (int j = 0; j < COUNT; j += VN) {
+            const typename Vec<E, VN>::type w = *reinterpret_cast<const typename Vec<E, VN>::type*>(p + j);
+#pragma unroll
+            for (int k = 0; k < VN; k++) to[j + k] = w[k];
+        }
+        if (st == -1) {
+#pragma unroll
+            for (int j = 0; j < COUNT / 2; j++) { const E t = to[j]; to[j] = to[COUNT - 1 - j]; to[COUNT - 1 - j] = t; }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; i++)
+            if (FULL || (from + i >= lo && from + i < hi)) to[i] = ((const E*)base)[(from + i) * st];
+    }
+}
+template <class E, bool FULL>
+__device__ __forceinline__ void put_run(char* base, int64_t st, int64_t from, int64_t hi, const E* v) {
+    constexpr int VN = (int)(16 / sizeof(E)) < L ? (int)(16 / sizeof(E)) : L;
+    if (FULL && (st == 1 || st == -1)) {
+        E* p = (E*)base + (st == 1 ? from : -(from + L - 1));
+#pragma unroll
+        for (int j = 0; j < L; j += VN) {
+            typename Vec<E, VN>::type w;
+#pragma unroll
+            for (int k = 0; k < VN; k++) w[k] = st == 1 ? v[j + k] : v[L - 1 - j - k];
+            *reinterpret_cast<typename Vec<E, VN>::type*>(p + j) = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < L; i++)
+            if (FULL || from + i < hi) ((E*)base)[(from + i) * st] = v[i];
+    }
+}
 
-template <Kind K, class T, int WT, Phase P>
+template <Kind K, class T, bool FULL, bool APPLYING>
+__device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<K, T, 1>& d) {
+    constexpr int shift = K == BACKWARD ? 1 : 0;
+    if (P.x) get_run<T, L, FULL>(P.x, S.x.st, u0, 0, end, d.x);
+    if constexpr (K != ADVANTAGES)
+        if (P.gate) get_run<T, L, FULL>(P.gate, S.gate.st, u0 - shift, 0, end, d.g);
+    if (P.resets) {
+        get_run<uint8_t, L, FULL>(P.resets, S.resets.st, u0 - shift, 0, end, d.r);
+        if constexpr (K == BACKWARD) get_run<uint8_t, 1, FULL>(P.resets, S.resets.st, u0 - 1 + L, 0, end, d.r + L);
+    }
+    if constexpr (K == ADVANTAGES) {
+        get_run<float, 1, FULL>(P.before, S.before.st, u0 - 1, 0, end, d.v);
+        get_run<float, L, FULL>(P.before, S.before.st, u0, 0, end, d.v + 1);
+    }
+    if constexpr (K == BACKWARD && APPLYING)
+        if (P.gate_out) get_run<T, L, FULL>(P.before, S.before.st, u0 + 1, 0, S.steps, d.before);
+}
+
+template <Kind K, class T, bool FULL>
+__device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<K, T, 1>& f, int64_t u0, int64_t end, typename State<T>::type h) {
+    using O = std::conditional_t<K == ADVANTAGES, float, T>;
+    O out[L], second[K == SCAN ? 1 : L];
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        h = step(f.a[i], h, f.x[i]);
+        out[i] = (O)h;
+        if constexpr (K != SCAN) second[i] = second_of<K, T, 1, O>(f, i, h);
+    }
+    if (P.h) put_run<O, FULL>(P.h, S.h.st, u0, end, out);
+    if constexpr (K != SCAN)
+        if (P.gate_out) put_run<O, FULL>(P.gate_out, S.gate_out.st, u0, end, second);
+}
+
+template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
+template <class W> __device__ __forceinline__ void wave_scan(Pair<W>& p, int lane) {
+#pragma unroll
+    for (int by = 1; by < 64; by <<= 1) {
+        const Pair<W> o = up(p, by);
+        if (lane >= by) p.after(o);
+    }
+}
+
+template <Kind K, class T, int WT, Phase PH>
 __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     using W = typename State<T>::type;
+    constexpr int64_t TURN = WT * 64 * L;
     __shared__ W pa[2][WT], ph[2][WT];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wt = WT > 1 ? wave : 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
     const int64_t q = WT > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (q >= S.cols) return;                          // WT > 1: a whole workgroup, else a whole wavefront and no barrier
-    const int64_t part = P == WHOLE ? 0 : blockIdx.y;
-    const int64_t begin = part * S.part, end = P == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Base B = base_of<K, T>(S, q);
+    const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
+    const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
+    const Place P = place_of<K, T>(S, q, q, 0);       // (one channel: the column is the sequence)
     W carry = first_state<K, W>(S, q);
-    if constexpr (P == APPLY) {
+    const W edge[1] = {edge_of<K, W>(S, q)};
+    Pair<W> all{W(1), W(0)};
+    const int64_t mine = (int64_t)(wt * 64 + lane) * L;
+    Raw<K, T, 1> raw;
+    bool full = inside<K>(S, begin, TURN, end);
+    auto fetch = [&](int64_t u0) {
+        if (full) load_run<K, T, true, PH != PAIRS>(S, P, u0, end, raw);
+        else load_run<K, T, false, PH != PAIRS>(S, P, u0, end, raw);
+    };
+    fetch(begin + mine);
+    if constexpr (PH == APPLY) {
         const int64_t share = (part + WT * 64 - 1) / (WT * 64), from = min((wt * 64 + lane) * share, part), to = min(from + share, part);
         Pair<W> p = joined_parts<W>(S, from, to, q);
-#pragma unroll
-        for (int by = 1; by < 64; by <<= 1) {
-            const Pair<W> o = up(p, by);
-            if (lane >= by) p.after(o);
-        }
+        wave_scan(p, lane);
         if (lane == 63) { pa[1][wt] = p.a; ph[1][wt] = p.h; }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < WT; w++) carry = step(pa[1][w], carry, ph[1][w]);
     }
-    if (P != PAIRS && S.steps == 0 && S.final && wt == 0 && lane == 0) ((W*)S.final)[q] = carry;
-    Pair<W> all{W(1), W(0)};
-    const int64_t mine = (int64_t)(wt * 64 + lane) * L;
-    Run<K, T, 1> next;
-    load<K, T, 1, true, P != PAIRS>(S, B, q, begin + mine, end, next);
     int turn = 0;
-    for (int64_t u = begin; u < end; u += WT * 64 * L, turn ^= 1) {
+    for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
         const int64_t u0 = u + mine;
-        const Run<K, T, 1> d = next;
-        if (u + WT * 64 * L < end) load<K, T, 1, true, P != PAIRS>(S, B, q, u0 + WT * 64 * L, end, next);
-        Pair<W> p = pair_of<K, T, 1>(S, d, u0, end, 0);
-#pragma unroll
-        for (int by = 1; by < 64; by <<= 1) {
-            const Pair<W> o = up(p, by);
-            if (lane >= by) p.after(o);
+        Run<K, T, 1> f;
+        const bool now_full = full;
+        if (now_full) fold<K, T, 1, true>(S, P, raw, edge, u0, end, f);
+        else fold<K, T, 1, false>(S, P, raw, edge, u0, end, f);
+        if (u + TURN < end) {
+            full = inside<K>(S, u + TURN, TURN, end);
+            fetch(u0 + TURN);
         }
+        Pair<W> p = pair_of<K, T, 1>(f, 0);
+        wave_scan(p, lane);
         Pair<W> front = up(p, 1);                     // of the lanes before this one
         if (lane == 0) front = Pair<W>{W(1), W(0)};
         Pair<W> whole{__shfl(p.a, 63), __shfl(p.h, 63)};
@@ -476,27 +530,26 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
 #pragma unroll
             for (int w = 0; w < WT; w++) {
                 if (w == wt) before = total;
-                Pair<W> o{pa[turn][w], ph[turn][w]};
-                o.after(total);
-                total = o;
+                total.then(pa[turn][w], ph[turn][w]);
             }
             front.after(before);
             whole = total;
         }
-        if constexpr (P == PAIRS) {
-            whole.after(all);
-            all = whole;
+        if constexpr (PH == PAIRS) {
+            all.then(whole.a, whole.h);
         } else {
-            W h[1] = {step(front.a, carry, front.h)};
+            const W h = step(front.a, carry, front.h);
             carry = step(whole.a, carry, whole.h);
-            if (u0 < end) walk<K, T, 1, true>(S, B, q, d, u0, end, h);
+            if (now_full) walk_run<K, T, true>(S, P, f, u0, end, h);
+            else walk_run<K, T, false>(S, P, f, u0, end, h);
         }
     }
-    if (P == PAIRS && wt == 0 && lane == 0) {
+    if (wt || lane) return;
+    if constexpr (PH == PAIRS) {
         W* pairs = (W*)S.pairs + 2 * part * S.cols + q;
         pairs[0] = all.a;
         pairs[S.cols] = all.h;
-    }
+    } else if (end == S.steps) put_final<K, T, W>(S, q, 0, q, carry);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
@@ -515,6 +568,12 @@ int checked(const lrn_seq* q, const char* who) {
     if (!q) return fail(-1, "%s: null sequence", who);
     if (q->steps < 0 || q->batch < 0 || q->channels < 0) return fail(-1, "%s: %lld steps, batch %lld, %lld channels", who, (long long)q->steps, (long long)q->batch, (long long)q->channels);
     if (q->dtype < LRN_F32 || q->dtype > LRN_F64) return fail(-1, "%s: dtype %d", who, q->dtype);
+    return 0;
+}
+
+int check_views(const char* who, std::initializer_list<const lrn_view*> views) {
+    for (const lrn_view* v : views)
+        if (v && v->data && (v->sb < 0 || v->sc < 0)) return fail(-1, "%s: batch and channel strides may not be negative", who);
     return 0;
 }
 
@@ -557,8 +616,17 @@ int64_t pair_bytes(const lrn_seq* q) {
     return parts > 1 ? parts * 2 * cols * (q->dtype == LRN_F64 ? 8 : 4) : 0;
 }
 
+// A lane's part of an address has 32 bits: how far the columns of one tile lie apart in a view.
+bool near(const View& v, const Seq& S, int64_t size, int tile) {
+    const int64_t over = std::min(S.cols / S.channels - 1, tile / S.channels + 1);
+    return !v.p || (v.sb <= ((int64_t)1 << 40) && over * v.sb * size + S.channels * v.sc * size < ((int64_t)1 << 32));
+}
+
 template <Kind K, class T, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
-    const int64_t tiles = cdiv(cdiv(S.cols, 64 * V), WT == 1 ? 4 : 1);
+    const bool flat = near(S.x, S, sizeof(T), 64 * V) && near(S.gate, S, sizeof(T), 64 * V) && near(S.before, S, sizeof(T), 64 * V) &&
+                      near(S.resets, S, 1, 64 * V) && near(S.h, S, sizeof(T), 64 * V) && near(S.gate_out, S, sizeof(T), 64 * V);
+    S.tight = flat ? 0 : cdiv(S.channels, 64 * V);
+    const int64_t tiles = cdiv(flat ? cdiv(S.cols, 64 * V) : S.cols / S.channels * S.tight, WT == 1 ? 4 : 1);
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
         if constexpr (WT == 16) {
@@ -640,6 +708,7 @@ int lrn_scan(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_vie
     if (int rc = checked(seq, "lrn_scan")) return rc;
     if (seq->batch * seq->channels == 0) return 0;
     if (seq->steps && (!x || !x->data || !h_out || !h_out->data)) return fail(-1, "lrn_scan: null x or h");
+    if (int rc = check_views("lrn_scan", {x, gate, resets, h_out})) return rc;
     if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_scan")) return rc;
     LRN_ON_DEVICE(device);
     const bool rev = seq->reverse != 0;
@@ -659,6 +728,7 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
     if (int rc = checked(seq, "lrn_scan_backward")) return rc;
     if (seq->batch * seq->channels == 0) return 0;
     if (grad_gate_out && grad_gate_out->data && seq->steps && (!h || !h->data)) return fail(-1, "lrn_scan_backward: null h");
+    if (int rc = check_views("lrn_scan_backward", {gate, resets, h, g_h, grad_x_out, grad_gate_out})) return rc;
     if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_scan_backward")) return rc;
     LRN_ON_DEVICE(device);
     const bool rev = seq->reverse == 0;
@@ -684,6 +754,7 @@ int lrn_advantages(int32_t device, void* hip_stream, const lrn_seq* seq, const l
     if (!rewards || !rewards->data || !values || !values->data || !ends || !ends->data || !last_values || !advantage_out ||
         !advantage_out->data || !target_out || !target_out->data)
         return fail(-1, "lrn_advantages: null argument");
+    if (int rc = check_views("lrn_advantages", {rewards, values, ends, advantage_out, target_out})) return rc;
     if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_advantages")) return rc;
     LRN_ON_DEVICE(device);
     Seq S{};
