@@ -17,7 +17,8 @@
 // workgroup along time; pairs go through LDS.  RUNS: time is the fast index, so lanes lie along time, pairs go through a
 // wavefront scan.  State, pairs and products are float32 (float64 for float64 sequences) whatever the elements' type.
 //
-// A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.
+// A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.  For float32 that is the
+// multiplication in which 0 times anything is 0, one instruction instead of a comparison and a selection behind an fma.
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -52,14 +53,18 @@ enum Phase { WHOLE, PAIRS, APPLY };
 template <class T> struct State { using type = float; };
 template <> struct State<double> { using type = double; };
 
-template <class W> __device__ __forceinline__ W step(W a, W h, W x) { return a == W(0) ? x : a * h + x; }
+extern "C" __device__ float product_with_zero(float, float) __asm("llvm.amdgcn.fmul.legacy");
+__device__ __forceinline__ float times(float a, float b) { return product_with_zero(a, b); }
+__device__ __forceinline__ double times(double a, double b) { return a == 0.0 ? 0.0 : a * b; }
+__device__ __forceinline__ float step(float a, float h, float x) { return times(a, h) + x; }
+__device__ __forceinline__ double step(double a, double h, double x) { return a == 0.0 ? x : __builtin_fma(a, h, x); }
 
 // (A, H) of a run
 template <class W> struct Pair {
     W a, h;
-    __device__ __forceinline__ void then(W a2, W x) { h = step(a2, h, x); a = a2 == W(0) ? W(0) : a2 * a; }
+    __device__ __forceinline__ void then(W a2, W x) { h = step(a2, h, x); a = times(a2, a); }
     // what came before it
-    __device__ __forceinline__ void after(const Pair& first) { h = step(a, first.h, h); a = a == W(0) ? W(0) : a * first.a; }
+    __device__ __forceinline__ void after(const Pair& first) { h = step(a, first.h, h); a = times(a, first.a); }
 };
 
 constexpr int L = 8;             // steps of a lane's run
@@ -112,13 +117,22 @@ template <class E, int V> __device__ __forceinline__ void put(char* base, uint32
     }
 }
 
+// One step further, by a scalar addition at its place: eight multiples of every stride kept ready would not fit the scalar
+// registers, and come back from vector lanes at two instructions a piece.
+template <class P> __device__ __forceinline__ void advance(P& p, int64_t bytes) {
+    p += bytes;
+    asm("" : "+s"(p));
+}
+
 // COUNT steps from `from`; FULL: all of them lie in [lo, hi), else what does not is left as it is
 template <class E, int V, int COUNT, bool FULL>
 __device__ __forceinline__ void get_steps(const char* base, int64_t st, uint32_t lane, int64_t from, int64_t lo, int64_t hi, E* to) {
     const char* p = base + from * st * (int64_t)sizeof(E);
 #pragma unroll
-    for (int i = 0; i < COUNT; i++)
-        if (FULL || (from + i >= lo && from + i < hi)) get<E, V>(p + i * st * (int64_t)sizeof(E), lane, to + i * V);
+    for (int i = 0; i < COUNT; i++) {
+        if (FULL || (from + i >= lo && from + i < hi)) get<E, V>(p, lane, to + i * V);
+        advance(p, st * (int64_t)sizeof(E));
+    }
 }
 
 // Steps u0 .. u0 + L - 1 as they are in memory.
@@ -131,11 +145,13 @@ __device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t q, in
     if (P.resets) {
         const char* p = P.resets + (u0 - shift) * S.resets.st;
 #pragma unroll
-        for (int i = 0; i < COUNT; i++)
+        for (int i = 0; i < COUNT; i++) {
             if (FULL || (u0 - shift + i >= 0 && u0 - shift + i < end)) {
 #pragma unroll
-                for (int k = 0; k < V; k++) d.r[i * V + k] = *reinterpret_cast<const uint8_t*>(p + i * S.resets.st + (P.orr + k * P.second));
+                for (int k = 0; k < V; k++) d.r[i * V + k] = *reinterpret_cast<const uint8_t*>(p + (P.orr + k * P.second));
             }
+            advance(p, S.resets.st);
+        }
     }
     if constexpr (K == ADVANTAGES) get_steps<float, V, L + 1, FULL>(P.before, S.before.st, P.ob, u0 - 1, 0, end, d.v);
     if constexpr (K == BACKWARD && APPLYING)
@@ -207,10 +223,12 @@ __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<K, 
             if constexpr (K != SCAN) second[k] = second_of<K, T, V, O>(f, i * V + k, h[k]);
         }
         if (FULL || u0 + i < end) {
-            if (P.h) put<O, V>(ph + i * S.h.st * (int64_t)sizeof(O), P.oh, out);
+            if (P.h) put<O, V>(ph, P.oh, out);
             if constexpr (K != SCAN)
-                if (P.gate_out) put<O, V>(po + i * S.gate_out.st * (int64_t)sizeof(O), P.oo, second);
+                if (P.gate_out) put<O, V>(po, P.oo, second);
         }
+        advance(ph, S.h.st * (int64_t)sizeof(O));
+        if constexpr (K != SCAN) advance(po, S.gate_out.st * (int64_t)sizeof(O));
     }
 }
 
@@ -277,7 +295,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     using W = typename State<T>::type;
     constexpr int WC = WT == 1 ? 4 : 1;               // tiles of columns to a workgroup
     constexpr int64_t TURN = WT * L;
-    __shared__ W pa[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1], ph[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1];
+    __shared__ Pair<W> pairs_of[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
     const int64_t tile = (int64_t)blockIdx.x * WC + (WT > 1 ? 0 : wave);
     int64_t b0, b, c, q;
@@ -320,15 +338,16 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
         const int64_t share = (part + WT - 1) / WT, from = min(wt * share, part), to = min(from + share, part);
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const Pair<W> p = joined_parts<W>(S, from, to, q + k);
-            pa[1][wt][lane * V + k] = p.a;
-            ph[1][wt][lane * V + k] = p.h;
+            pairs_of[1][wt][lane * V + k] = joined_parts<W>(S, from, to, q + k);
         }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < V; k++)
 #pragma unroll
-            for (int w = 0; w < WT; w++) carry[k] = step(pa[1][w][lane * V + k], carry[k], ph[1][w][lane * V + k]);
+            for (int w = 0; w < WT; w++) {
+                const Pair<W> p = pairs_of[1][w][lane * V + k];
+                carry[k] = step(p.a, carry[k], p.h);
+            }
     }
     int turn = 0;
     for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
@@ -344,24 +363,24 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
         W mine[V];
         if constexpr (WT > 1) {
 #pragma unroll
-            for (int k = 0; k < V; k++) {
-                const Pair<W> p = pair_of<K, T, V>(f, k);
-                pa[turn][wt][lane * V + k] = p.a;
-                ph[turn][wt][lane * V + k] = p.h;
-            }
+            for (int k = 0; k < V; k++) pairs_of[turn][wt][lane * V + k] = pair_of<K, T, V>(f, k);
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < V; k++) {
                 if constexpr (PH == PAIRS) {
                     if (wt == 0) {
 #pragma unroll
-                        for (int w = 0; w < WT; w++) all[k].then(pa[turn][w][lane * V + k], ph[turn][w][lane * V + k]);
+                        for (int w = 0; w < WT; w++) {
+                            const Pair<W> p = pairs_of[turn][w][lane * V + k];
+                            all[k].then(p.a, p.h);
+                        }
                     }
                 } else {
 #pragma unroll
                     for (int w = 0; w < WT; w++) {
                         if (w == wt) mine[k] = carry[k];
-                        carry[k] = step(pa[turn][w][lane * V + k], carry[k], ph[turn][w][lane * V + k]);
+                        const Pair<W> p = pairs_of[turn][w][lane * V + k];
+                        carry[k] = step(p.a, carry[k], p.h);
                     }
                 }
             }
