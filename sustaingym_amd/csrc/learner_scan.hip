@@ -412,66 +412,63 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
 
 // ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column -----------------------------------------------
 
-// COUNT adjacent steps from `from`, 16 bytes at a time where time has a stride of 1 or -1 and all of them are there
-template <class E, int COUNT, bool FULL>
-__device__ __forceinline__ void get_run(const char* base, int64_t st, int64_t from, int64_t lo, int64_t hi, E* to) {
+// COUNT steps from `from`, 16 bytes at a time (at any alignment); DIR: whether they rise or fall in memory.  Not FULL: one by
+// one, what lies outside [lo, hi) is left as it is.
+template <class E, int DIR, int COUNT, bool FULL>
+__device__ __forceinline__ void get_run(const char* base, int64_t from, int64_t lo, int64_t hi, E* to) {
     constexpr int VN = (int)(16 / sizeof(E)) < COUNT ? (int)(16 / sizeof(E)) : COUNT;
-    if (FULL && (st == 1 || st == -1)) {
-        const E* p = (const E*)base + (st == 1 ? from : -(from + COUNT - 1));
+    const E* p = (const E*)base + (DIR > 0 ? from : -(from + COUNT - 1));
+    if constexpr (FULL) {
 #pragma unroll
         for (int j = 0; j < COUNT; j += VN) {
             const typename Vec<E, VN>::type w = *reinterpret_cast<const typename Vec<E, VN>::type*>(p + j);
 #pragma unroll
-            for (int k = 0; k < VN; k++) to[j + k] = w[k];
-        }
-        if (st == -1) {
-#pragma unroll
-            for (int j = 0; j < COUNT / 2; j++) { const E t = to[j]; to[j] = to[COUNT - 1 - j]; to[COUNT - 1 - j] = t; }
+            for (int k = 0; k < VN; k++) to[DIR > 0 ? j + k : COUNT - 1 - j - k] = w[k];
         }
     } else {
 #pragma unroll
         for (int i = 0; i < COUNT; i++)
-            if (FULL || (from + i >= lo && from + i < hi)) to[i] = ((const E*)base)[(from + i) * st];
+            if (from + i >= lo && from + i < hi) to[i] = p[DIR > 0 ? i : COUNT - 1 - i];
     }
 }
-template <class E, bool FULL>
-__device__ __forceinline__ void put_run(char* base, int64_t st, int64_t from, int64_t hi, const E* v) {
+template <class E, int DIR, bool FULL>
+__device__ __forceinline__ void put_run(char* base, int64_t from, int64_t hi, const E* v) {
     constexpr int VN = (int)(16 / sizeof(E)) < L ? (int)(16 / sizeof(E)) : L;
-    if (FULL && (st == 1 || st == -1)) {
-        E* p = (E*)base + (st == 1 ? from : -(from + L - 1));
+    E* p = (E*)base + (DIR > 0 ? from : -(from + L - 1));
+    if constexpr (FULL) {
 #pragma unroll
         for (int j = 0; j < L; j += VN) {
             typename Vec<E, VN>::type w;
 #pragma unroll
-            for (int k = 0; k < VN; k++) w[k] = st == 1 ? v[j + k] : v[L - 1 - j - k];
+            for (int k = 0; k < VN; k++) w[k] = v[DIR > 0 ? j + k : L - 1 - j - k];
             *reinterpret_cast<typename Vec<E, VN>::type*>(p + j) = w;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < L; i++)
-            if (FULL || from + i < hi) ((E*)base)[(from + i) * st] = v[i];
+            if (from + i < hi) p[DIR > 0 ? i : L - 1 - i] = v[i];
     }
 }
 
-template <Kind K, class T, bool FULL, bool APPLYING>
+template <Kind K, class T, int DIR, bool FULL, bool APPLYING>
 __device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<K, T, 1>& d) {
     constexpr int shift = K == BACKWARD ? 1 : 0;
-    if (P.x) get_run<T, L, FULL>(P.x, S.x.st, u0, 0, end, d.x);
+    if (P.x) get_run<T, DIR, L, FULL>(P.x, u0, 0, end, d.x);
     if constexpr (K != ADVANTAGES)
-        if (P.gate) get_run<T, L, FULL>(P.gate, S.gate.st, u0 - shift, 0, end, d.g);
+        if (P.gate) get_run<T, DIR, L, FULL>(P.gate, u0 - shift, 0, end, d.g);
     if (P.resets) {
-        get_run<uint8_t, L, FULL>(P.resets, S.resets.st, u0 - shift, 0, end, d.r);
-        if constexpr (K == BACKWARD) get_run<uint8_t, 1, FULL>(P.resets, S.resets.st, u0 - 1 + L, 0, end, d.r + L);
+        get_run<uint8_t, DIR, L, FULL>(P.resets, u0 - shift, 0, end, d.r);
+        if constexpr (K == BACKWARD) get_run<uint8_t, DIR, 1, FULL>(P.resets, u0 - 1 + L, 0, end, d.r + L);
     }
     if constexpr (K == ADVANTAGES) {
-        get_run<float, 1, FULL>(P.before, S.before.st, u0 - 1, 0, end, d.v);
-        get_run<float, L, FULL>(P.before, S.before.st, u0, 0, end, d.v + 1);
+        get_run<float, DIR, 1, FULL>(P.before, u0 - 1, 0, end, d.v);
+        get_run<float, DIR, L, FULL>(P.before, u0, 0, end, d.v + 1);
     }
     if constexpr (K == BACKWARD && APPLYING)
-        if (P.gate_out) get_run<T, L, FULL>(P.before, S.before.st, u0 + 1, 0, S.steps, d.before);
+        if (P.gate_out) get_run<T, DIR, L, FULL>(P.before, u0 + 1, 0, S.steps, d.before);
 }
 
-template <Kind K, class T, bool FULL>
+template <Kind K, class T, int DIR, bool FULL>
 __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<K, T, 1>& f, int64_t u0, int64_t end, typename State<T>::type h) {
     using O = std::conditional_t<K == ADVANTAGES, float, T>;
     O out[L], second[K == SCAN ? 1 : L];
@@ -481,9 +478,9 @@ __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run
         out[i] = (O)h;
         if constexpr (K != SCAN) second[i] = second_of<K, T, 1, O>(f, i, h);
     }
-    if (P.h) put_run<O, FULL>(P.h, S.h.st, u0, end, out);
+    if (P.h) put_run<O, DIR, FULL>(P.h, u0, end, out);
     if constexpr (K != SCAN)
-        if (P.gate_out) put_run<O, FULL>(P.gate_out, S.gate_out.st, u0, end, second);
+        if (P.gate_out) put_run<O, DIR, FULL>(P.gate_out, u0, end, second);
 }
 
 template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
@@ -495,7 +492,7 @@ template <class W> __device__ __forceinline__ void wave_scan(Pair<W>& p, int lan
     }
 }
 
-template <Kind K, class T, int WT, Phase PH>
+template <Kind K, class T, int DIR, int WT, Phase PH>
 __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     using W = typename State<T>::type;
     constexpr int64_t TURN = WT * 64 * L;
@@ -513,8 +510,8 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     Raw<K, T, 1> raw;
     bool full = inside<K>(S, begin, TURN, end);
     auto fetch = [&](int64_t u0) {
-        if (full) load_run<K, T, true, PH != PAIRS>(S, P, u0, end, raw);
-        else load_run<K, T, false, PH != PAIRS>(S, P, u0, end, raw);
+        if (full) load_run<K, T, DIR, true, PH != PAIRS>(S, P, u0, end, raw);
+        else load_run<K, T, DIR, false, PH != PAIRS>(S, P, u0, end, raw);
     };
     fetch(begin + mine);
     if constexpr (PH == APPLY) {
@@ -559,8 +556,8 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
         } else {
             const W h = step(front.a, carry, front.h);
             carry = step(whole.a, carry, whole.h);
-            if (now_full) walk_run<K, T, true>(S, P, f, u0, end, h);
-            else walk_run<K, T, false>(S, P, f, u0, end, h);
+            if (now_full) walk_run<K, T, DIR, true>(S, P, f, u0, end, h);
+            else walk_run<K, T, DIR, false>(S, P, f, u0, end, h);
         }
     }
     if (wt || lane) return;
@@ -641,6 +638,9 @@ bool near(const View& v, const Seq& S, int64_t size, int tile) {
     return !v.p || (v.sb <= ((int64_t)1 << 40) && over * v.sb * size + S.channels * v.sc * size < ((int64_t)1 << 32));
 }
 
+// 16 wavefronts of a workgroup have 128 registers each, which the float64 backward pass does not fit: 8 there.
+template <Kind K, class T> constexpr int kMany = K == BACKWARD && std::is_same<T, double>::value ? 8 : 16;
+
 template <Kind K, class T, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
     const bool flat = near(S.x, S, sizeof(T), 64 * V) && near(S.gate, S, sizeof(T), 64 * V) && near(S.before, S, sizeof(T), 64 * V) &&
                       near(S.resets, S, 1, 64 * V) && near(S.h, S, sizeof(T), 64 * V) && near(S.gate_out, S, sizeof(T), 64 * V);
@@ -648,37 +648,44 @@ template <Kind K, class T, int V, int WT> void launch_columns(Seq& S, const Deal
     const int64_t tiles = cdiv(flat ? cdiv(S.cols, 64 * V) : S.cols / S.channels * S.tight, WT == 1 ? 4 : 1);
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
-        if constexpr (WT == 16) {
+        if constexpr (WT == kMany<K, T>) {
             columns_kernel<K, T, V, WT, PAIRS><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
             columns_kernel<K, T, V, WT, APPLY><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
         }
     } else columns_kernel<K, T, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
 }
-template <Kind K, class T, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
+template <Kind K, class T, int DIR, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
     const int64_t blocks = WT == 1 ? cdiv(S.cols, 4) : S.cols;
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
-        if constexpr (WT == 16) {
-            runs_kernel<K, T, WT, PAIRS><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
-            runs_kernel<K, T, WT, APPLY><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
+        if constexpr (WT == kMany<K, T>) {
+            runs_kernel<K, T, DIR, WT, PAIRS><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
+            runs_kernel<K, T, DIR, WT, APPLY><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
         }
-    } else runs_kernel<K, T, WT, WHOLE><<<(unsigned)blocks, threads, 0, stream>>>(S);
+    } else runs_kernel<K, T, DIR, WT, WHOLE><<<(unsigned)blocks, threads, 0, stream>>>(S);
+}
+
+template <Kind K, class T, int DIR> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
+    if (d.wt == 1) launch_runs<K, T, DIR, 1>(S, d, stream);
+    else if (d.wt == 4) launch_runs<K, T, DIR, 4>(S, d, stream);
+    else launch_runs<K, T, DIR, kMany<K, T>>(S, d, stream);
 }
 
 bool dense(const View& v, int64_t channels) { return !v.p || (channels == 1 ? v.sb : v.sc) == 1; }
 
 template <Kind K, class T> int launch(Seq S, void* workspace, int64_t bytes, hipStream_t stream, const char* who) {
-    // time is the fast index of what is read
-    const View& main = S.x.p ? S.x : S.h;
-    const bool runs = S.channels == 1 && S.steps > 1 && (main.st == 1 || main.st == -1) && (main.sb != 1 || S.cols == 1);
+    // time is the fast index of everything there is (a view that is the same at all steps, say, is read by columns)
+    const int64_t st = S.x.p ? S.x.st : S.h.p ? S.h.st : S.gate_out.st;
+    bool runs = S.channels == 1 && S.steps > 1 && (st == 1 || st == -1);
+    for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.gate_out}) runs = runs && (!v->p || v->st == st);
+    for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || !v->p || v->sb != 1);
     const Deal d = runs ? deal_runs(S.steps, S.cols) : deal_columns(S.steps, S.cols);
     if (d.parts > 65535 || S.cols > ((int64_t)1 << 32)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
     S.part = d.part;
     S.pairs = workspace;
     if (runs) {
-        if (d.wt == 1) launch_runs<K, T, 1>(S, d, stream);
-        else if (d.wt == 4) launch_runs<K, T, 4>(S, d, stream);
-        else launch_runs<K, T, 16>(S, d, stream);
+        if (st == 1) launch_runs<K, T, 1>(S, d, stream);
+        else launch_runs<K, T, -1>(S, d, stream);
     } else {
         // Two columns to a lane (wider rows, half the instructions) where there are enough for the GPU all the same.
         const bool two = S.cols >= 65536 && S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) &&
@@ -688,7 +695,7 @@ template <Kind K, class T> int launch(Seq S, void* workspace, int64_t bytes, hip
             else launch_columns<K, T, 2, 4>(S, Deal{4, S.steps, 1}, stream);
         } else if (d.wt == 1) launch_columns<K, T, 1, 1>(S, d, stream);
         else if (d.wt == 4) launch_columns<K, T, 1, 4>(S, d, stream);
-        else launch_columns<K, T, 1, 16>(S, d, stream);
+        else launch_columns<K, T, 1, kMany<K, T>>(S, d, stream);
     }
     LRN_LAUNCHED(who);
     return 0;
