@@ -18,7 +18,6 @@ To capture a backward pass, ask for it with ``torch.autograd.grad`` inside the c
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import NamedTuple
 
 import torch
@@ -54,15 +53,21 @@ def _check(rc: int, what: str) -> None:
         raise _lib.EngineLibraryError(f'{what} failed with code {rc}: {_lib.load().lrn_last_error().decode("utf-8", "replace")}')
 
 
-def _need(ok: bool, text: str) -> None:
-    if not ok:
-        raise ValueError(text)
-
-
 def _on_device(name: str, t, device=None) -> None:
-    _need(isinstance(t, torch.Tensor), f'{name}: a tensor is needed, not {type(t).__name__}')
-    _need(t.is_cuda, f'{name}: a CUDA tensor is needed (there is no CPU form)')
-    _need(device is None or t.device == device, f'{name}: on {t.device}, the first argument is on {device}')
+    if isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device):
+        return
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f'{name}: a tensor is needed, not {type(t).__name__}')
+    if not t.is_cuda:
+        raise ValueError(f'{name}: a CUDA tensor is needed (there is no CPU form)')
+    raise ValueError(f'{name}: on {t.device}, the first argument is on {device}')
+
+
+def _broadcasts(t, shape) -> bool:
+    try:
+        return torch.broadcast_shapes(t.shape, shape) == shape
+    except RuntimeError:
+        return False
 
 
 def _stream(device) -> int:
@@ -104,63 +109,61 @@ class _Rows:
     __slots__ = ('struct', 'keep', 'noise', 'noise_strides')
 
     def __init__(self, logits, mask, noise=None):
-        lead, K = logits.shape[:-1], logits.shape[-1]
+        shape = logits.shape
+        K = shape[-1]
+        if logits.is_contiguous() and (mask is None or mask.shape == shape and mask.is_contiguous()) and (
+                noise is None or noise.shape == shape and noise.is_contiguous()):
+            self.struct = _lib.LearnerRows(logits.data_ptr(), 1, logits.numel() // K, K, 0, K,
+                                           None if mask is None else mask.data_ptr(), 0, K, 1, _ROW_TYPES[logits.dtype])
+            self.keep = (logits, mask, noise)
+            self.noise, self.noise_strides = noise, (0, K)
+            return
+        mask_level = 1
         if logits.stride(-1) != 1 and K > 1:
             logits = logits.contiguous()
-        mask_level = 1
         if mask is not None:
-            if mask.shape != logits.shape:
-                mask = mask.expand(logits.shape)
+            mask = mask.expand(shape)
             mask_level = mask.stride(-1)
             if mask_level not in (0, 1):
-                mask = mask.contiguous()
-                mask_level = 1 if K > 1 else 0
+                mask, mask_level = mask.contiguous(), 1
         if noise is not None:
-            if noise.shape != logits.shape:
-                noise = noise.expand(logits.shape)
+            noise = noise.expand(shape)
             if noise.stride(-1) != 1 and K > 1:
                 noise = noise.contiguous()
-        n = math.prod(lead)
-        if logits.is_contiguous() and (mask is None or mask.is_contiguous()) and (noise is None or noise.is_contiguous()):
-            outer, inner, strides = 1, n, [(0, K)] * 3
-        elif n == 0:
-            outer, inner, strides = 0, 0, [(0, 0)] * 3
+        folded = _folded(shape[:-1], [t.stride()[:-1] for t in (logits, mask, noise) if t is not None])
+        if folded is None:
+            logits = logits.contiguous()
+            mask = None if mask is None else mask.contiguous()
+            noise = None if noise is None else noise.contiguous()
+            mask_level = 1
+            outer, inner, strides = 1, logits.numel() // K, [(0, K)] * 3
         else:
-            there = [t for t in (logits, mask, noise) if t is not None]
-            folded = _folded(lead, [t.stride()[:-1] for t in there])
-            if folded is None:
-                logits = logits.contiguous()
-                mask = None if mask is None else mask.contiguous()
-                noise = None if noise is None else noise.contiguous()
-                mask_level = 1
-                folded = 1, n, [(0, K)] * 3
             outer, inner, strides = folded
-            strides = list(strides)
             if mask is None:
                 strides.insert(1, (0, 0))
             if noise is None:
                 strides.append((0, 0))
-        self.struct = _lib.LearnerRows(logits.data_ptr(), outer, inner, K, strides[0][0], strides[0][1], _ptr(mask),
-                                       strides[1][0], strides[1][1], mask_level, _ROW_TYPES[logits.dtype])
+        self.struct = _lib.LearnerRows(logits.data_ptr(), outer, inner, K, *strides[0], _ptr(mask), *strides[1], mask_level,
+                                       _ROW_TYPES[logits.dtype])
         self.keep = (logits, mask, noise)
         self.noise, self.noise_strides = noise, strides[2]
 
 
 def _check_rows(logits, mask, noise=None):
     _on_device('logits', logits)
-    _need(logits.dtype in _ROW_TYPES, f'logits: float32, bfloat16 or float16, not {logits.dtype}')
-    _need(logits.dim() >= 1 and 1 <= logits.shape[-1] < 2 ** 30, f'logits: [..., levels], got {tuple(logits.shape)}')
-    for name, t, kinds in (('mask', mask, (torch.bool,)), ('noise', noise, (torch.float32,))):
+    if logits.dtype not in _ROW_TYPES:
+        raise ValueError(f'logits: float32, bfloat16 or float16, not {logits.dtype}')
+    shape = logits.shape
+    if not shape or not 1 <= shape[-1] < 2 ** 30:
+        raise ValueError(f'logits: [..., levels], got {tuple(shape)}')
+    for name, t, kind in (('mask', mask, torch.bool), ('noise', noise, torch.float32)):
         if t is None:
             continue
         _on_device(name, t, logits.device)
-        _need(t.dtype in kinds, f'{name}: {kinds[0]}, not {t.dtype}')
-        if t.shape != logits.shape:
-            try:
-                ok = torch.broadcast_shapes(t.shape, logits.shape) == logits.shape
-            except RuntimeError:
-                ok = False
-            _need(ok, f'{name}: {tuple(t.shape)} does not broadcast to the logits\' {tuple(logits.shape)}')
+        if t.dtype != kind:
+            raise ValueError(f'{name}: {kind}, not {t.dtype}')
+        if t.shape != shape and not _broadcasts(t, shape):
+            raise ValueError(f'{name}: {tuple(t.shape)} does not broadcast to the logits\' {tuple(shape)}')
 
 
 def choose_levels(logits, noise=None, mask=None) -> LevelChoice:
@@ -208,9 +211,16 @@ def _row_gradient(g):
     """A per-row gradient and its element stride: one value for all rows (a sum's gradient) is not spread out."""
     if g is None:
         return None, 0
+    if g.is_contiguous():
+        return g, 1
     if all(s == 0 or n == 1 for n, s in zip(g.shape, g.stride())):
         return g, 0
     return g.contiguous(), 1
+
+
+def _no_second(gradient, ctx, *grads):
+    """``gradient(ctx, *grads)``; under ``create_graph`` its results say, when differentiated, that they cannot be."""
+    return once_differentiable(gradient)(ctx, *grads) if torch.is_grad_enabled() else gradient(ctx, *grads)
 
 
 class _LevelLogprobs(torch.autograd.Function):
@@ -226,10 +236,13 @@ class _LevelLogprobs(torch.autograd.Function):
         return logprobs, entropy, tl, ti
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, *_):
+        return _no_second(_LevelLogprobs._gradient, ctx, g_logprobs, g_entropy)
+
+    @staticmethod
+    def _gradient(ctx, g_logprobs, g_entropy):
         logits, levels, mask, stat, entropy = ctx.saved_tensors
-        rows = _Rows(logits, mask)
+        rows = _Rows(logits, mask)       # (from what was saved: hooks may have moved it meanwhile)
         g_logprobs, s_lp = _row_gradient(g_logprobs)
         g_entropy, s_h = _row_gradient(g_entropy)
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
@@ -253,12 +266,16 @@ def level_logprobs(logits, levels, mask=None, top: int = 0) -> LevelScores:
     Log probabilities, entropies and all sums are float32 whatever the logits' type; the gradient has the logits' type."""
     _check_rows(logits, mask)
     _on_device('levels', levels, logits.device)
-    _need(levels.dtype in (torch.int64, torch.int32), f'levels: int64 or int32, not {levels.dtype}')
-    _need(levels.shape == logits.shape[:-1], f'levels: {tuple(levels.shape)}, the logits have rows {tuple(logits.shape[:-1])}')
+    if levels.shape != logits.shape[:-1]:
+        raise ValueError(f'levels: {tuple(levels.shape)}, the logits have rows {tuple(logits.shape[:-1])}')
+    if levels.dtype != torch.int64:
+        if levels.dtype != torch.int32:
+            raise ValueError(f'levels: int64 or int32, not {levels.dtype}')
+        levels = levels.to(torch.int64)
+    levels = levels.contiguous()
     top = int(top)
-    _need(0 <= top <= min(MAX_TOP, logits.shape[-1]), f'top: 0 .. {min(MAX_TOP, logits.shape[-1])}, got {top}')
-    if levels.dtype != torch.int64 or not levels.is_contiguous():
-        levels = levels.to(torch.int64).contiguous()
+    if not 0 <= top <= min(MAX_TOP, logits.shape[-1]):
+        raise ValueError(f'top: 0 .. {min(MAX_TOP, logits.shape[-1])}, got {top}')
     if logits.requires_grad and torch.is_grad_enabled():
         return LevelScores(*_LevelLogprobs.apply(logits, levels, mask, top))
     rows = _Rows(logits.detach(), mask)
@@ -294,9 +311,11 @@ def _state_type(dtype):
 def _laid_out(shape, stride, dtype, device):
     """An output in the layout of the input with these strides (a batch-major trajectory stays one); contiguous where that one
     has holes or overlaps."""
+    if 0 in shape:
+        return torch.empty(shape, dtype=dtype, device=device)
     expect = 1
     for s, n in sorted((s, n) for n, s in zip(shape, stride) if n != 1):
-        if s != expect or n == 0:
+        if s != expect:
             return torch.empty(shape, dtype=dtype, device=device)
         expect *= n
     return torch.empty_strided(shape, stride, dtype=dtype, device=device)
@@ -304,8 +323,8 @@ def _laid_out(shape, stride, dtype, device):
 
 def _scan(x, gate, gate_const, initial, resets, dim, reverse):
     lib, device = _lib.load(), x.device
-    h = _laid_out(x.shape, x.stride(), x.dtype, device)
-    final = torch.empty([n for i, n in enumerate(x.shape) if i != dim], dtype=_state_type(x.dtype), device=device)
+    h = torch.empty(x.shape, dtype=x.dtype, device=device) if x.is_contiguous() else _laid_out(x.shape, x.stride(), x.dtype, device)
+    final = torch.empty(x.shape[:dim] + x.shape[dim + 1:], dtype=_state_type(x.dtype), device=device)
     seq = _sequence(x.shape, dim, reverse, x.dtype)
     ref = C.byref(seq)
     nbytes = lib.lrn_scan_workspace(ref)
@@ -328,8 +347,11 @@ class _GatedScan(torch.autograd.Function):
         return h, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_h, g_final):
+        return _no_second(_GatedScan._gradient, ctx, g_h, g_final)
+
+    @staticmethod
+    def _gradient(ctx, g_h, g_final):
         gate, resets, initial, h = ctx.saved_tensors
         gate_const, dim, reverse, shape, stride, dtype, device = ctx.args
         want_x, want_gate, want_initial = ctx.needs_input_grad[:3]
@@ -366,33 +388,40 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
     ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the state's own type, what a following
     call takes as ``initial``.  Differentiable in x, gate and initial."""
     _on_device('x', x)
-    _need(x.dtype in _SEQ_TYPES, f'x: float32, bfloat16, float16 or float64, not {x.dtype}')
-    _need(1 <= x.dim() <= 3, f'x: one to three dimensions, got {tuple(x.shape)}')
-    _need(dim in (0, 1) and dim < x.dim(), f'dim: 0 or 1 of {tuple(x.shape)}, got {dim}')
+    device, shape = x.device, x.shape
+    if x.dtype not in _SEQ_TYPES:
+        raise ValueError(f'x: float32, bfloat16, float16 or float64, not {x.dtype}')
+    if not 1 <= len(shape) <= 3:
+        raise ValueError(f'x: one to three dimensions, got {tuple(shape)}')
+    if dim not in (0, 1) or dim >= len(shape):
+        raise ValueError(f'dim: 0 or 1 of {tuple(shape)}, got {dim}')
     const = 0.0
     if isinstance(gate, torch.Tensor):
-        _on_device('gate', gate, x.device)
-        _need(gate.dtype == x.dtype, f'gate: {gate.dtype}, x is {x.dtype}')
-        if gate.shape != x.shape:
-            try:
-                ok = torch.broadcast_shapes(gate.shape, x.shape) == x.shape
-            except RuntimeError:
-                ok = False
-            _need(ok, f'gate: {tuple(gate.shape)} does not broadcast to x\'s {tuple(x.shape)}')
-            gate = gate.expand(x.shape)
-    else:
-        _need(isinstance(gate, (int, float)), f'gate: a tensor or a number, not {type(gate).__name__}')
+        _on_device('gate', gate, device)
+        if gate.dtype != x.dtype:
+            raise ValueError(f'gate: {gate.dtype}, x is {x.dtype}')
+        if gate.shape != shape:
+            if not _broadcasts(gate, shape):
+                raise ValueError(f'gate: {tuple(gate.shape)} does not broadcast to x\'s {tuple(shape)}')
+            gate = gate.expand(shape)
+    elif isinstance(gate, (int, float)):
         const, gate = float(gate), None
+    else:
+        raise ValueError(f'gate: a tensor or a number, not {type(gate).__name__}')
     if initial is not None:
-        _on_device('initial', initial, x.device)
-        shape = tuple(n for i, n in enumerate(x.shape) if i != dim)
-        _need(tuple(initial.shape) == shape, f'initial: {tuple(initial.shape)} instead of {shape}')
-        _need(initial.dtype == _state_type(x.dtype), f'initial: {_state_type(x.dtype)}, not {initial.dtype}')
+        _on_device('initial', initial, device)
+        rest = shape[:dim] + shape[dim + 1:]
+        if initial.shape != rest:
+            raise ValueError(f'initial: {tuple(initial.shape)} instead of {tuple(rest)}')
+        if initial.dtype != _state_type(x.dtype):
+            raise ValueError(f'initial: {_state_type(x.dtype)}, not {initial.dtype}')
         initial = initial.contiguous()
     if resets is not None:
-        _on_device('resets', resets, x.device)
-        _need(resets.dtype == torch.bool, f'resets: torch.bool, not {resets.dtype}')
-        _need(resets.shape == x.shape[:2], f'resets: {tuple(resets.shape)} instead of {tuple(x.shape[:2])}')
+        _on_device('resets', resets, device)
+        if resets.dtype != torch.bool:
+            raise ValueError(f'resets: torch.bool, not {resets.dtype}')
+        if resets.shape != shape[:2]:
+            raise ValueError(f'resets: {tuple(resets.shape)} instead of {tuple(shape[:2])}')
     reverse = bool(reverse)
     if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad)
                                     or (initial is not None and initial.requires_grad)):
@@ -409,13 +438,17 @@ def advantages(rewards, values, ends, last_values, gamma: float = 0.99, lam: flo
     state behind the last step.  Float32 results; the arithmetic is float64 where the rewards are.  No gradient flows."""
     _on_device('rewards', rewards)
     device, shape = rewards.device, rewards.shape
-    _need(rewards.dtype in (torch.float64, torch.float32), f'rewards: float64 or float32, not {rewards.dtype}')
-    _need(1 <= rewards.dim() <= 2, f'rewards: [T, N] or [T], got {tuple(shape)}')
+    if rewards.dtype not in (torch.float64, torch.float32):
+        raise ValueError(f'rewards: float64 or float32, not {rewards.dtype}')
+    if not 1 <= len(shape) <= 2:
+        raise ValueError(f'rewards: [T, N] or [T], got {tuple(shape)}')
     for name, t, kind, want in (('values', values, torch.float32, shape), ('ends', ends, torch.bool, shape),
                                 ('last_values', last_values, torch.float32, shape[1:])):
         _on_device(name, t, device)
-        _need(t.dtype == kind, f'{name}: {kind}, not {t.dtype}')
-        _need(t.shape == want, f'{name}: {tuple(t.shape)} instead of {tuple(want)}')
+        if t.dtype != kind:
+            raise ValueError(f'{name}: {kind}, not {t.dtype}')
+        if t.shape != want:
+            raise ValueError(f'{name}: {tuple(t.shape)} instead of {tuple(want)}')
     lib = _lib.load()
     adv = _laid_out(shape, rewards.stride(), torch.float32, device)
     tgt = _laid_out(shape, rewards.stride(), torch.float32, device)
