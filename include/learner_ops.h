@@ -9,7 +9,7 @@
  * -2 no device, -4 HIP error.
  *
  * ROWS.  `rows = outer * inner` rows of `levels` logits; row (o, i) starts at o * stride_outer + i * stride_inner
- * ELEMENTS, its logits are adjacent.  mask (NULL = all allowed): bytes, non-zero = allowed, at
+ * ELEMENTS (strides are not negative), its logits are adjacent.  What lies between two rows may be read, and is not used.  mask (NULL = all allowed): bytes, non-zero = allowed, at
  * o * mask_outer + i * mask_inner + j * mask_level (mask_level 0 or 1; strides of 0 broadcast).  What a masked place
  * holds (infinities, NaN) is never used.  A logit of -inf is a masked one.  Per-row arrays are contiguous [rows].
  *   m = max z_j, s = sum exp(z_j - m) over the allowed j

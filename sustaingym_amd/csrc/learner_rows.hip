@@ -23,7 +23,8 @@ struct Rows {
     int64_t rows, inner;
     int64_t so, si, mo, mi;
     int32_t levels, mask_level;
-    uint32_t per_level;          // ceil(2^32 / levels): e / levels = e per_level >> 32 for e < 2^16, levels <= 1024
+    int64_t limit, mask_limit;   // elements from the first of any row to behind the last of any
+    bool dense, mask_dense;      // row r starts at r * levels
 };
 
 struct Sums {
@@ -116,19 +117,32 @@ __device__ __forceinline__ const uint8_t* row_mask(const Rows& R, int64_t r) {
 __device__ __forceinline__ void finish(Sums& a) { if (a.m == -kNegInf) a.s = __builtin_nanf(""); }
 __device__ __forceinline__ float entropy_of(const Sums& a, float logs) { return a.s != 0.0f ? logs - a.t / a.s : 0.0f; }
 
-struct ChooseOut { const float* noise; int64_t no, ni; int64_t* level; float* logprob; float* entropy; };
+struct ChooseOut { const float* noise; int64_t no, ni, limit; bool dense; int64_t* level; float* logprob; float* entropy; };
+
+// Where row r starts in the logits, the mask and the noise.
+__device__ __forceinline__ void offsets(const Rows& R, int64_t r, int64_t& off, int64_t& moff, const ChooseOut* O = nullptr, int64_t* noff = nullptr) {
+    off = moff = r * R.levels;
+    if (O) *noff = off;
+    if (R.dense && (!R.mask || R.mask_dense) && (!O || O->dense)) return;
+    int64_t o, i;
+    split(R, r, o, i);
+    off = o * R.so + i * R.si;
+    moff = o * R.mo + i * R.mi;
+    if (O) *noff = o * O->no + i * O->ni;
+}
+
 struct ScoreOut { const int64_t* level; float* logprob; float* entropy; float* stat; int top; float* top_logprob; int64_t* top_level; };
 
 struct BackIn { const int64_t* level; const float* stat; const float* entropy; const float* g_lp; const float* g_h; int g_lp_stride, g_h_stride; };
 
-// ---- rows of up to 1024 levels: G lanes to a row -----------------------------------------------------------------------
+// ---- rows of up to 1024 levels: G lanes to a row, E adjacent levels to a lane --------------------------------------------
 //
-// A workgroup takes 256 / G rows.  Their logits are one run of memory (FLAT): 16-byte loads by all lanes bring it, whatever
-// the rows' length, and the rows are picked out of LDS, where they sit an odd number of words apart (no two lanes of a
-// half-wavefront on one bank).  A lane holds E levels of its row in registers, so that the maximum comes first and every
-// weight is computed once; the group's sums go through DPP.  The backward pass computes the row's maximum and sums again from
-// the logits that it has to read anyway: cheaper than 12 bytes a row of saved statistics.  Rows at other strides, broadcast
-// masks and unaligned starts are read a row at a time by the row's own lanes (not FLAT).
+// A lane takes its levels with one or two vector loads (at any alignment; what they read beyond the row belongs to the next
+// one and is dropped, and only where there is no next one do single loads take over), so no index is computed per level and
+// rows at any stride go the same way.  Rows of up to eight levels have their length compiled in.  The maximum comes first and
+// every weight is computed once; the group's sums go through DPP.  The backward pass computes the row's maximum and sums again
+// from the logits that it has to read anyway: cheaper than 12 bytes a row of saved statistics.  Its results meet in LDS, from
+// where they leave as one run of 16-byte stores.
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -146,7 +160,46 @@ template <int G, class F> __device__ __forceinline__ void over_group(F&& f) {
     if constexpr (G >= 64) f([](auto v) { return __shfl_xor(v, 32); });
 }
 
-// What a group knows of its row: the levels g, g + G, ... are z[0], z[1], ... of lane g (-inf behind the row and where masked).
+template <class V, int N> __device__ __forceinline__ void take(const V* p, V (&to)[N]) { __builtin_memcpy(to, p, sizeof(to)); }
+
+// Lane g's levels g E .. of row r: -inf where masked or behind the row.
+template <class T, int G, int E>
+__device__ __forceinline__ void load_levels(const Rows& R, int64_t off, int64_t moff, int g, float (&z)[E]) {
+    const int j0 = g * E, valid = R.levels - j0;
+    T v[E];
+    uint8_t b[E];
+    const T* src = (const T*)R.logits + off + j0;
+    if (valid > 0) {
+        if (off + j0 + E <= R.limit) take(src, v);
+        else {
+#pragma unroll
+            for (int k = 0; k < E; k++)
+                if (k < valid) v[k] = src[k];
+        }
+    }
+    if (R.mask) {
+        const uint8_t* mk = R.mask + moff;
+        if (!R.mask_level) {
+            const uint8_t on = mk[0];
+#pragma unroll
+            for (int k = 0; k < E; k++) b[k] = on;
+        } else if (valid > 0) {
+            if (moff + j0 + E <= R.mask_limit) take(mk + j0, b);
+            else {
+#pragma unroll
+                for (int k = 0; k < E; k++)
+                    if (k < valid) b[k] = mk[j0 + k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < E; k++) z[k] = k < valid && b[k] ? to_f32(v[k]) : kNegInf;
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; k++) z[k] = k < valid ? to_f32(v[k]) : kNegInf;
+    }
+}
+
+// The row's maximum and sums, and the weights of the lane's own levels.
 template <int G, int E>
 __device__ __forceinline__ Sums group_sums(const float (&z)[E], float (&e)[E]) {
     Sums a;
@@ -154,227 +207,240 @@ __device__ __forceinline__ Sums group_sums(const float (&z)[E], float (&e)[E]) {
 #pragma unroll
     for (int k = 1; k < E; k++) a.m = fmaxf(a.m, z[k]);
     over_group<G>([&](auto from) { a.m = fmaxf(a.m, from(a.m)); });
+    const float m = a.m == kNegInf ? 0.0f : a.m;       // nothing allowed: all weights 0 (or NaN)
     a.s = a.t = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const float d = z[k] - a.m;
-        e[k] = z[k] == kNegInf ? 0.0f : fast_exp(d);
+        const float d = z[k] - m;
+        e[k] = fast_exp(d);
         a.s += e[k];
-        a.t += e[k] > 0.0f ? e[k] * d : 0.0f;
+        a.t += e[k] * fmaxf(d, -3.0e38f);              // a masked level: 0 times a number
     }
     over_group<G>([&](auto from) { a.s += from(a.s); a.t += from(a.t); });
     finish(a);
     return a;
 }
 
-template <int G, int E> constexpr int kTile = 256 / G * (G * E + 1);
-
-// The tile's logits (and noise) into LDS as float32; masked ones as -inf.
-template <class T, int G, int E, bool FLAT, bool NOISE>
-__device__ __forceinline__ void load_tile(const Rows& R, const ChooseOut* C, int64_t r0, int rows, float* z, float* nz) {
-    const int K = R.levels, pitch = K | 1, tid = threadIdx.x;
-    if constexpr (FLAT) {
-        constexpr int VE = 16 / sizeof(T);
-        const int n = rows * K;
-        const T* src = (const T*)R.logits + r0 * K;
-        const uint8_t* mk = R.mask ? R.mask + r0 * K : nullptr;
-        const float* ns = NOISE && C->noise ? C->noise + r0 * K : nullptr;
-        for (int e0 = tid * VE; e0 < n; e0 += 256 * VE) {
-            int row = __umulhi((uint32_t)e0, R.per_level), col = e0 - row * K;
-            T v[VE];
-            uint8_t b[VE];
-            float w[VE];
-            const bool whole = e0 + VE <= n;
-            if (whole) {
-                *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + e0);
-                if (mk) {
-                    if constexpr (VE == 8) *reinterpret_cast<uint2*>(b) = *reinterpret_cast<const uint2*>(mk + e0);
-                    else *reinterpret_cast<uint32_t*>(b) = *reinterpret_cast<const uint32_t*>(mk + e0);
-                }
-                if (NOISE && ns) {
-#pragma unroll
-                    for (int k = 0; k < VE; k += 4) *reinterpret_cast<float4*>(w + k) = *reinterpret_cast<const float4*>(ns + e0 + k);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < VE; k++)
-                    if (e0 + k < n) { v[k] = src[e0 + k]; if (mk) b[k] = mk[e0 + k]; if (NOISE && ns) w[k] = ns[e0 + k]; }
-            }
-#pragma unroll
-            for (int k = 0; k < VE; k++) {
-                if (whole || e0 + k < n) {
-                    z[row * pitch + col] = mk && !b[k] ? kNegInf : to_f32(v[k]);
-                    if (NOISE && ns) nz[row * pitch + col] = w[k];
-                }
-                if (++col == K) { col = 0; row++; }
-            }
-        }
-    } else {
-        const int row = tid / G, g = tid % G;
-        if (row < rows) {
-            int64_t o, i;
-            split(R, r0 + row, o, i);
-            const T* src = (const T*)R.logits + o * R.so + i * R.si;
-            const uint8_t* mk = R.mask ? R.mask + o * R.mo + i * R.mi : nullptr;
-            const float* ns = NOISE && C->noise ? C->noise + o * C->no + i * C->ni : nullptr;
-#pragma unroll
-            for (int k = 0; k < E; k++) {
-                const int j = g + G * k;
-                if (j < K) {
-                    z[row * pitch + j] = mk && !mk[j * R.mask_level] ? kNegInf : to_f32(src[j]);
-                    if (NOISE && ns) nz[row * pitch + j] = ns[j];
-                }
-            }
-        }
-    }
-    __syncthreads();
-}
-
-template <class T, int G, int E, bool FLAT>
+template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) {
-    __shared__ float zs[kTile<G, E>], ns[kTile<G, E>];
-    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
-    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels;
-    load_tile<T, G, E, FLAT, true>(R, &O, r0, rows, zs, ns);
-    const int row = threadIdx.x / G, g = threadIdx.x % G;
-    if (row >= rows) return;                    // whole groups: no lane of a group leaves alone
-    const float* mine = zs + row * (K | 1);
-    const float* noise = ns + row * (K | 1);
-    float z[E], e[E];
+    const int g = threadIdx.x % G;
+    const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (r >= R.rows) return;                    // whole groups: no lane of a group leaves alone
+    int64_t off, moff, noff;
+    offsets(R, r, off, moff, &O, &noff);
+    float z[E], e[E], w[E];
+    load_levels<T, G, E>(R, off, moff, g, z);
     Best b;
     b.clear();
+    if (O.noise) {
+        const float* ns = O.noise + noff + g * E;
+        if (noff + g * E + E <= O.limit) take(ns, w);
+        else {
 #pragma unroll
-    for (int k = 0; k < E; k++) {
-        const int j = g + G * k;
-        z[k] = j < K ? mine[j] : kNegInf;
-        if (z[k] != kNegInf) b.add(O.noise ? z[k] + noise[j] : z[k], j);
+            for (int k = 0; k < E; k++) w[k] = g * E + k < R.levels ? ns[k] : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < E; k++) w[k] = 0.0f;
     }
     const Sums a = group_sums<G, E>(z, e);
-    over_group<G>([&](auto from) { b.add(from(b.v), from(b.j)); });
+    float chosen = 0.0f;
+#pragma unroll
+    for (int k = 0; k < E; k++) {
+        const float key = O.noise ? z[k] + w[k] : z[k];
+        if (z[k] > kNegInf && key > b.v) { b.v = key; b.j = g * E + k; chosen = z[k]; }
+    }
+    over_group<G>([&](auto from) {
+        const float v = from(b.v), c = from(chosen);
+        const int j = from(b.j);
+        if (v > b.v || (v == b.v && j < b.j)) { b.v = v; b.j = j; chosen = c; }
+    });
     if (g == 0) {
-        const bool some = a.s != 0.0f, found = b.j < K;
+        const bool some = a.s != 0.0f, found = b.j < R.levels;
         const float logs = logf(a.s);
-        O.level[r0 + row] = some && found ? b.j : 0;
-        O.logprob[r0 + row] = !some ? 0.0f : found ? mine[b.j] - a.m - logs : __builtin_nanf("");
-        O.entropy[r0 + row] = entropy_of(a, logs);
+        O.level[r] = some && found ? b.j : 0;
+        O.logprob[r] = !some ? 0.0f : found ? chosen - a.m - logs : __builtin_nanf("");
+        O.entropy[r] = entropy_of(a, logs);
     }
 }
 
-template <class T, int G, int E, bool FLAT>
+// A level in the order of alternatives: by logit, the lowest index first among equals.  16-bit logits and their index fit one
+// word whose unsigned order is that order; 0: none.
+template <class T> struct Key {
+    uint32_t k;
+    __device__ __forceinline__ void set(float z, int j) {
+        const T t = (T)(z + 0.0f);                                       // (-0 is 0)
+        const uint32_t u = __builtin_bit_cast(uint16_t, t);
+        k = z > kNegInf ? ((u & 0x8000 ? ~u & 0xffff : u | 0x8000) << 16) | (0xffffu - j) : 0u;
+    }
+    __device__ __forceinline__ bool some() const { return k != 0; }
+    __device__ __forceinline__ float value() const {
+        const uint32_t u = k >> 16;
+        return to_f32(__builtin_bit_cast(T, (uint16_t)(u & 0x8000 ? u & 0x7fff : ~u)));
+    }
+    __device__ __forceinline__ int level() const { return 0xffff - (int)(k & 0xffff); }
+    __device__ __forceinline__ void order(Key& o) { const uint32_t hi = max(k, o.k), lo = min(k, o.k); k = hi; o.k = lo; }
+    template <int G> __device__ __forceinline__ Key best() const {
+        uint32_t b = k;
+        over_group<G>([&](auto from) { b = max(b, (uint32_t)from((int)b)); });
+        return Key{b};
+    }
+    __device__ __forceinline__ bool is(const Key& o) const { return k == o.k; }
+};
+template <> struct Key<float> {
+    float v;
+    int j;
+    __device__ __forceinline__ void set(float z, int i) { v = z > kNegInf ? z : kNegInf; j = z > kNegInf ? i : 0x7fffffff; }
+    __device__ __forceinline__ bool some() const { return v > kNegInf; }
+    __device__ __forceinline__ float value() const { return v; }
+    __device__ __forceinline__ int level() const { return j; }
+    __device__ __forceinline__ void order(Key& o) {
+        const bool swap = o.v > v || (o.v == v && o.j < j);
+        const Key t = *this;
+        if (swap) { *this = o; o = t; }
+    }
+    template <int G> __device__ __forceinline__ Key best() const {
+        float b = v;
+        over_group<G>([&](auto from) { b = fmaxf(b, from(b)); });
+        int i = v == b ? j : 0x7fffffff;
+        over_group<G>([&](auto from) { i = min(i, from(i)); });
+        return Key{b, i};
+    }
+    __device__ __forceinline__ bool is(const Key& o) const { return j == o.j; }
+};
+
+// A merge-exchange network for N values (Batcher 1968; Knuth volume 3, 5.2.2 M).
+template <int N> struct Network {
+    int a[64], b[64], n;
+    constexpr Network() : a(), b(), n(0) {
+        int t = 0;
+        while ((1 << t) < N) t++;
+        for (int p = t ? 1 << (t - 1) : 0; p > 0; p >>= 1) {
+            int q = 1 << (t - 1), r = 0, d = p;
+            for (;;) {
+                for (int i = 0; i + d < N; i++)
+                    if ((i & p) == r) { a[n] = i; b[n++] = i + d; }
+                if (q == p) break;
+                d = q - p;
+                q >>= 1;
+                r = p;
+            }
+        }
+    }
+};
+
+template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_score_kernel(Rows R, ScoreOut O) {
-    __shared__ float zs[kTile<G, E>];
-    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
-    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels;
-    load_tile<T, G, E, FLAT, false>(R, nullptr, r0, rows, zs, nullptr);
-    const int row = threadIdx.x / G, g = threadIdx.x % G;
-    if (row >= rows) return;
-    const int64_t r = r0 + row;
-    const float* mine = zs + row * (K | 1);
-    const int64_t l = g == 0 ? O.level[r] : 0;
-    float z[E], e[E];
-#pragma unroll
-    for (int k = 0; k < E; k++) z[k] = g + G * k < K ? mine[g + G * k] : kNegInf;
+    const int g = threadIdx.x % G;
+    const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    if (r >= R.rows) return;
+    int64_t off, moff;
+    offsets(R, r, off, moff);
+    const int K = R.levels;
+    const int64_t l = O.level[r];
+    float z[E], e[E], zl = kNegInf;
+    load_levels<T, G, E>(R, off, moff, g, z);
+    if (g == 0 && l >= 0 && l < K && !(R.mask && !R.mask[moff + l * R.mask_level])) zl = to_f32(((const T*)R.logits)[off + l]);
     const Sums a = group_sums<G, E>(z, e);
     const float logs = logf(a.s);
     if (g == 0) {
-        O.logprob[r] = l >= K ? __builtin_nanf("") : l < 0 || a.s == 0.0f ? 0.0f : mine[l] - a.m - logs;
+        O.logprob[r] = l >= K ? __builtin_nanf("") : l < 0 || a.s == 0.0f ? 0.0f : zl - a.m - logs;
         O.entropy[r] = entropy_of(a, logs);
         if (O.stat) { O.stat[2 * r] = a.m; O.stat[2 * r + 1] = a.s; }
     }
-    for (int n = 0; n < O.top; n++) {           // the best of what is left, O.top times
-        Best b;
-        b.clear();
+    if (!O.top) return;
+    // Every lane puts its levels in order; the best of the lanes' first ones is the next alternative, O.top times.  Lane n % G
+    // keeps the n-th, so that G of them leave together.
+    Key<T> key[E];
 #pragma unroll
-        for (int k = 0; k < E; k++)
-            if (z[k] > kNegInf) b.add(z[k], g + G * k);
-        over_group<G>([&](auto from) { b.add(from(b.v), from(b.j)); });
+    for (int k = 0; k < E; k++) key[k].set(z[k], g * E + k);
+    constexpr Network<E> net;
 #pragma unroll
-        for (int k = 0; k < E; k++)
-            if (g + G * k == b.j) z[k] = kNegInf;
-        if (g == 0) {
-            const bool some = b.j < K;
-            O.top_logprob[r * O.top + n] = some ? b.v - a.m - logs : a.s == a.s ? kNegInf : a.s;
-            O.top_level[r * O.top + n] = some ? b.j : -1;
+    for (int c = 0; c < net.n; c++) key[net.a[c]].order(key[net.b[c]]);
+    Key<T> kept = key[0];
+    for (int n = 0; n < O.top; n++) {
+        const Key<T> best = key[0].template best<G>();
+        if (n % G == g) kept = best;
+        if (key[0].is(best)) {
+#pragma unroll
+            for (int k = 0; k + 1 < E; k++) key[k] = key[k + 1];
+            key[E - 1].set(kNegInf, 0);
+        }
+        if (n % G == G - 1 || n == O.top - 1) {
+            const int at = n - n % G + g;
+            if (at <= n) {
+                O.top_logprob[r * O.top + at] = kept.some() ? kept.value() - a.m - logs : a.s == a.s ? kNegInf : a.s;
+                O.top_level[r * O.top + at] = kept.some() ? kept.level() : -1;
+            }
         }
     }
 }
 
-template <class T, int G, int E, bool FLAT>
-__global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T* grad, bool aligned) {
-    __shared__ float zs[kTile<G, E>];
-    const int64_t r0 = (int64_t)blockIdx.x * (256 / G);
-    const int rows = (int)min((int64_t)(256 / G), R.rows - r0), K = R.levels, pitch = K | 1;
-    load_tile<T, G, E, FLAT, false>(R, nullptr, r0, rows, zs, nullptr);
-    const int row = threadIdx.x / G, g = threadIdx.x % G;
-    if (row < rows) {
-        const int64_t r = r0 + row;
-        float* mine = zs + row * pitch;
+template <class T, int G, int E>
+__global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T* grad) {
+    __shared__ __attribute__((aligned(16))) T out[256 * E];
+    const int row = threadIdx.x / G, g = threadIdx.x % G, K = R.levels;
+    const int64_t r0 = (int64_t)blockIdx.x * (256 / G), r = r0 + row;
+    if (r < R.rows) {
+        int64_t off, moff;
+        offsets(R, r, off, moff);
         const int64_t l = I.level[r];
-        const float gl = I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f, gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f;
+        const float gl = l >= K ? __builtin_nanf("") : I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f;
+        const float gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f;
         float z[E], e[E];
-#pragma unroll
-        for (int k = 0; k < E; k++) z[k] = g + G * k < K ? mine[g + G * k] : kNegInf;
+        load_levels<T, G, E>(R, off, moff, g, z);
         const Sums a = group_sums<G, E>(z, e);
-        const float logs = logf(a.s), inv = 1.0f / a.s, H = entropy_of(a, logs);
+        const float logs = logf(a.s), inv = 1.0f / a.s, lift = entropy_of(a, logs) - logs, m = a.m;
+        const int mine = l >= 0 && l < K ? (int)l - g * E : -1;
+        T* to = out + row * K + g * E;
 #pragma unroll
         for (int k = 0; k < E; k++) {
-            const int j = g + G * k;
-            const float p = e[k] * inv;
-            float d = (j == l ? gl : 0.0f) - p * (gl + gh * (e[k] > 0.0f ? z[k] - a.m - logs + H : 0.0f));
-            if (z[k] == kNegInf) d = 0.0f;
-            if (l >= K) d = __builtin_nanf("");
-            if (j < K) mine[j] = d;
+            // p (g_lp + g_h (log p + H)), log p = z - m - log s; a weight of 0 has p log p = 0
+            float d = -(e[k] * inv) * (gl + gh * (e[k] > 0.0f ? z[k] - m + lift : 0.0f));
+            if (k == mine) d += gl;
+            if (z[k] == kNegInf) d = l >= K ? gl : 0.0f;
+            if (g * E + k < K) to[k] = (T)d;
         }
     }
     __syncthreads();
-    constexpr int VE = 16 / sizeof(T);
-    const int n = rows * K;
-    T* out = grad + r0 * K;
-    for (int e0 = threadIdx.x * VE; e0 < n; e0 += 256 * VE) {
-        int at = __umulhi((uint32_t)e0, R.per_level), col = e0 - at * K;
-        T v[VE];
-#pragma unroll
-        for (int k = 0; k < VE; k++) {
-            v[k] = e0 + k < n ? (T)zs[at * pitch + col] : (T)0.0f;
-            if (++col == K) { col = 0; at++; }
-        }
-        if (aligned && e0 + VE <= n) *reinterpret_cast<uint4*>(out + e0) = *reinterpret_cast<const uint4*>(v);
+    constexpr int N = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+    const int n = (int)min((int64_t)(256 / G), R.rows - r0) * K;
+    T* to = grad + r0 * K;
+    for (int e0 = threadIdx.x * N; e0 < n; e0 += 256 * N) {
+        if (e0 + N <= n) *reinterpret_cast<vec*>(to + e0) = *reinterpret_cast<const vec*>(out + e0);
         else {
 #pragma unroll
-            for (int k = 0; k < VE; k++)
-                if (e0 + k < n) out[e0 + k] = v[k];
+            for (int k = 0; k < N; k++)
+                if (e0 + k < n) to[e0 + k] = out[e0 + k];
         }
     }
 }
 
-// 8 levels to a lane fill the registers of a full set of wavefronts; up to 1024 levels a wavefront is one row.
+// Up to eight levels: the row itself; then eight levels to a lane (a full set of wavefronts has the registers), sixteen where
+// a row would not fit a wavefront otherwise.
 constexpr int kGroupLevels = 1024;
 #define BY_LEVELS(K, call)                                                          \
-    do {                                                                            \
-        if ((K) <= 4) { constexpr int G = 1, E = 4; call; }                         \
-        else if ((K) <= 8) { constexpr int G = 1, E = 8; call; }                    \
-        else if ((K) <= 16) { constexpr int G = 2, E = 8; call; }                   \
-        else if ((K) <= 32) { constexpr int G = 4, E = 8; call; }                   \
-        else if ((K) <= 64) { constexpr int G = 8, E = 8; call; }                   \
-        else if ((K) <= 128) { constexpr int G = 16, E = 8; call; }                 \
-        else if ((K) <= 256) { constexpr int G = 32, E = 8; call; }                 \
-        else if ((K) <= 512) { constexpr int G = 64, E = 8; call; }                 \
-        else { constexpr int G = 64, E = 16; call; }                                \
-    } while (0)
+    switch (K) {                                                                    \
+        case 1: { constexpr int G = 1, E = 1; call; break; }                        \
+        case 2: { constexpr int G = 1, E = 2; call; break; }                        \
+        case 3: { constexpr int G = 1, E = 3; call; break; }                        \
+        case 4: { constexpr int G = 1, E = 4; call; break; }                        \
+        case 5: { constexpr int G = 1, E = 5; call; break; }                        \
+        case 6: { constexpr int G = 1, E = 6; call; break; }                        \
+        case 7: { constexpr int G = 1, E = 7; call; break; }                        \
+        case 8: { constexpr int G = 1, E = 8; call; break; }                        \
+        default:                                                                    \
+            if ((K) <= 16) { constexpr int G = 2, E = 8; call; }                    \
+            else if ((K) <= 32) { constexpr int G = 4, E = 8; call; }               \
+            else if ((K) <= 64) { constexpr int G = 8, E = 8; call; }               \
+            else if ((K) <= 128) { constexpr int G = 16, E = 8; call; }             \
+            else if ((K) <= 256) { constexpr int G = 32, E = 8; call; }             \
+            else if ((K) <= 512) { constexpr int G = 64, E = 8; call; }             \
+            else { constexpr int G = 64, E = 16; call; }                            \
+    }
 
-int group_rows(int64_t K) { int g = 256; BY_LEVELS(K, (g = 256 / G, (void)E)); return g; }
-
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-// Whether the rows (and mask, noise) are one dense run whose tiles start on 16 bytes (the mask's on 8, float32: 4).
-bool flat(const Rows& R, int64_t size, const float* noise, int64_t no, int64_t ni) {
-    const int64_t K = R.levels, per = group_rows(K) * K;
-    const bool one = R.rows == R.inner;
-    auto dense = [&](int64_t o, int64_t i) { return (R.inner == 1 || i == K) && (one || o == K * R.inner); };
-    if (!dense(R.so, R.si) || !aligned16(R.logits) || (per * size) % 16) return false;
-    if (R.mask && (R.mask_level != 1 || !dense(R.mo, R.mi) || ((uintptr_t)R.mask & 7) || per % 8)) return false;
-    return !noise || (dense(no, ni) && aligned16(noise) && per % 4 == 0);
-}
+int group_rows(int K) { int n = 256; BY_LEVELS(K, (n = 256 / G, (void)E)); return n; }
 
 // ---- longer rows: a workgroup to a row, or to a part of one -----------------------------------------------------------
 //
@@ -686,6 +752,11 @@ int64_t cut_bytes(const Rows& R, int top) {
     return c.parts > 1 ? R.rows * c.parts * (int64_t)(sizeof(Part) + 8 * top) : 0;
 }
 
+bool dense(const lrn_rows& in, int64_t so, int64_t si) { return (in.inner <= 1 || si == in.levels) && (in.outer <= 1 || so == in.levels * in.inner); }
+int64_t extent(const lrn_rows& in, int64_t so, int64_t si, int64_t levels) {
+    return (in.outer > 0 ? in.outer - 1 : 0) * so + (in.inner > 0 ? in.inner - 1 : 0) * si + levels;
+}
+
 int checked(const lrn_rows* in, Rows* out) {
     if (!in) return fail(-1, "rows: null");
     if (in->outer < 0 || in->inner < 0 || in->levels < 1 || in->levels > 0x3fffffff)
@@ -701,7 +772,11 @@ int checked(const lrn_rows* in, Rows* out) {
     out->mo = in->mask_outer; out->mi = in->mask_inner;
     out->levels = (int32_t)in->levels;
     out->mask_level = in->mask_level;
-    out->per_level = (uint32_t)((0xffffffffull + in->levels) / in->levels);
+    if (in->stride_outer < 0 || in->stride_inner < 0 || in->mask_outer < 0 || in->mask_inner < 0) return fail(-1, "rows: negative strides");
+    out->dense = dense(*in, out->so, out->si);
+    out->mask_dense = out->mask_level == 1 && dense(*in, out->mo, out->mi);
+    out->limit = extent(*in, out->so, out->si, in->levels);
+    out->mask_limit = extent(*in, out->mo, out->mi, out->mask_level ? in->levels : 1);
     return 0;
 }
 
@@ -755,17 +830,16 @@ int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const flo
     if (int rc = checked(rows, &R)) return rc;
     if (!R.rows) return 0;
     if (!level_out || !logprob_out || !entropy_out) return fail(-1, "lrn_choose: null output");
+    if (noise_outer < 0 || noise_inner < 0) return fail(-1, "lrn_choose: negative noise strides");
     if (int rc = check_workspace(cut_bytes(R, 0), workspace, workspace_bytes, "lrn_choose")) return rc;
     LRN_ON_DEVICE(device);
-    const ChooseOut O{noise, noise_outer, noise_inner, level_out, logprob_out, entropy_out};
+    const ChooseOut O{noise, noise_outer, noise_inner, extent(*rows, noise_outer, noise_inner, R.levels),
+                      !noise || dense(*rows, noise_outer, noise_inner), level_out, logprob_out, entropy_out};
     if (R.levels <= kGroupLevels) {
         unsigned grid;
         if (int rc = tiles(R, &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
-        if (flat(R, size_of(rows->dtype), noise, noise_outer, noise_inner))
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, O))))
-        else
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, O))))
+        BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, O))));
         LRN_LAUNCHED("lrn_choose");
         return 0;
     }
@@ -792,10 +866,7 @@ int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int6
         unsigned grid;
         if (int rc = tiles(R, &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
-        if (flat(R, size_of(rows->dtype), nullptr, 0, 0))
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, O))))
-        else
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, O))))
+        BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, O))));
         LRN_LAUNCHED("lrn_score");
         return 0;
     }
@@ -819,11 +890,7 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
         unsigned grid;
         if (int rc = tiles(R, &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
-        const bool out16 = aligned16(grad_out) && (group_rows(R.levels) * (int64_t)R.levels * size_of(rows->dtype)) % 16 == 0;
-        if (flat(R, size_of(rows->dtype), nullptr, 0, 0))
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E, true><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out, out16))))
-        else
-            BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E, false><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out, out16))))
+        BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out))));
         LRN_LAUNCHED("lrn_score_backward");
         return 0;
     }
