@@ -115,7 +115,7 @@ __device__ __forceinline__ const uint8_t* row_mask(const Rows& R, int64_t r) {
 
 // +inf among the allowed logits: no distribution
 __device__ __forceinline__ void finish(Sums& a) { if (a.m == -kNegInf) a.s = __builtin_nanf(""); }
-__device__ __forceinline__ float entropy_of(const Sums& a, float logs) { return a.s != 0.0f ? logs - a.t / a.s : 0.0f; }
+__device__ __forceinline__ float entropy_of(const Sums& a, float logs) { return a.s != 0.0f ? logs - a.t * fast_inverse(a.s) : 0.0f; }
 
 struct ChooseOut { const float* noise; int64_t no, ni, limit; bool dense; int64_t* level; float* logprob; float* entropy; };
 
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) 
     });
     if (g == 0) {
         const bool some = a.s != 0.0f, found = b.j < R.levels;
-        const float logs = logf(a.s);
+        const float logs = fast_log(a.s);
         O.level[r] = some && found ? b.j : 0;
         O.logprob[r] = !some ? 0.0f : found ? chosen - a.m - logs : __builtin_nanf("");
         O.entropy[r] = entropy_of(a, logs);
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void group_score_kernel(Rows R, ScoreOut O) {
     load_levels<T, G, E>(R, off, moff, g, z);
     if (g == 0 && l >= 0 && l < K && !(R.mask && !R.mask[moff + l * R.mask_level])) zl = to_f32(((const T*)R.logits)[off + l]);
     const Sums a = group_sums<G, E>(z, e);
-    const float logs = logf(a.s);
+    const float logs = fast_log(a.s);
     if (g == 0) {
         O.logprob[r] = l >= K ? __builtin_nanf("") : l < 0 || a.s == 0.0f ? 0.0f : zl - a.m - logs;
         O.entropy[r] = entropy_of(a, logs);
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T
         float z[E], e[E];
         load_levels<T, G, E>(R, off, moff, g, z);
         const Sums a = group_sums<G, E>(z, e);
-        const float logs = logf(a.s), inv = 1.0f / a.s, lift = entropy_of(a, logs) - logs, m = a.m;
+        const float logs = fast_log(a.s), inv = fast_inverse(a.s), lift = entropy_of(a, logs) - logs, m = a.m;
         const int mine = l >= 0 && l < K ? (int)l - g * E : -1;
         T* to = out + row * K + g * E;
 #pragma unroll
@@ -481,8 +481,8 @@ __device__ __forceinline__ void load_piece(const T* src, const uint8_t* mk, int 
 
 // f(z, e0) for every piece of a lane; kAhead pieces are asked for before the first is used.
 constexpr int kAhead = 4;
-template <class T, bool MASK, class F>
-__device__ __forceinline__ void over_pieces(const T* src, const uint8_t* mk, int mask_level, int begin, int end, F&& f) {
+template <class T, bool MASK, bool NOISE, class F>
+__device__ __forceinline__ void over_pieces(const T* src, const uint8_t* mk, int mask_level, const float* ns, int begin, int end, F&& f) {
     constexpr int N = Piece<T>::N, STEP = 256 * N;
     using V = typename Piece<T>::vec;
     using M = typename std::conditional_t<N == 8, Mask8, Mask4>::vec;
@@ -491,8 +491,13 @@ __device__ __forceinline__ void over_pieces(const T* src, const uint8_t* mk, int
         const int e0 = base + (int)threadIdx.x * N;
         V v[kAhead];
         M b[kAhead];
+        float w[NOISE ? kAhead : 1][N];
 #pragma unroll
         for (int u = 0; u < kAhead; u++) v[u] = *reinterpret_cast<const V*>(src + e0 + u * STEP);
+        if (NOISE && ns) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) take(ns + e0 + u * STEP, w[NOISE ? u : 0]);
+        }
         if (MASK && mask_level) {
 #pragma unroll
             for (int u = 0; u < kAhead; u++) b[u] = *reinterpret_cast<const M*>(mk + e0 + u * STEP);
@@ -506,14 +511,19 @@ __device__ __forceinline__ void over_pieces(const T* src, const uint8_t* mk, int
             float z[N];
 #pragma unroll
             for (int k = 0; k < N; k++) z[k] = !MASK || b[u][k] ? to_f32(v[u][k]) : kNegInf;
-            f(z, e0 + u * STEP);
+            f(z, w[NOISE ? u : 0], e0 + u * STEP);
         }
     }
     for (; base < end; base += STEP) {
         const int e0 = base + (int)threadIdx.x * N;
         float z[N];
+        float w[N];
         load_piece<T>(src, mk, mask_level, e0, end, z);
-        f(z, e0);
+        if (NOISE && ns) {
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = e0 + k < end ? ns[e0 + k] : 0.0f;
+        }
+        f(z, w, e0);
     }
 }
 
@@ -558,22 +568,25 @@ struct Cut {
 template <class T> __device__ __forceinline__ void put_choice(const Rows& R, const ChooseOut& O, int64_t r, const Sums& a, const Best& b, int lane) {
     if (lane) return;
     const bool some = a.s != 0.0f, found = b.j < R.levels;
-    const float logs = logf(a.s);
+    const float logs = fast_log(a.s);
     O.level[r] = some && found ? b.j : 0;
     O.logprob[r] = !some ? 0.0f : found ? to_f32(((const T*)R.logits + row_base(R, r))[b.j]) - a.m - logs : __builtin_nanf("");
     O.entropy[r] = entropy_of(a, logs);
 }
-template <class T> __device__ __forceinline__ void put_score(const Rows& R, const ScoreOut& O, int64_t r, const Sums& a, const TopList& list, int lane) {
-    const float logs = logf(a.s);
+// (asked for early: two dependent loads)
+struct Given { int64_t l; float z; };
+template <class T> __device__ __forceinline__ Given given_level(const Rows& R, const ScoreOut& O, int64_t r) {
+    Given x{O.level[r], kNegInf};
+    if (x.l >= 0 && x.l < R.levels) {
+        const uint8_t* mk = row_mask(R, r);
+        if (!mk || mk[x.l * R.mask_level]) x.z = to_f32(((const T*)R.logits + row_base(R, r))[x.l]);
+    }
+    return x;
+}
+template <class T> __device__ __forceinline__ void put_score(const Rows& R, const ScoreOut& O, int64_t r, const Given& x, const Sums& a, const TopList& list, int lane) {
+    const float logs = fast_log(a.s);
     if (lane == 0) {
-        const int64_t l = O.level[r];
-        float lp = 0.0f;
-        if (l >= R.levels) lp = __builtin_nanf("");
-        else if (l >= 0 && a.s != 0.0f) {
-            const uint8_t* mk = row_mask(R, r);
-            lp = (mk && !mk[l * R.mask_level] ? kNegInf : to_f32(((const T*)R.logits + row_base(R, r))[l])) - a.m - logs;
-        }
-        O.logprob[r] = lp;
+        O.logprob[r] = x.l >= R.levels ? __builtin_nanf("") : x.l < 0 || a.s == 0.0f ? 0.0f : x.z - a.m - logs;
         O.entropy[r] = entropy_of(a, logs);
         if (O.stat) { O.stat[2 * r] = a.m; O.stat[2 * r + 1] = a.s; }
     }
@@ -607,12 +620,16 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
     TopList list;
     list.clear();
     const int top = CHOOSE ? 0 : O.top;
-    over_pieces<T, MASK>(src, mk, R.mask_level, begin, end, [&](const float (&z)[N], int e0) {
+    Given given{};
+    if (!CHOOSE && cut.parts == 1 && tid == 0) given = given_level<T>(R, O, r);
+    over_pieces<T, MASK, CHOOSE>(src, mk, R.mask_level, ns, begin, end, [&](const float (&z)[N], const float (&w)[N], int e0) {
         add_piece(a, z);
         if constexpr (CHOOSE) {
 #pragma unroll
-            for (int k = 0; k < N; k++)
-                if (z[k] != kNegInf) b.add(ns ? z[k] + ns[e0 + k] : z[k], e0 + k);
+            for (int k = 0; k < N; k++) {                        // (a lane's levels rise)
+                const float key = ns ? z[k] + w[k] : z[k];
+                if (z[k] > kNegInf && key > b.v) { b.v = key; b.j = e0 + k; }
+            }
         }
     });
     if (top) {
@@ -621,7 +638,7 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
         maxima[tid] = a.m;
         __syncthreads();
         list.clear(nth_of_256({maxima[lane], maxima[lane + 64], maxima[lane + 128], maxima[lane + 192]}, top));
-        over_pieces<T, MASK>(src, mk, R.mask_level, begin, end, [&](const float (&z)[N], int e0) {      // (whole wavefronts)
+        over_pieces<T, MASK, false>(src, mk, R.mask_level, nullptr, begin, end, [&](const float (&z)[N], const float (&)[N], int e0) {      // (whole wavefronts)
             float best = z[0];
 #pragma unroll
             for (int k = 1; k < N; k++) best = fmaxf(best, z[k]);
@@ -646,7 +663,7 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
     if (cut.parts == 1) {
         finish(a);
         if constexpr (CHOOSE) put_choice<T>(R, C, r, a, b, lane);
-        else put_score<T>(R, O, r, a, list, lane);
+        else put_score<T>(R, O, r, given, a, list, lane);
     } else {
         if (lane == 0) cut.part[blockIdx.x] = Part{a.m, a.s, a.t, b.v, b.j};
         if (lane < top) { cut.top_v[(int64_t)blockIdx.x * top + lane] = list.v; cut.top_j[(int64_t)blockIdx.x * top + lane] = list.j; }
@@ -657,15 +674,17 @@ template <class T, bool CHOOSE>
 __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut O, Cut cut) {
     const int lane = threadIdx.x;
     const int64_t r = blockIdx.x;
+    Given given{};
+    if (!CHOOSE && lane == 0) given = given_level<T>(R, O, r);
     Part mine{kNegInf, 0.0f, 0.0f, kNegInf, 0x7fffffff};
     if (lane < cut.parts) mine = cut.part[r * cut.parts + lane];
     Sums a{mine.m, mine.s, mine.t};
     Best b{mine.v, mine.j};
     TopList list;
     list.clear();
-    wave_join(a);
-    finish(a);
     if constexpr (CHOOSE) {
+        wave_join(a);
+        finish(a);
         over_group<64>([&](auto from) { b.add(from(b.v), from(b.j)); });
         put_choice<T>(R, C, r, a, b, lane);
     } else {
@@ -680,6 +699,8 @@ __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut 
         float v, next_v;
         int j, next_j;
         fetch(lane, next_v, next_j);
+        wave_join(a);
+        finish(a);
         for (int k0 = 0; k0 < n; k0 += 64) {
             v = next_v;
             j = next_j;
@@ -687,7 +708,7 @@ __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut 
             fetch(k0 + 64 + lane, next_v, next_j);
             list.offer(v, j, top, lane);
         }
-        put_score<T>(R, O, r, a, list, lane);
+        put_score<T>(R, O, r, given, a, list, lane);
     }
 }
 
@@ -706,8 +727,8 @@ __global__ __launch_bounds__(256) void wide_backward_kernel(Rows R, BackIn I, T*
     const float m = I.stat[2 * r], s = I.stat[2 * r + 1], H = I.entropy[r];
     const int64_t l = I.level[r];
     float g = I.g_lp && l >= 0 ? I.g_lp[r * I.g_lp_stride] : 0.0f;
-    const float gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f, inv = s != 0.0f ? 1.0f / s : 0.0f;
-    const float lift = s != 0.0f ? H - logf(s) : 0.0f;           // log p + H = z - m + lift
+    const float gh = I.g_h ? I.g_h[r * I.g_h_stride] : 0.0f, inv = s != 0.0f ? fast_inverse(s) : 0.0f;
+    const float lift = s != 0.0f ? H - fast_log(s) : 0.0f;           // log p + H = z - m + lift
     if (l >= R.levels) g = __builtin_nanf("");
 #pragma unroll
     for (int n = 0; n < kBackPieces; n++) {

@@ -55,6 +55,10 @@ constexpr double kLog2e = 1.4426950408889634;
 // |x| 2^-24 + 1 unit): the weights below are exp(z - max), where a large |x| is a small weight.
 __device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * (float)kLog2e); }
 
+// log(s) of a sum of weights (1 <= s, or 0: -inf) on the logarithm unit, 1 unit and one rounding off; 1 / s likewise.
+__device__ __forceinline__ float fast_log(float s) { return __builtin_amdgcn_logf(s) * 0.6931471805599453f; }
+__device__ __forceinline__ float fast_inverse(float s) { return __builtin_amdgcn_rcpf(s); }
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace lrn
