@@ -96,8 +96,8 @@ int lrn_scan(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_vie
              double gate_const, const lrn_view* resets, const void* initial, const lrn_view* h_out, void* final_out,
              void* workspace, int64_t workspace_bytes);
 /* Gradients: G_t = g_h_t + a_{t+1} G_{t+1} with g_final behind the last step;  grad_x = G, grad_gate_t = G_t h_{t-1}
- * (0 at a reset), grad_initial = a_0 G_0.  g_h / g_final may be NULL (zero; not both), grad_gate is wanted only with a
- * gate tensor; every output may be NULL. */
+ * (0 at a reset), grad_initial = a_0 G_0.  g_final NULL = zero; grad_gate (wanted only with a gate tensor; then h is read) and
+ * grad_initial may be NULL.  h and g_final are not read where they are not needed. */
 int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const,
                       const lrn_view* resets, const void* initial, const lrn_view* h, const lrn_view* g_h,
                       const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,

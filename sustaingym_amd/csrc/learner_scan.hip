@@ -37,7 +37,7 @@ struct View {
 struct Seq {
     int64_t steps, cols;        // cols = batch * channels, column q = (q / channels, q % channels)
     int64_t channels;
-    View x, gate, resets, before, h, gate_out;
+    View x, gate, resets, before, h, second;
     double gate_const, scale;   // advantages: gamma lam, gamma
     const void* initial;
     const void* edge;           // backward: the initial state; advantages: V behind the last step (float32)
@@ -69,122 +69,159 @@ template <class W> struct Pair {
 
 constexpr int L = 8;             // steps of a lane's run
 
+// One of the three, for one type of elements: whether there is a gate tensor (else a constant), whether there are resets, and
+// whether the second output is wanted.  Compiled in: a condition between loads keeps them from being in flight together.
+template <Kind K_, class T_, bool GATE_, bool RESETS_, bool SECOND_>
+struct Op {
+    static constexpr Kind K = K_;
+    static constexpr bool GATE = GATE_, RESETS = RESETS_, SECOND = SECOND_;
+    using T = T_;
+    using W = typename State<T_>::type;
+    using Out = std::conditional_t<K_ == ADVANTAGES, float, T_>;
+};
+
 // One lane's run, L steps of V adjacent columns: as it comes from memory ...
-template <Kind K, class T, int V>
+template <class O, int V>
 struct Raw {
+    using T = typename O::T;
     static constexpr int N = L * V;
     T x[N];
-    T g[K == ADVANTAGES ? 1 : N];              // SCAN: gate of the step; BACKWARD: of the step before in this order
-    T before[K == BACKWARD ? N : 1];           // the state before the step
-    float v[K == ADVANTAGES ? N + V : 1];      // values of the steps u0 - 1 .. u0 + L - 1
-    uint8_t r[K == BACKWARD ? N + V : N];      // flags of the steps u0 .., BACKWARD: u0 - 1 ..
+    T g[O::GATE ? N : 1];                                  // SCAN: gate of the step; BACKWARD: of the step before in this order
+    T before[O::K == BACKWARD && O::SECOND ? N : 1];       // the state before the step
+    float v[O::K == ADVANTAGES ? N + V : 1];               // values of the steps u0 - 1 .. u0 + L - 1
+    uint8_t r[O::RESETS ? N + V : 1];                      // flags of the steps u0 .., BACKWARD: u0 - 1 ..
 };
 // ... and as it acts
-template <Kind K, class T, int V>
+template <class O, int V>
 struct Run {
-    using W = typename State<T>::type;
+    using W = typename O::W;
     W a[L * V], x[L * V];
-    std::conditional_t<K == ADVANTAGES, float, W> extra[K == SCAN ? 1 : L * V];    // BACKWARD: d h / d gate; ADVANTAGES: V
+    std::conditional_t<O::K == ADVANTAGES, float, W> extra[O::SECOND ? L * V : 1];    // BACKWARD: d h / d gate; ADVANTAGES: V
 };
 
 // A lane's V columns in every view: the part of the address that is the same for the wavefront, and the lane's own.
 struct Place {
     const char *x, *gate, *before, *resets;
-    char *h, *gate_out;
+    char *h, *second;
     uint32_t ox, og, ob, orr, oh, oo;          // bytes
-    uint32_t second;                           // from the first column's flags to the second's
+    uint32_t next_flags;                       // from the first column's flags to the second's
 };
 
 // ---- COLUMNS: loads and stores ------------------------------------------------------------------------------------------
 
+typedef const char __attribute__((address_space(1)))* Global;
 template <class E, int V> struct Vec { typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E)))); };
 
-template <class E, int V> __device__ __forceinline__ void get(const char* base, uint32_t lane, E* to) {
-    if constexpr (V == 1) to[0] = *reinterpret_cast<const E*>(base + lane);
+template <class E, int V> __device__ __forceinline__ void get(Global base, uint32_t lane, E* to) {
+    if constexpr (V == 1) to[0] = *(const E __attribute__((address_space(1)))*)(base + lane);
     else {
-        const typename Vec<E, V>::type w = *reinterpret_cast<const typename Vec<E, V>::type*>(base + lane);
+        typedef typename Vec<E, V>::type vec;
+        const vec w = *(const vec __attribute__((address_space(1)))*)(base + lane);
 #pragma unroll
         for (int k = 0; k < V; k++) to[k] = w[k];
     }
 }
-template <class E, int V> __device__ __forceinline__ void put(char* base, uint32_t lane, const E* from) {
-    if constexpr (V == 1) *reinterpret_cast<E*>(base + lane) = from[0];
+template <class E, int V> __device__ __forceinline__ void put(Global base, uint32_t lane, const E* from) {
+    if constexpr (V == 1) *(E __attribute__((address_space(1)))*)(base + lane) = from[0];
     else {
-        typename Vec<E, V>::type w;
+        typedef typename Vec<E, V>::type vec;
+        vec w;
 #pragma unroll
         for (int k = 0; k < V; k++) w[k] = from[k];
-        *reinterpret_cast<typename Vec<E, V>::type*>(base + lane) = w;
+        *(vec __attribute__((address_space(1)))*)(base + lane) = w;
     }
 }
 
 // One step further, by a scalar addition at its place: eight multiples of every stride kept ready would not fit the scalar
-// registers, and come back from vector lanes at two instructions a piece.
-template <class P> __device__ __forceinline__ void advance(P& p, int64_t bytes) {
+// registers, and come back from vector lanes at two instructions a piece.  (Behind the asm only the type says what memory it is.)
+__device__ __forceinline__ void advance(Global& p, int64_t bytes) {
     p += bytes;
     asm("" : "+s"(p));
 }
 
-// COUNT steps from `from`; FULL: all of them lie in [lo, hi), else what does not is left as it is
-template <class E, int V, int COUNT, bool FULL>
-__device__ __forceinline__ void get_steps(const char* base, int64_t st, uint32_t lane, int64_t from, int64_t lo, int64_t hi, E* to) {
-    const char* p = base + from * st * (int64_t)sizeof(E);
+// How many of `count` steps from `from` lie in front of `to`, and in it.
+__device__ __forceinline__ int in_front(int64_t from, int64_t to, int count) { return to <= from ? 0 : to - from < count ? (int)(to - from) : count; }
+
+// The lane's part of an address, as the 32-bit half of a load that has its other half in scalar registers: known to be
+// invariant it would be added to the base ahead of the loop, and every load would add 64 bits in vector registers.
+__device__ __forceinline__ uint32_t kept_apart(uint32_t lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// COUNT steps from `from`.  FULL: all of them are there, but with BEFORE the first may lie in front of step 0 and with BEHIND the
+// last at `hi`: its neighbour is read in its place, and whoever uses it knows.  Not FULL: what lies outside [0, hi) is 0.
+template <class E, int V, int COUNT, bool FULL, bool BEFORE = false, bool BEHIND = false>
+__device__ __forceinline__ void get_steps(const char* base, int64_t st, uint32_t lane, int64_t from, int64_t hi, E* to) {
+    const int64_t stride = st * (int64_t)sizeof(E);
+    const bool short_front = FULL && BEFORE && from < 0, short_back = FULL && BEHIND && from + COUNT > hi;
+    Global p = (Global)(base + (short_front ? 0 : from * stride));
+    lane = kept_apart(lane);
+    const int first = FULL ? 0 : in_front(from, 0, COUNT), last = FULL ? COUNT : in_front(from, hi, COUNT);
 #pragma unroll
     for (int i = 0; i < COUNT; i++) {
-        if (FULL || (from + i >= lo && from + i < hi)) get<E, V>(p, lane, to + i * V);
-        advance(p, st * (int64_t)sizeof(E));
+        if constexpr (!FULL) {
+#pragma unroll
+            for (int k = 0; k < V; k++) to[i * V + k] = E(0);
+        }
+        if (FULL || (i >= first && i < last)) get<E, V>(p, lane, to + i * V);
+        if (i + 1 < COUNT) advance(p, (i == 0 && short_front) || (i == COUNT - 2 && short_back) ? 0 : stride);
     }
 }
 
 // Steps u0 .. u0 + L - 1 as they are in memory.
-template <Kind K, class T, int V, bool FULL, bool APPLYING>
-__device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t q, int64_t u0, int64_t end, Raw<K, T, V>& d) {
-    constexpr int shift = K == BACKWARD ? 1 : 0, COUNT = L + shift;
-    if (P.x) get_steps<T, V, L, FULL>(P.x, S.x.st, P.ox, u0, 0, end, d.x);
-    if constexpr (K != ADVANTAGES)
-        if (P.gate) get_steps<T, V, L, FULL>(P.gate, S.gate.st, P.og, u0 - shift, 0, end, d.g);
-    if (P.resets) {
-        const char* p = P.resets + (u0 - shift) * S.resets.st;
+template <class O, int V, bool FULL, bool APPLYING>
+__device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<O, V>& d) {
+    using T = typename O::T;
+    constexpr int shift = O::K == BACKWARD ? 1 : 0;
+    constexpr bool back = O::K == BACKWARD;
+    get_steps<T, V, L, FULL>(P.x, S.x.st, P.ox, u0, end, d.x);
+    if constexpr (O::GATE) get_steps<T, V, L, FULL, back>(P.gate, S.gate.st, P.og, u0 - shift, end, d.g);
+    if constexpr (O::RESETS) {
+        constexpr int COUNT = L + (O::K == BACKWARD && O::SECOND ? 1 : 0);
+        if constexpr (V == 1) get_steps<uint8_t, 1, COUNT, FULL, back>(P.resets, S.resets.st, P.orr, u0 - shift, end, d.r);
+        else {
+            // (two sequences' flags are adjacent or the same)
+            uint8_t one[V][COUNT];
 #pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            if (FULL || (u0 - shift + i >= 0 && u0 - shift + i < end)) {
+            for (int k = 0; k < V; k++) get_steps<uint8_t, 1, COUNT, FULL, back>(P.resets, S.resets.st, P.orr + k * P.next_flags, u0 - shift, end, one[k]);
 #pragma unroll
-                for (int k = 0; k < V; k++) d.r[i * V + k] = *reinterpret_cast<const uint8_t*>(p + (P.orr + k * P.second));
-            }
-            advance(p, S.resets.st);
+            for (int i = 0; i < COUNT * V; i++) d.r[i] = one[i % V][i / V];
         }
     }
-    if constexpr (K == ADVANTAGES) get_steps<float, V, L + 1, FULL>(P.before, S.before.st, P.ob, u0 - 1, 0, end, d.v);
-    if constexpr (K == BACKWARD && APPLYING)
-        if (P.gate_out) get_steps<T, V, L, FULL>(P.before, S.before.st, P.ob, u0 + 1, 0, S.steps, d.before);
+    if constexpr (O::K == ADVANTAGES) get_steps<float, V, L + 1, FULL, true>(P.before, S.before.st, P.ob, u0 - 1, end, d.v);
+    if constexpr (O::K == BACKWARD && O::SECOND && APPLYING) get_steps<T, V, L, FULL, false, true>(P.before, S.before.st, P.ob, u0 + 1, S.steps, d.before);
 }
 
 // What the steps do.  Behind the end: a = 1, x = 0, so that a run that is cut short has the pair of what it holds.
-template <Kind K, class T, int V, bool FULL>
-__device__ __forceinline__ void fold(const Seq& S, const Place& P, const Raw<K, T, V>& d, const typename State<T>::type (&edge)[V], int64_t u0, int64_t end,
-                                     Run<K, T, V>& f) {
-    using W = typename State<T>::type;
+template <class O, int V, bool FULL>
+__device__ __forceinline__ void fold(const Seq& S, const Raw<O, V>& d, const typename O::W (&edge)[V], int64_t u0, int64_t end, Run<O, V>& f) {
+    using W = typename O::W;
+    const int count = FULL ? L : in_front(u0, end, L), final_step = in_front(u0 + 1, S.steps, L);
 #pragma unroll
     for (int i = 0; i < L; i++) {
-        const bool in = FULL || u0 + i < end;
+        const bool in = FULL || i < count;
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const int n = i * V + k;
-            const bool cut = P.resets && d.r[n];
-            W x = P.x ? (W)d.x[n] : W(0), a;
-            if constexpr (K == ADVANTAGES) {
-                const W now = (W)d.v[n + V], next = !FULL && u0 + i == 0 ? edge[k] : (W)d.v[n];
+            W x = (W)d.x[n], a = (W)S.gate_const;
+            bool cut = false;
+            if constexpr (O::RESETS) cut = d.r[n] != 0;
+            if constexpr (O::GATE) a = (W)d.g[n];
+            if constexpr (O::K == ADVANTAGES) {
+                const W now = (W)d.v[n + V], next = i == 0 && u0 == 0 ? edge[k] : (W)d.v[n];
                 x = cut ? x - now : x + (W)S.scale * next - now;
-                a = cut ? W(0) : (W)S.gate_const;
                 f.extra[n] = d.v[n + V];
-            } else {
-                a = P.gate ? (W)d.g[n] : (W)S.gate_const;
-                if (cut) a = W(0);
             }
-            if constexpr (K == BACKWARD) {
-                if (!FULL && u0 + i == 0) a = W(1);                        // g_final enters as it is
-                W prev = (W)d.before[n];
-                if (!FULL && u0 + i + 1 == S.steps) prev = edge[k];
-                f.extra[n] = P.resets && d.r[n + V] ? W(0) : prev;
+            if (cut) a = W(0);
+            if constexpr (O::K == BACKWARD) {
+                if (i == 0 && u0 == 0) a = W(1);                        // g_final enters as it is
+                if constexpr (O::SECOND) {
+                    W prev = (W)d.before[n];
+                    if (FULL ? i == L - 1 && final_step < L : i == final_step) prev = edge[k];
+                    if constexpr (O::RESETS) prev = d.r[n + V] ? W(0) : prev;
+                    f.extra[n] = prev;
+                }
             }
             f.a[n] = in ? a : W(1);
             f.x[n] = in ? x : W(0);
@@ -192,65 +229,67 @@ __device__ __forceinline__ void fold(const Seq& S, const Place& P, const Raw<K, 
     }
 }
 
-template <Kind K, class T, int V> __device__ __forceinline__ Pair<typename State<T>::type> pair_of(const Run<K, T, V>& f, int k) {
-    using W = typename State<T>::type;
-    Pair<W> p{W(1), W(0)};
+template <class O, int V, bool FULL, bool APPLYING>
+__device__ __forceinline__ void take(const Seq& S, const Place& P, const typename O::W (&edge)[V], int64_t u0, int64_t end, Run<O, V>& f) {
+    Raw<O, V> raw;
+    load<O, V, FULL, APPLYING>(S, P, u0, end, raw);
+    fold<O, V, FULL>(S, raw, edge, u0, end, f);
+}
+
+template <class O, int V> __device__ __forceinline__ Pair<typename O::W> pair_of(const Run<O, V>& f, int k) {
+    Pair<typename O::W> p{f.a[k], f.x[k]};
 #pragma unroll
-    for (int i = 0; i < L; i++) p.then(f.a[i * V + k], f.x[i * V + k]);
+    for (int i = 1; i < L; i++) p.then(f.a[i * V + k], f.x[i * V + k]);
     return p;
 }
 
-// The outputs of step i from the state behind it.
-template <Kind K, class T, int V, class O> __device__ __forceinline__ O second_of(const Run<K, T, V>& f, int n, typename State<T>::type h) {
-    using W = typename State<T>::type;
-    if constexpr (K == BACKWARD) return (O)(h * f.extra[n]);
-    else return (O)(h + (W)f.extra[n]);
+// The second output of a step from the state behind it.
+template <class O, int V> __device__ __forceinline__ typename O::Out second_of(const Run<O, V>& f, int n, typename O::W h) {
+    using W = typename O::W;
+    if constexpr (O::K == BACKWARD) return (typename O::Out)(h * f.extra[n]);
+    else return (typename O::Out)(h + (W)f.extra[n]);
 }
 
 // Walks the run from the state in front of it and writes.
-template <Kind K, class T, int V, bool FULL>
-__device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<K, T, V>& f, int64_t u0, int64_t end, typename State<T>::type (&h)[V]) {
-    using O = std::conditional_t<K == ADVANTAGES, float, T>;
-    char* ph = P.h + u0 * S.h.st * (int64_t)sizeof(O);
-    char* po = P.gate_out + u0 * S.gate_out.st * (int64_t)sizeof(O);
+template <class O, int V, bool FULL>
+__device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, V>& f, int64_t u0, int64_t end, typename O::W (&h)[V]) {
+    using E = typename O::Out;
+    Global ph = (Global)(P.h + u0 * S.h.st * (int64_t)sizeof(E)), po = (Global)(P.second + u0 * S.second.st * (int64_t)sizeof(E));
+    const int last = FULL ? L : in_front(u0, end, L);
+    const uint32_t oh = kept_apart(P.oh), oo = O::SECOND ? kept_apart(P.oo) : 0;
 #pragma unroll
     for (int i = 0; i < L; i++) {
-        O out[V], second[V];
+        E out[V], second[V];
 #pragma unroll
         for (int k = 0; k < V; k++) {
             h[k] = step(f.a[i * V + k], h[k], f.x[i * V + k]);
-            out[k] = (O)h[k];
-            if constexpr (K != SCAN) second[k] = second_of<K, T, V, O>(f, i * V + k, h[k]);
+            out[k] = (E)h[k];
+            if constexpr (O::SECOND) second[k] = second_of<O, V>(f, i * V + k, h[k]);
         }
-        if (FULL || u0 + i < end) {
-            if (P.h) put<O, V>(ph, P.oh, out);
-            if constexpr (K != SCAN)
-                if (P.gate_out) put<O, V>(po, P.oo, second);
+        if (FULL || i < last) {
+            put<E, V>(ph, oh, out);
+            if constexpr (O::SECOND) put<E, V>(po, oo, second);
         }
-        advance(ph, S.h.st * (int64_t)sizeof(O));
-        if constexpr (K != SCAN) advance(po, S.gate_out.st * (int64_t)sizeof(O));
+        advance(ph, S.h.st * (int64_t)sizeof(E));
+        if constexpr (O::SECOND) advance(po, S.second.st * (int64_t)sizeof(E));
     }
-}
-
-// Whether the turn of `length` steps from u lies inside in every respect: its own steps, the one before and the one behind.
-template <Kind K> __device__ __forceinline__ bool inside(const Seq& S, int64_t u, int64_t length, int64_t end) {
-    return u + length <= end && (K == SCAN || u > 0) && (K != BACKWARD || u + length < S.steps);
 }
 
 template <class E> __device__ __forceinline__ const char* uniform_part(const View& v, int64_t b) { return v.p ? (const char*)v.p + b * v.sb * (int64_t)sizeof(E) : nullptr; }
 template <class E> __device__ __forceinline__ uint32_t lane_part(const View& v, int64_t b, int64_t c) { return (uint32_t)((b * v.sb + c * v.sc) * (int64_t)sizeof(E)); }
 
 // Column q = (b, c) seen from sequence b0.
-template <Kind K, class T> __device__ __forceinline__ Place place_of(const Seq& S, int64_t b0, int64_t b, int64_t c) {
-    using O = std::conditional_t<K == ADVANTAGES, float, T>;
+template <class O> __device__ __forceinline__ Place place_of(const Seq& S, int64_t b0, int64_t b, int64_t c) {
+    using T = typename O::T;
+    using E = typename O::Out;
     Place P;
     P.x = uniform_part<T>(S.x, b0); P.ox = lane_part<T>(S.x, b - b0, c);
     P.gate = uniform_part<T>(S.gate, b0); P.og = lane_part<T>(S.gate, b - b0, c);
-    P.before = uniform_part<O>(S.before, b0); P.ob = lane_part<O>(S.before, b - b0, c);
+    P.before = uniform_part<E>(S.before, b0); P.ob = lane_part<E>(S.before, b - b0, c);
     P.resets = uniform_part<uint8_t>(S.resets, b0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
-    P.h = (char*)uniform_part<O>(S.h, b0); P.oh = lane_part<O>(S.h, b - b0, c);
-    P.gate_out = (char*)uniform_part<O>(S.gate_out, b0); P.oo = lane_part<O>(S.gate_out, b - b0, c);
-    P.second = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
+    P.h = (char*)uniform_part<E>(S.h, b0); P.oh = lane_part<E>(S.h, b - b0, c);
+    P.second = (char*)uniform_part<E>(S.second, b0); P.oo = lane_part<E>(S.second, b - b0, c);
+    P.next_flags = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
     return P;
 }
 
@@ -290,9 +329,11 @@ template <Kind K, class T, class W> __device__ __forceinline__ void put_final(co
 
 // ---- COLUMNS: 64 V columns to a wavefront, WT wavefronts of a workgroup one behind the other in time -----------------------
 
-template <Kind K, class T, int V, int WT, Phase PH>
+template <class O, int V, int WT, Phase PH>
 __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S) {
-    using W = typename State<T>::type;
+    constexpr Kind K = O::K;
+    using T = typename O::T;
+    using W = typename O::W;
     constexpr int WC = WT == 1 ? 4 : 1;               // tiles of columns to a workgroup
     constexpr int64_t TURN = WT * L;
     __shared__ Pair<W> pairs_of[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1];
@@ -317,7 +358,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     if (q >= S.cols) return;                          // WT = 1: a whole wavefront behind the last tile
     const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
     const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Place P = place_of<K, T>(S, b0, b, c);
+    const Place P = place_of<O>(S, b0, b, c);
     W carry[V], edge[V];
     Pair<W> all[V];
 #pragma unroll
@@ -326,13 +367,6 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
         edge[k] = edge_of<K, W>(S, q + k);
         all[k] = Pair<W>{W(1), W(0)};
     }
-    Raw<K, T, V> raw;
-    bool full = inside<K>(S, begin, TURN, end);
-    auto fetch = [&](int64_t u0) {
-        if (full) load<K, T, V, true, PH != PAIRS>(S, P, q, u0, end, raw);
-        else load<K, T, V, false, PH != PAIRS>(S, P, q, u0, end, raw);
-    };
-    fetch(begin + wt * L);
     if constexpr (PH == APPLY) {
         // what came before this part: a wavefront joins its share of the parts, the workgroup the wavefronts'
         const int64_t share = (part + WT - 1) / WT, from = min(wt * share, part), to = min(from + share, part);
@@ -352,18 +386,14 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     int turn = 0;
     for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
         const int64_t u0 = u + wt * L;
-        Run<K, T, V> f;
-        const bool now_full = full;
-        if (now_full) fold<K, T, V, true>(S, P, raw, edge, u0, end, f);
-        else fold<K, T, V, false>(S, P, raw, edge, u0, end, f);
-        if (u + TURN < end) {                         // the next turn is on its way while this one is worked on
-            full = inside<K>(S, u + TURN, TURN, end);
-            fetch(u0 + TURN);
-        }
+        const bool full = u0 + L <= end;                  // (the same for the wavefront)
+        Run<O, V> f;
+        if (full) take<O, V, true, PH != PAIRS>(S, P, edge, u0, end, f);
+        else take<O, V, false, PH != PAIRS>(S, P, edge, u0, end, f);
         W mine[V];
         if constexpr (WT > 1) {
 #pragma unroll
-            for (int k = 0; k < V; k++) pairs_of[turn][wt][lane * V + k] = pair_of<K, T, V>(f, k);
+            for (int k = 0; k < V; k++) pairs_of[turn][wt][lane * V + k] = pair_of<O, V>(f, k);
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < V; k++) {
@@ -390,8 +420,8 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
         }
         if constexpr (PH != PAIRS) {
             if (there) {
-                if (now_full) walk<K, T, V, true>(S, P, f, u0, end, mine);
-                else walk<K, T, V, false>(S, P, f, u0, end, mine);
+                if (full) walk<O, V, true>(S, P, f, u0, end, mine);
+                else walk<O, V, false>(S, P, f, u0, end, mine);
             }
             if constexpr (WT == 1) {
 #pragma unroll
@@ -413,9 +443,9 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
 // ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column -----------------------------------------------
 
 // COUNT steps from `from`, 16 bytes at a time (at any alignment); DIR: whether they rise or fall in memory.  Not FULL: one by
-// one, what lies outside [lo, hi) is left as it is.
+// one, what lies outside [0, hi) is 0.
 template <class E, int DIR, int COUNT, bool FULL>
-__device__ __forceinline__ void get_run(const char* base, int64_t from, int64_t lo, int64_t hi, E* to) {
+__device__ __forceinline__ void get_run(const char* base, int64_t from, int64_t hi, E* to) {
     constexpr int VN = (int)(16 / sizeof(E)) < COUNT ? (int)(16 / sizeof(E)) : COUNT;
     const E* p = (const E*)base + (DIR > 0 ? from : -(from + COUNT - 1));
     if constexpr (FULL) {
@@ -427,8 +457,10 @@ __device__ __forceinline__ void get_run(const char* base, int64_t from, int64_t 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < COUNT; i++)
-            if (from + i >= lo && from + i < hi) to[i] = p[DIR > 0 ? i : COUNT - 1 - i];
+        for (int i = 0; i < COUNT; i++) {
+            to[i] = E(0);
+            if (from + i >= 0 && from + i < hi) to[i] = p[DIR > 0 ? i : COUNT - 1 - i];
+        }
     }
 }
 template <class E, int DIR, bool FULL>
@@ -450,37 +482,42 @@ __device__ __forceinline__ void put_run(char* base, int64_t from, int64_t hi, co
     }
 }
 
-template <Kind K, class T, int DIR, bool FULL, bool APPLYING>
-__device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<K, T, 1>& d) {
-    constexpr int shift = K == BACKWARD ? 1 : 0;
-    if (P.x) get_run<T, DIR, L, FULL>(P.x, u0, 0, end, d.x);
-    if constexpr (K != ADVANTAGES)
-        if (P.gate) get_run<T, DIR, L, FULL>(P.gate, u0 - shift, 0, end, d.g);
-    if (P.resets) {
-        get_run<uint8_t, DIR, L, FULL>(P.resets, u0 - shift, 0, end, d.r);
-        if constexpr (K == BACKWARD) get_run<uint8_t, DIR, 1, FULL>(P.resets, u0 - 1 + L, 0, end, d.r + L);
+template <class O, int DIR, bool FULL, bool APPLYING>
+__device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<O, 1>& d) {
+    using T = typename O::T;
+    constexpr int shift = O::K == BACKWARD ? 1 : 0;
+    get_run<T, DIR, L, FULL>(P.x, u0, end, d.x);
+    if constexpr (O::GATE) get_run<T, DIR, L, FULL>(P.gate, u0 - shift, end, d.g);
+    if constexpr (O::RESETS) {
+        get_run<uint8_t, DIR, L, FULL>(P.resets, u0 - shift, end, d.r);
+        if constexpr (O::K == BACKWARD && O::SECOND) get_run<uint8_t, DIR, 1, FULL>(P.resets, u0 - 1 + L, end, d.r + L);
     }
-    if constexpr (K == ADVANTAGES) {
-        get_run<float, DIR, 1, FULL>(P.before, u0 - 1, 0, end, d.v);
-        get_run<float, DIR, L, FULL>(P.before, u0, 0, end, d.v + 1);
+    if constexpr (O::K == ADVANTAGES) {
+        get_run<float, DIR, 1, FULL>(P.before, u0 - 1, end, d.v);
+        get_run<float, DIR, L, FULL>(P.before, u0, end, d.v + 1);
     }
-    if constexpr (K == BACKWARD && APPLYING)
-        if (P.gate_out) get_run<T, DIR, L, FULL>(P.before, u0 + 1, 0, S.steps, d.before);
+    if constexpr (O::K == BACKWARD && O::SECOND && APPLYING) get_run<T, DIR, L, FULL>(P.before, u0 + 1, S.steps, d.before);
 }
 
-template <Kind K, class T, int DIR, bool FULL>
-__device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<K, T, 1>& f, int64_t u0, int64_t end, typename State<T>::type h) {
-    using O = std::conditional_t<K == ADVANTAGES, float, T>;
-    O out[L], second[K == SCAN ? 1 : L];
+template <class O, int DIR, bool FULL, bool APPLYING>
+__device__ __forceinline__ void take_run(const Seq& S, const Place& P, const typename O::W (&edge)[1], int64_t u0, int64_t end, Run<O, 1>& f) {
+    Raw<O, 1> raw;
+    load_run<O, DIR, FULL, APPLYING>(S, P, u0, end, raw);
+    fold<O, 1, FULL>(S, raw, edge, u0, end, f);
+}
+
+template <class O, int DIR, bool FULL>
+__device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<O, 1>& f, int64_t u0, int64_t end, typename O::W h) {
+    using E = typename O::Out;
+    E out[L], second[O::SECOND ? L : 1];
 #pragma unroll
     for (int i = 0; i < L; i++) {
         h = step(f.a[i], h, f.x[i]);
-        out[i] = (O)h;
-        if constexpr (K != SCAN) second[i] = second_of<K, T, 1, O>(f, i, h);
+        out[i] = (E)h;
+        if constexpr (O::SECOND) second[i] = second_of<O, 1>(f, i, h);
     }
-    if (P.h) put_run<O, DIR, FULL>(P.h, u0, end, out);
-    if constexpr (K != SCAN)
-        if (P.gate_out) put_run<O, DIR, FULL>(P.gate_out, u0, end, second);
+    put_run<E, DIR, FULL>(P.h, u0, end, out);
+    if constexpr (O::SECOND) put_run<E, DIR, FULL>(P.second, u0, end, second);
 }
 
 template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
@@ -492,9 +529,11 @@ template <class W> __device__ __forceinline__ void wave_scan(Pair<W>& p, int lan
     }
 }
 
-template <Kind K, class T, int DIR, int WT, Phase PH>
+template <class O, int DIR, int WT, Phase PH>
 __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
-    using W = typename State<T>::type;
+    constexpr Kind K = O::K;
+    using T = typename O::T;
+    using W = typename O::W;
     constexpr int64_t TURN = WT * 64 * L;
     __shared__ W pa[2][WT], ph[2][WT];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
@@ -502,18 +541,11 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     if (q >= S.cols) return;                          // WT > 1: a whole workgroup, else a whole wavefront and no barrier
     const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
     const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Place P = place_of<K, T>(S, q, q, 0);       // (one channel: the column is the sequence)
+    const Place P = place_of<O>(S, q, q, 0);       // (one channel: the column is the sequence)
     W carry = first_state<K, W>(S, q);
     const W edge[1] = {edge_of<K, W>(S, q)};
     Pair<W> all{W(1), W(0)};
     const int64_t mine = (int64_t)(wt * 64 + lane) * L;
-    Raw<K, T, 1> raw;
-    bool full = inside<K>(S, begin, TURN, end);
-    auto fetch = [&](int64_t u0) {
-        if (full) load_run<K, T, DIR, true, PH != PAIRS>(S, P, u0, end, raw);
-        else load_run<K, T, DIR, false, PH != PAIRS>(S, P, u0, end, raw);
-    };
-    fetch(begin + mine);
     if constexpr (PH == APPLY) {
         const int64_t share = (part + WT * 64 - 1) / (WT * 64), from = min((wt * 64 + lane) * share, part), to = min(from + share, part);
         Pair<W> p = joined_parts<W>(S, from, to, q);
@@ -525,16 +557,13 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     }
     int turn = 0;
     for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
-        const int64_t u0 = u + mine;
-        Run<K, T, 1> f;
-        const bool now_full = full;
-        if (now_full) fold<K, T, 1, true>(S, P, raw, edge, u0, end, f);
-        else fold<K, T, 1, false>(S, P, raw, edge, u0, end, f);
-        if (u + TURN < end) {
-            full = inside<K>(S, u + TURN, TURN, end);
-            fetch(u0 + TURN);
-        }
-        Pair<W> p = pair_of<K, T, 1>(f, 0);
+        const int64_t u0 = u + mine, first = u + (int64_t)wt * 64 * L;
+        // all lanes' steps, the ones before them and the ones behind them are there (the same for the wavefront)
+        const bool full = first + 64 * L <= end && (K == SCAN || first > 0) && (K != BACKWARD || first + 64 * L < S.steps);
+        Run<O, 1> f;
+        if (full) take_run<O, DIR, true, PH != PAIRS>(S, P, edge, u0, end, f);
+        else take_run<O, DIR, false, PH != PAIRS>(S, P, edge, u0, end, f);
+        Pair<W> p = pair_of<O, 1>(f, 0);
         wave_scan(p, lane);
         Pair<W> front = up(p, 1);                     // of the lanes before this one
         if (lane == 0) front = Pair<W>{W(1), W(0)};
@@ -556,8 +585,8 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
         } else {
             const W h = step(front.a, carry, front.h);
             carry = step(whole.a, carry, whole.h);
-            if (now_full) walk_run<K, T, DIR, true>(S, P, f, u0, end, h);
-            else walk_run<K, T, DIR, false>(S, P, f, u0, end, h);
+            if (full) walk_run<O, DIR, true>(S, P, f, u0, end, h);
+            else walk_run<O, DIR, false>(S, P, f, u0, end, h);
         }
     }
     if (wt || lane) return;
@@ -632,81 +661,101 @@ int64_t pair_bytes(const lrn_seq* q) {
     return parts > 1 ? parts * 2 * cols * (q->dtype == LRN_F64 ? 8 : 4) : 0;
 }
 
+// 16 wavefronts of a workgroup have 128 registers each, which float64 states and elements do not fit: 8 there.
+template <class O> constexpr int kMany = std::is_same<typename O::T, double>::value ? 8 : 16;
+
 // A lane's part of an address has 32 bits: how far the columns of one tile lie apart in a view.
 bool near(const View& v, const Seq& S, int64_t size, int tile) {
     const int64_t over = std::min(S.cols / S.channels - 1, tile / S.channels + 1);
     return !v.p || (v.sb <= ((int64_t)1 << 40) && over * v.sb * size + S.channels * v.sc * size < ((int64_t)1 << 32));
 }
 
-// 16 wavefronts of a workgroup have 128 registers each, which the float64 backward pass does not fit: 8 there.
-template <Kind K, class T> constexpr int kMany = K == BACKWARD && std::is_same<T, double>::value ? 8 : 16;
-
-template <Kind K, class T, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
-    const bool flat = near(S.x, S, sizeof(T), 64 * V) && near(S.gate, S, sizeof(T), 64 * V) && near(S.before, S, sizeof(T), 64 * V) &&
-                      near(S.resets, S, 1, 64 * V) && near(S.h, S, sizeof(T), 64 * V) && near(S.gate_out, S, sizeof(T), 64 * V);
+template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
+    constexpr int64_t n = sizeof(typename O::T);
+    const bool flat = near(S.x, S, n, 64 * V) && near(S.gate, S, n, 64 * V) && near(S.before, S, n, 64 * V) && near(S.resets, S, 1, 64 * V) &&
+                      near(S.h, S, n, 64 * V) && near(S.second, S, n, 64 * V);
     S.tight = flat ? 0 : cdiv(S.channels, 64 * V);
     const int64_t tiles = cdiv(flat ? cdiv(S.cols, 64 * V) : S.cols / S.channels * S.tight, WT == 1 ? 4 : 1);
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
-        if constexpr (WT == kMany<K, T>) {
-            columns_kernel<K, T, V, WT, PAIRS><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
-            columns_kernel<K, T, V, WT, APPLY><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
+        if constexpr (WT == kMany<O>) {
+            columns_kernel<O, V, WT, PAIRS><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
+            columns_kernel<O, V, WT, APPLY><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
         }
-    } else columns_kernel<K, T, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
+    } else columns_kernel<O, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
 }
-template <Kind K, class T, int DIR, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
+template <class O, int DIR, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
     const int64_t blocks = WT == 1 ? cdiv(S.cols, 4) : S.cols;
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
-        if constexpr (WT == kMany<K, T>) {
-            runs_kernel<K, T, DIR, WT, PAIRS><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
-            runs_kernel<K, T, DIR, WT, APPLY><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
+        if constexpr (WT == kMany<O>) {
+            runs_kernel<O, DIR, WT, PAIRS><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
+            runs_kernel<O, DIR, WT, APPLY><<<dim3((unsigned)blocks, (unsigned)d.parts), threads, 0, stream>>>(S);
         }
-    } else runs_kernel<K, T, DIR, WT, WHOLE><<<(unsigned)blocks, threads, 0, stream>>>(S);
+    } else runs_kernel<O, DIR, WT, WHOLE><<<(unsigned)blocks, threads, 0, stream>>>(S);
 }
-
-template <Kind K, class T, int DIR> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
-    if (d.wt == 1) launch_runs<K, T, DIR, 1>(S, d, stream);
-    else if (d.wt == 4) launch_runs<K, T, DIR, 4>(S, d, stream);
-    else launch_runs<K, T, DIR, kMany<K, T>>(S, d, stream);
+template <class O, int DIR> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
+    if (d.wt == 1) launch_runs<O, DIR, 1>(S, d, stream);
+    else if (d.wt == 4) launch_runs<O, DIR, 4>(S, d, stream);
+    else launch_runs<O, DIR, kMany<O>>(S, d, stream);
 }
 
 bool dense(const View& v, int64_t channels) { return !v.p || (channels == 1 ? v.sb : v.sc) == 1; }
 
-template <Kind K, class T> int launch(Seq S, void* workspace, int64_t bytes, hipStream_t stream, const char* who) {
+template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const char* who) {
     // time is the fast index of everything there is (a view that is the same at all steps, say, is read by columns)
-    const int64_t st = S.x.p ? S.x.st : S.h.p ? S.h.st : S.gate_out.st;
+    const int64_t st = S.h.st;
     bool runs = S.channels == 1 && S.steps > 1 && (st == 1 || st == -1);
-    for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.gate_out}) runs = runs && (!v->p || v->st == st);
-    for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || !v->p || v->sb != 1);
+    for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.second}) runs = runs && (!v->p || v->st == st);
+    for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || v->sb != 1);
     const Deal d = runs ? deal_runs(S.steps, S.cols) : deal_columns(S.steps, S.cols);
     if (d.parts > 65535 || S.cols > ((int64_t)1 << 32)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
     S.part = d.part;
     S.pairs = workspace;
     if (runs) {
-        if (st == 1) launch_runs<K, T, 1>(S, d, stream);
-        else launch_runs<K, T, -1>(S, d, stream);
+        if (st == 1) launch_runs<O, 1>(S, d, stream);
+        else launch_runs<O, -1>(S, d, stream);
     } else {
-        // Two columns to a lane (wider rows, half the instructions) where there are enough for the GPU all the same.
-        const bool two = S.cols >= 65536 && S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) &&
-                         dense(S.gate, S.channels) && dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.gate_out, S.channels);
-        if (two) {
-            if (d.wt == 1) launch_columns<K, T, 2, 1>(S, d, stream);
-            else launch_columns<K, T, 2, 4>(S, Deal{4, S.steps, 1}, stream);
-        } else if (d.wt == 1) launch_columns<K, T, 1, 1>(S, d, stream);
-        else if (d.wt == 4) launch_columns<K, T, 1, 4>(S, d, stream);
-        else launch_columns<K, T, 1, kMany<K, T>>(S, d, stream);
+        if constexpr (O::K == ADVANTAGES) {
+            // Two columns to a lane (wider rows, half the instructions) where there are enough for the GPU all the same.
+            const bool two = S.cols >= 65536 && S.cols % 2 == 0 && dense(S.x, 1) && dense(S.before, 1) && dense(S.h, 1) && dense(S.second, 1);
+            if (two && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
+            if (two && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
+        }
+        if (d.wt == 1) launch_columns<O, 1, 1>(S, d, stream);
+        else if (d.wt == 4) launch_columns<O, 1, 4>(S, d, stream);
+        else launch_columns<O, 1, kMany<O>>(S, d, stream);
     }
+    return 0;
+}
+
+template <Kind K, class T> int run(const Seq& S, void* workspace, hipStream_t stream, const char* who) {
+    int rc;
+    if constexpr (K == ADVANTAGES) rc = launch<Op<K, T, false, true, true>>(S, workspace, stream, who);
+    else {
+        const bool resets = S.resets.p;
+        if (K == BACKWARD && S.second.p) {
+            if (resets) rc = launch<Op<K, T, true, true, K == BACKWARD>>(S, workspace, stream, who);
+            else rc = launch<Op<K, T, true, false, K == BACKWARD>>(S, workspace, stream, who);
+        } else if (S.gate.p) {
+            if (resets) rc = launch<Op<K, T, true, true, false>>(S, workspace, stream, who);
+            else rc = launch<Op<K, T, true, false, false>>(S, workspace, stream, who);
+        } else {
+            if (resets) rc = launch<Op<K, T, false, true, false>>(S, workspace, stream, who);
+            else rc = launch<Op<K, T, false, false, false>>(S, workspace, stream, who);
+        }
+    }
+    if (rc) return rc;
     LRN_LAUNCHED(who);
     return 0;
 }
 
-template <Kind K> int run(const Seq& S, int dtype, void* workspace, int64_t bytes, hipStream_t stream, const char* who) {
-    if (dtype == LRN_F32) return launch<K, float>(S, workspace, bytes, stream, who);
-    if (dtype == LRN_F64) return launch<K, double>(S, workspace, bytes, stream, who);
+template <Kind K> int run(const Seq& S, int dtype, void* workspace, hipStream_t stream, const char* who) {
+    if (dtype == LRN_F32) return run<K, float>(S, workspace, stream, who);
+    if (dtype == LRN_F64) return run<K, double>(S, workspace, stream, who);
     if constexpr (K != ADVANTAGES) {
-        if (dtype == LRN_BF16) return launch<K, bf16>(S, workspace, bytes, stream, who);
-        return launch<K, f16>(S, workspace, bytes, stream, who);
+        if (dtype == LRN_BF16) return run<K, bf16>(S, workspace, stream, who);
+        return run<K, f16>(S, workspace, stream, who);
     }
     return 0;
 }
@@ -744,7 +793,7 @@ int lrn_scan(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_vie
     S.x = ordered(x, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
     S.resets = ordered(resets, seq->steps, 1, rev); S.h = ordered(h_out, seq->steps, n, rev);
     S.gate_const = gate_const; S.initial = initial; S.final = final_out;
-    return run<SCAN>(S, seq->dtype, workspace, workspace_bytes, (hipStream_t)hip_stream, "lrn_scan");
+    return run<SCAN>(S, seq->dtype, workspace, (hipStream_t)hip_stream, "lrn_scan");
 }
 
 int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const,
@@ -753,7 +802,9 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
                       void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
     if (int rc = checked(seq, "lrn_scan_backward")) return rc;
     if (seq->batch * seq->channels == 0) return 0;
-    if (grad_gate_out && grad_gate_out->data && seq->steps && (!h || !h->data)) return fail(-1, "lrn_scan_backward: null h");
+    if (seq->steps && (!g_h || !g_h->data || !grad_x_out || !grad_x_out->data)) return fail(-1, "lrn_scan_backward: null g_h or grad_x");
+    const bool want_gate = seq->steps && grad_gate_out && grad_gate_out->data;
+    if (want_gate && (!h || !h->data || !gate || !gate->data)) return fail(-1, "lrn_scan_backward: null h or gate");
     if (int rc = check_views("lrn_scan_backward", {gate, resets, h, g_h, grad_x_out, grad_gate_out})) return rc;
     if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_scan_backward")) return rc;
     LRN_ON_DEVICE(device);
@@ -762,10 +813,10 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
     Seq S{};
     S.steps = seq->steps; S.cols = seq->batch * seq->channels; S.channels = seq->channels;
     S.x = ordered(g_h, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
-    S.resets = ordered(resets, seq->steps, 1, rev); S.before = ordered(h, seq->steps, n, rev);
-    S.h = ordered(grad_x_out, seq->steps, n, rev); S.gate_out = ordered(grad_gate_out, seq->steps, n, rev);
+    S.resets = ordered(resets, seq->steps, 1, rev); S.before = ordered(want_gate ? h : nullptr, seq->steps, n, rev);
+    S.h = ordered(grad_x_out, seq->steps, n, rev); S.second = ordered(want_gate ? grad_gate_out : nullptr, seq->steps, n, rev);
     S.gate_const = gate_const; S.initial = g_final; S.edge = initial; S.final = grad_initial_out;
-    return run<BACKWARD>(S, seq->dtype, workspace, workspace_bytes, (hipStream_t)hip_stream, "lrn_scan_backward");
+    return run<BACKWARD>(S, seq->dtype, workspace, (hipStream_t)hip_stream, "lrn_scan_backward");
 }
 
 int64_t lrn_advantages_workspace(const lrn_seq* seq) { return workspace_of(seq); }
@@ -787,9 +838,9 @@ int lrn_advantages(int32_t device, void* hip_stream, const lrn_seq* seq, const l
     S.steps = seq->steps; S.cols = seq->batch; S.channels = 1;
     S.x = ordered(rewards, seq->steps, bytes_of(seq->dtype), true); S.before = ordered(values, seq->steps, 4, true);
     S.resets = ordered(ends, seq->steps, 1, true);
-    S.h = ordered(advantage_out, seq->steps, 4, true); S.gate_out = ordered(target_out, seq->steps, 4, true);
+    S.h = ordered(advantage_out, seq->steps, 4, true); S.second = ordered(target_out, seq->steps, 4, true);
     S.gate_const = gamma * lam; S.scale = gamma; S.edge = last_values;
-    return run<ADVANTAGES>(S, seq->dtype, workspace, workspace_bytes, (hipStream_t)hip_stream, "lrn_advantages");
+    return run<ADVANTAGES>(S, seq->dtype, workspace, (hipStream_t)hip_stream, "lrn_advantages");
 }
 
 }  // extern "C"

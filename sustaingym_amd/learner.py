@@ -359,7 +359,9 @@ class _GatedScan(torch.autograd.Function):
             return (None,) * 7
         lib = _lib.load()
         g_final = None if g_final is None else g_final.contiguous()
-        gx = _laid_out(shape, stride, dtype, device) if want_x else None
+        if g_h is None:                                              # only the last state was used
+            g_h = torch.zeros((), dtype=dtype, device=device).expand(shape)
+        gx = _laid_out(shape, stride, dtype, device)
         gg = _laid_out(shape, stride, dtype, device) if want_gate else None
         gi = torch.empty(initial.shape, dtype=initial.dtype, device=device) if want_initial else None
         seq = _sequence(shape, dim, reverse, dtype)
@@ -370,7 +372,7 @@ class _GatedScan(torch.autograd.Function):
                                      _ref(_view(resets, dim)), _ptr(initial), _ref(_view(h, dim)), _ref(_view(g_h, dim)),
                                      _ptr(g_final), _ref(_view(gx, dim)), _ref(_view(gg, dim)), _ptr(gi), _ptr(ws), nbytes),
                'gated_scan backward')
-        return gx, gg, gi, None, None, None, None
+        return gx if want_x else None, gg, gi, None, None, None, None
 
 
 def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool = False):

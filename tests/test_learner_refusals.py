@@ -133,7 +133,12 @@ def test_the_c_abi_refuses():
         assert lib.lrn_scan_backward(0, None, seq(**kw), None, 0.5, None, None, None, v, None, v, None, None, None, 0) == -1
     assert lib.lrn_scan(0, None, seq(), None, None, 0.5, None, None, v, None, None, 0) == -1
     assert lib.lrn_scan(0, None, seq(), v, None, 0.5, None, None, None, None, None, 0) == -1
-    assert lib.lrn_scan_backward(0, None, seq(), v, 0.0, None, None, None, v, None, v, v, None, None, 0) == -1 and 'null h' in text()
+    assert lib.lrn_scan_backward(0, None, seq(), v, 0.0, None, None, None, v, None, v, v, None, None, 0) == -1 and 'null h or gate' in text()
+    assert lib.lrn_scan_backward(0, None, seq(), None, 0.5, None, None, v, v, None, v, v, None, None, 0) == -1 and 'null h or gate' in text()
+    assert lib.lrn_scan_backward(0, None, seq(), v, 0.0, None, None, None, None, one, v, None, None, None, 0) == -1 and 'null g_h' in text()
+    assert lib.lrn_scan_backward(0, None, seq(), v, 0.0, None, None, None, v, None, None, None, None, None, 0) == -1 and 'grad_x' in text()
+    back = C.byref(_lib.LearnerView(64, 6, -3, 1))
+    assert lib.lrn_scan(0, None, seq(), back, None, 0.5, None, None, v, None, None, 0) == -1 and 'negative' in text()
     long = seq(steps=10 ** 6, batch=1, channels=1)
     need = lib.lrn_scan_workspace(long)
     if need:
