@@ -682,7 +682,7 @@ template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hip
             columns_kernel<O, V, WT, PAIRS><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
             columns_kernel<O, V, WT, APPLY><<<dim3((unsigned)tiles, (unsigned)d.parts), threads, 0, stream>>>(S);
         }
-    } else columns_kernel<O, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
+    } else if constexpr (V == 1 || WT != kMany<O>) columns_kernel<O, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
 }
 template <class O, int DIR, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
     const int64_t blocks = WT == 1 ? cdiv(S.cols, 4) : S.cols;
@@ -716,11 +716,16 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
         if (st == 1) launch_runs<O, 1>(S, d, stream);
         else launch_runs<O, -1>(S, d, stream);
     } else {
+        // Two columns to a lane, wider rows and half the instructions: in sequences in parts where it takes fewer tiles (131 073
+        // steps of 72 float32: 45 us instead of 55; float64 gains nothing), and for advantages of many sequences, whose 21 bytes
+        // a step keep the memory busy with half the wavefronts (but not in parts: 2048 x 2000 float64 41 us instead of 31).
+        const bool even = S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) && dense(S.gate, S.channels) &&
+                          dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels);
         if constexpr (O::K == ADVANTAGES) {
-            // Two columns to a lane (wider rows, half the instructions) where there are enough for the GPU all the same.
-            const bool two = S.cols >= 65536 && S.cols % 2 == 0 && dense(S.x, 1) && dense(S.before, 1) && dense(S.h, 1) && dense(S.second, 1);
-            if (two && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
-            if (two && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
+            if (even && S.cols >= 65536 && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
+            if (even && S.cols >= 65536 && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
+        } else if constexpr (sizeof(typename O::T) <= 4) {
+            if (even && d.parts > 1 && S.cols > 64) return launch_columns<O, 2, kMany<O>>(S, d, stream), 0;
         }
         if (d.wt == 1) launch_columns<O, 1, 1>(S, d, stream);
         else if (d.wt == 4) launch_columns<O, 1, 4>(S, d, stream);
