@@ -8,6 +8,8 @@ Public surface (mirrors ``sustaingym.envs.evcharging``):
     DeviceGMMTraceGenerator, RealTraceBank                              (episode generators)
     StepEngine                                                          (C-ABI handle)
     BatteryDispatchVectorEnv                                            (config 4, synthetic: battery.py)
+    learner                                                             (choose_levels, level_logprobs, gated_scan, advantages)
+    rollouts                                                            (PolicyRollout, run_policy, collect, score)
 
 The HIP library is loaded lazily (``sustaingym_amd._lib.load``); importing the package does not
 need a GPU, constructing an environment does.

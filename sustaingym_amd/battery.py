@@ -133,14 +133,17 @@ class BatteryDispatchVectorEnv:
         self._owned_traj[view.data_ptr()] = store            # (keeps the allocation alive as long as the environment)
         return view, torch.zeros((steps, self.N), dtype=torch.float64, device=obs.device)
 
-    def rollout(self, bids_ring, steps: int, trajectory: bool = False, out=None):
+    def rollout(self, bids_ring, steps: int, trajectory: bool = False, out=None, gamma: float | None = None):
         """``steps`` steps in ONE launch (``bat_rollout``): step i uses ``bids_ring[i % R]`` (CUDA float32 ``[R, N, 2k]``).
         Returns ``(obs, reward, terminated)`` of the last step (the persistent buffers of ``step``) and, with
         ``trajectory=True``, also ``(obs_traj [steps, N, 4k+6] float32, reward_traj [steps, N] float64)`` — every step's
-        observation and reward, what a learner's rollout buffer holds (pass ``out=(obs_traj, reward_traj)`` to reuse buffers)."""
+        observation and reward, what a learner's rollout buffer holds (pass ``out=(obs_traj, reward_traj)`` to reuse buffers).
+        ``gamma`` (with ``trajectory=True``) adds a third tensor to the trajectory: the discounted rewards from each step on,
+        ``[steps, N]`` float64 (``learner.gated_scan``; steps behind an episode's end have reward 0)."""
         import torch
         assert self.output == 'torch' and bids_ring.is_cuda and bids_ring.dtype == torch.float32 and bids_ring.is_contiguous()
         assert bids_ring.dim() == 3 and tuple(bids_ring.shape[1:]) == (self.N, 2 * self.k)
+        assert gamma is None or trajectory, 'gamma= needs trajectory=True'
         obs, rew, term = self._device_buffers()
         traj = None
         pitch = self.F
@@ -162,6 +165,9 @@ class BatteryDispatchVectorEnv:
                                                  C.c_void_p(obs.data_ptr()), C.c_void_p(rew.data_ptr()), C.c_void_p(term.data_ptr()),
                                                  C.c_void_p(traj[0].data_ptr()) if traj else None, pitch,
                                                  C.c_void_p(traj[1].data_ptr()) if traj else None), 'bat_rollout')
+        if gamma is not None:
+            from .learner import gated_scan
+            traj = (*traj, gated_scan(traj[1], gamma, reverse=True)[0])
         return (obs, rew, term) + ((traj,) if traj else ())
 
     def make_stepper(self):

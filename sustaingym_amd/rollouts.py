@@ -13,10 +13,15 @@ MPC / OfflineOptimal (baselines.py:54-223) are cvxpy programs that merely call `
 out of scope.  Policies that need Python (a trained network, a user's controller) go
 through :func:`run_policy`, which drives any environment of this package — ``EVChargingEnv``, a wrapped
 one, the multi-agent one — through its own ``reset`` / ``step``.
+
+A network that lives on the GPU plays the whole batch: :func:`collect` steps an ``EVChargingVectorEnv(output='torch',
+discrete_bins=K)`` on the levels that it chooses (:func:`learner.choose_levels`) and returns the trajectory with advantages
+(:func:`learner.advantages`); :func:`score` asks a policy again about the levels that were played, with gradients
+(:func:`learner.level_logprobs`).
 """
 from __future__ import annotations
 
-from typing import Iterable, Sequence
+from typing import Any, Iterable, NamedTuple, Sequence
 
 import numpy as np
 
@@ -152,3 +157,73 @@ def run_policy(env, policy, seeds: Iterable[int] | int) -> dict[str, list]:
         out['max_profit'].append(info.get('max_profit'))
         out['reward_breakdown'].append(info.get('reward_breakdown'))
     return out
+
+
+class Trajectory(NamedTuple):
+    """``T`` steps of ``N`` environments with ``n`` stations (device tensors; ``obs``: a dict of ``[T, N, ...]``)."""
+    obs: dict
+    levels: Any          # int64 [T, N, n], what was played
+    logprobs: Any        # float32 [T, N, n], under the policy that played
+    entropy: Any         # float32 [T, N, n]
+    mask: Any            # bool [T, N, n, 1 or K] or None: what the policy allowed
+    rewards: Any         # float64 [T, N]
+    values: Any          # float32 [T, N], the policy's estimates
+    ends: Any            # bool [T, N]: the episode ended with this step
+    last_values: Any     # float32 [N]: of the observation behind the last step
+    advantages: Any      # float32 [T, N]
+    targets: Any         # float32 [T, N]: advantages + values
+
+
+def _ask(policy, obs):
+    answer = policy(obs)
+    return answer if len(answer) == 3 else (*answer, None)
+
+
+def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float = 0.95, greedy: bool = False, generator=None):
+    """``steps`` steps of a batch under a policy on the GPU; returns ``(Trajectory, obs)``, the observation to go on from.
+
+    venv: ``EVChargingVectorEnv(..., output='torch', discrete_bins=K)``; episodes begin anew by themselves.
+    policy: ``policy(obs) -> (logits [N, n, K], values [N])`` or ``(logits, values, mask)``; mask: bool, broadcastable to the
+        logits, True = allowed (a station that it leaves nothing gets level 0).
+    obs: the observation to begin with; None resets the environments.
+    greedy: the most probable level instead of a sampled one (``generator``: the torch generator of the samples).
+
+    Nothing is synchronised: the steps are enqueued on the current stream, and no gradient is recorded."""
+    import torch
+    from . import learner
+    if getattr(venv, 'output', None) != 'torch' or not venv.discrete_bins > 0:
+        raise ValueError("collect needs an EVChargingVectorEnv with output='torch' and discrete_bins > 0")
+    if steps < 1:
+        raise ValueError(f'steps: at least 1, got {steps}')
+    rows: dict[str, list] = {key: [] for key in ('levels', 'logprobs', 'entropy', 'mask', 'rewards', 'values', 'ends')}
+    seen: list[dict] = []
+    with torch.no_grad():
+        if obs is None:
+            obs, _ = venv.reset()
+        for _ in range(steps):
+            seen.append({key: val.clone() for key, val in obs.items()})      # (the environments overwrite theirs)
+            logits, values, mask = _ask(policy, seen[-1])
+            noise = None if greedy else torch.empty(logits.shape, dtype=torch.float32, device=logits.device).exponential_(
+                generator=generator).clamp_(min=1e-30).log_().neg_()         # Gumbel
+            choice = learner.choose_levels(logits, noise, mask)
+            obs, rewards, ends, _, _ = venv.step(choice.levels)
+            for key, val in (*zip(('levels', 'logprobs', 'entropy'), choice), ('values', values.float()), ('rewards', rewards.clone()),
+                             ('ends', ends.clone())):
+                rows[key].append(val)
+            if mask is not None:
+                rows['mask'].append(mask.expand((*logits.shape[:-1], mask.shape[-1])).clone())
+        last_values = _ask(policy, obs)[1].float()
+        out = {key: torch.stack(val) if val else None for key, val in rows.items()}
+        adv = learner.advantages(out['rewards'], out['values'], out['ends'], last_values, gamma, lam)
+        return Trajectory(obs={key: torch.stack([o[key] for o in seen]) for key in seen[0]}, last_values=last_values,
+                          advantages=adv.advantages, targets=adv.targets, **out), {key: val.clone() for key, val in obs.items()}
+
+
+def score(trajectory: Trajectory, policy, top: int = 0):
+    """The levels of a trajectory under ``policy`` as it is now: ``(learner.LevelScores, values [T, N])`` with gradients to its
+    parameters.  The policy is asked once, about ``T * N`` observations; what was allowed is what the trajectory says."""
+    from . import learner
+    T, N = trajectory.rewards.shape
+    logits, values, _ = _ask(policy, {key: val.flatten(0, 1) for key, val in trajectory.obs.items()})
+    logits = logits.unflatten(0, (T, N))
+    return learner.level_logprobs(logits, trajectory.levels, trajectory.mask, top), values.unflatten(0, (T, N))
