@@ -4,8 +4,8 @@
  *
  * Every call is asynchronous on `hip_stream` (a stream of `device`), allocates nothing, keeps nothing between
  * calls and may be captured into a graph.  Workspaces are the caller's, at least as large as the *_workspace
- * call for the same arguments says (0 = none, the pointer may be NULL); a workspace is used by one call at a
- * time.  Returns 0, or a negative code with a text in lrn_last_error() (thread-local): -1 argument,
+ * call for the same arguments says (0 = none, the pointer may be NULL), aligned to 16 bytes; a workspace is used by one call
+ * at a time.  Returns 0, or a negative code with a text in lrn_last_error() (thread-local): -1 argument,
  * -2 no device, -4 HIP error.
  *
  * ROWS.  `rows = outer * inner` rows of `levels` logits; row (o, i) starts at o * stride_outer + i * stride_inner
@@ -77,7 +77,9 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
  * lrn_scan:  h_t = a_t h_{t-1} + x_t,  t = 0 .. steps-1  (reverse: from the last step to the first; "before" and "last"
  * below are meant in that order).  a_t = gate_t (the type of x, or gate_const where gate is NULL), and exactly 0 where
  * resets (bytes, (time, batch) strides, NULL = none) says that the sequence starts anew: nothing of what came before
- * enters, not even a NaN (nor does it where the gate itself is exactly 0).  initial [batch][channels] contiguous (NULL = 0) is the state before the first step; final
+ * enters, not even a NaN (nor does it where the gate itself is exactly 0; in float32
+ * states a product with a factor of 0 is 0).  Meant for |gate| <= 1: the products of larger gates over a run of steps must stay
+ * in range.  initial [batch][channels] contiguous (NULL = 0) is the state before the first step; final
  * (NULL = not wanted) receives the last one.  initial / final are float32, float64 for LRN_F64; the state is carried in
  * those types whatever the type of x and h.  h may not overlap an input.
  */

@@ -17,6 +17,9 @@ char* error_text() {
 
 namespace {
 
+// Workgroups are numbered over two dimensions of the grid: one holds fewer than 2^32 lanes.
+__device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 struct Rows {
     const void* logits;
     const uint8_t* mask;
@@ -265,9 +268,9 @@ __device__ __forceinline__ Sums group_sums(const float (&z)[E], float (&e)[E]) {
 template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) {
     const int g = threadIdx.x % G;
-    const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t r = block_number() * (256 / G) + threadIdx.x / G;
     __shared__ StageOf<T, G, E> S;
-    stage<T, G, E>(R, (int64_t)blockIdx.x * (256 / G), S);
+    stage<T, G, E>(R, block_number() * (256 / G), S);
     if (r >= R.rows) return;                    // whole groups: no lane of a group leaves alone
     int64_t off, moff, noff;
     offsets(R, r, off, moff, &O, &noff);
@@ -375,9 +378,9 @@ template <int N> struct Network {
 template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_score_kernel(Rows R, ScoreOut O) {
     const int g = threadIdx.x % G;
-    const int64_t r = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+    const int64_t r = block_number() * (256 / G) + threadIdx.x / G;
     __shared__ StageOf<T, G, E> S;
-    stage<T, G, E>(R, (int64_t)blockIdx.x * (256 / G), S);
+    stage<T, G, E>(R, block_number() * (256 / G), S);
     if (r >= R.rows) return;
     int64_t off, moff;
     offsets(R, r, off, moff);
@@ -425,7 +428,7 @@ template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T* grad) {
     __shared__ __attribute__((aligned(16))) T out[256 * E];
     const int row = threadIdx.x / G, g = threadIdx.x % G, K = R.levels;
-    const int64_t r0 = (int64_t)blockIdx.x * (256 / G), r = r0 + row;
+    const int64_t r0 = block_number() * (256 / G), r = r0 + row;
     __shared__ StageOf<T, G, E> S;
     stage<T, G, E>(R, r0, S);
     if (r < R.rows) {
@@ -652,8 +655,9 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
     __shared__ float list_v[3 * LRN_MAX_TOP];
     __shared__ int list_j[3 * LRN_MAX_TOP];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = cut.parts > 1 ? (int64_t)blockIdx.x / cut.parts : blockIdx.x;
-    const int p = cut.parts > 1 ? (int)(blockIdx.x - r * cut.parts) : 0;
+    const int64_t number = block_number(), r = cut.parts > 1 ? number / cut.parts : number;
+    const int p = (int)(number - r * cut.parts);
+    if (r >= R.rows) return;
     const int begin = p * cut.length, end = min(begin + cut.length, R.levels);
     int64_t o, i;
     split(R, r, o, i);
@@ -712,15 +716,16 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
         if constexpr (CHOOSE) put_choice<T>(R, C, r, a, b, lane);
         else put_score<T>(R, O, r, given, a, list, lane);
     } else {
-        if (lane == 0) cut.part[blockIdx.x] = Part{a.m, a.s, a.t, b.v, b.j};
-        if (lane < top) { cut.top_v[(int64_t)blockIdx.x * top + lane] = list.v; cut.top_j[(int64_t)blockIdx.x * top + lane] = list.j; }
+        if (lane == 0) cut.part[number] = Part{a.m, a.s, a.t, b.v, b.j};
+        if (lane < top) { cut.top_v[number * top + lane] = list.v; cut.top_j[number * top + lane] = list.j; }
     }
 }
 
 template <class T, bool CHOOSE>
 __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut O, Cut cut) {
     const int lane = threadIdx.x;
-    const int64_t r = blockIdx.x;
+    const int64_t r = block_number();
+    if (r >= R.rows) return;
     Given given{};
     if (!CHOOSE && lane == 0) given = given_level<T>(R, O, r);
     Part mine{kNegInf, 0.0f, 0.0f, kNegInf, 0x7fffffff};
@@ -764,8 +769,9 @@ constexpr int kBackPieces = 4;       // pieces a lane
 template <class T>
 __global__ __launch_bounds__(256) void wide_backward_kernel(Rows R, BackIn I, T* grad, int parts) {
     constexpr int N = Piece<T>::N;
-    const int64_t r = blockIdx.x / (unsigned)parts;
-    const int begin = (int)(blockIdx.x - r * parts) * (256 * N * kBackPieces), end = min(begin + 256 * N * kBackPieces, R.levels);
+    const int64_t number = block_number(), r = number / parts;
+    if (r >= R.rows) return;
+    const int begin = (int)(number - r * parts) * (256 * N * kBackPieces), end = min(begin + 256 * N * kBackPieces, R.levels);
     int64_t o, i;
     split(R, r, o, i);
     const T* src = (const T*)R.logits + o * R.so + i * R.si;
@@ -849,10 +855,10 @@ int checked(const lrn_rows* in, Rows* out) {
 }
 
 int64_t size_of(int dtype) { return dtype == LRN_F32 ? 4 : 2; }
-int tiles(const Rows& R, unsigned* grid) {
-    const int64_t n = cdiv(R.rows, group_rows(R.levels));
-    if (n > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
-    *grid = (unsigned)n;
+int grid_of(int64_t blocks, dim3* grid) {
+    if (blocks >= (int64_t)1 << 36) return fail(-1, "rows: too many for one call");
+    const int64_t x = std::min<int64_t>(blocks, 1 << 20);
+    *grid = dim3((unsigned)x, (unsigned)cdiv(blocks, x));
     return 0;
 }
 
@@ -863,10 +869,12 @@ int check_workspace(int64_t need, const void* workspace, int64_t bytes, const ch
 
 template <class T, bool CHOOSE> int launch_wide(const Rows& R, const ChooseOut& C, const ScoreOut& O, int top, void* workspace, hipStream_t stream, const char* who) {
     const Cut cut = cut_of(R, top, workspace);
-    if (R.rows * cut.parts > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
-    if (R.mask) wide_kernel<T, CHOOSE, true><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
-    else wide_kernel<T, CHOOSE, false><<<(unsigned)(R.rows * cut.parts), 256, 0, stream>>>(R, C, O, cut);
-    if (cut.parts > 1) join_kernel<T, CHOOSE><<<(unsigned)R.rows, 64, 0, stream>>>(R, C, O, cut);
+    dim3 grid, rows;
+    if (int rc = grid_of(R.rows * cut.parts, &grid)) return rc;
+    if (int rc = grid_of(R.rows, &rows)) return rc;
+    if (R.mask) wide_kernel<T, CHOOSE, true><<<grid, 256, 0, stream>>>(R, C, O, cut);
+    else wide_kernel<T, CHOOSE, false><<<grid, 256, 0, stream>>>(R, C, O, cut);
+    if (cut.parts > 1) join_kernel<T, CHOOSE><<<rows, 64, 0, stream>>>(R, C, O, cut);
     LRN_LAUNCHED(who);
     return 0;
 }
@@ -904,8 +912,8 @@ int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const flo
     const ChooseOut O{noise, noise_outer, noise_inner, extent(*rows, noise_outer, noise_inner, R.levels),
                       !noise || dense(*rows, noise_outer, noise_inner), level_out, logprob_out, entropy_out};
     if (R.levels <= kGroupLevels) {
-        unsigned grid;
-        if (int rc = tiles(R, &grid)) return rc;
+        dim3 grid;
+        if (int rc = grid_of(cdiv(R.rows, group_rows(R.levels)), &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
         BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_choose_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, O))));
         LRN_LAUNCHED("lrn_choose");
@@ -931,8 +939,8 @@ int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int6
     LRN_ON_DEVICE(device);
     const ScoreOut O{level, logprob_out, entropy_out, stat_out, top, top_logprob_out, top_level_out};
     if (R.levels <= kGroupLevels) {
-        unsigned grid;
-        if (int rc = tiles(R, &grid)) return rc;
+        dim3 grid;
+        if (int rc = grid_of(cdiv(R.rows, group_rows(R.levels)), &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
         BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_score_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, O))));
         LRN_LAUNCHED("lrn_score");
@@ -955,16 +963,17 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
     LRN_ON_DEVICE(device);
     const BackIn I{level, stat, entropy, g_logprob, g_entropy, g_logprob_stride, g_entropy_stride};
     if (again) {
-        unsigned grid;
-        if (int rc = tiles(R, &grid)) return rc;
+        dim3 grid;
+        if (int rc = grid_of(cdiv(R.rows, group_rows(R.levels)), &grid)) return rc;
         hipStream_t stream = (hipStream_t)hip_stream;
         BY_TYPE(rows->dtype, BY_LEVELS(R.levels, (group_backward_kernel<T, G, E><<<grid, 256, 0, stream>>>(R, I, (T*)grad_out))));
         LRN_LAUNCHED("lrn_score_backward");
         return 0;
     }
     const int64_t parts = cdiv(R.levels, 256 * kBackPieces * 16 / size_of(rows->dtype));
-    if (R.rows * parts > 0x7fffffff) return fail(-1, "rows: %lld are too many for one call", (long long)R.rows);
-    BY_TYPE(rows->dtype, (wide_backward_kernel<T><<<(unsigned)(R.rows * parts), 256, 0, (hipStream_t)hip_stream>>>(R, I, (T*)grad_out, (int)parts)));
+    dim3 grid;
+    if (int rc = grid_of(R.rows * parts, &grid)) return rc;
+    BY_TYPE(rows->dtype, (wide_backward_kernel<T><<<grid, 256, 0, (hipStream_t)hip_stream>>>(R, I, (T*)grad_out, (int)parts)));
     LRN_LAUNCHED("lrn_score_backward");
     return 0;
 }

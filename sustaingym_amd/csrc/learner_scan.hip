@@ -709,7 +709,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
     for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.second}) runs = runs && (!v->p || v->st == st);
     for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || v->sb != 1);
     const Deal d = runs ? deal_runs(S.steps, S.cols) : deal_columns(S.steps, S.cols);
-    if (d.parts > 65535 || S.cols > ((int64_t)1 << 32)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
+    if (d.parts > 65535 || S.cols > ((int64_t)1 << 31)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
     S.part = d.part;
     S.pairs = workspace;
     if (runs) {

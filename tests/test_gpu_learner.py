@@ -244,7 +244,7 @@ def test_row_gradient_against_differences(K):
 
 SCANS = [((1, 1, 1), 0), ((1, 256, 512), 0), ((2, 3, 5), 0), ((5, 1, 64), 0), ((7, 2, 65), 1), ((288, 4, 3), 0), ((3, 289, 33), 1), ((2, 128, 128), 1),
          ((129, 2, 72), 0), ((1, 1000, 72), 1), ((2, 511, 4), 1), ((17, 200), 0), ((200, 17), 1), ((3, 1025), 1), ((1, 4099), 1), ((4099,), 0),
-         ((31,), 0), ((64, 64), 1), ((1, 3000, 8), 1), ((1, 9000, 1), 1), ((4000, 1, 2), 0), ((20, 33, 1), 0)]
+         ((31,), 0), ((64, 64), 1), ((1, 3000, 8), 1), ((1, 9000, 1), 1), ((4000, 1, 2), 0), ((20, 33, 1), 0), ((40, 70, 1000), 0), ((9, 65540), 0), ((600, 3, 34), 0)]
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16', 'f64'])
@@ -413,7 +413,7 @@ def test_scan_of_any_stride():
     near(learner.gated_scan(one, 0.5)[0], *ref.scan(host(one.contiguous()), 0.5, None, None, 0, False)['h'], 'expanded')
 
 
-@pytest.mark.parametrize('T,N', [(1, 1), (288, 1), (5, 64), (100, 1000), (288, 4096), (1, 70000), (2049, 3), (20000, 2)])
+@pytest.mark.parametrize('T,N', [(1, 1), (288, 1), (5, 64), (100, 1000), (288, 4096), (1, 70000), (2049, 3), (20000, 2), (40, 66000), (20, 65537)])
 def test_advantages_against_float64(T, N):
     from sustaingym_amd import learner
     g = gen(T + N)
@@ -568,3 +568,114 @@ def test_on_another_stream():
     torch.cuda.current_stream().wait_stream(side)
     for one in got:
         assert all(torch.equal(a, b) for a, b in zip(one, want))
+
+
+def test_offsets_beyond_32_bits():
+    """Rows, sequences and steps that lie more than 2^32 bytes (and elements) apart."""
+    from sustaingym_amd import learner
+    g = gen(31)
+    far = 2 ** 32 + 8
+    big = torch.empty(far + 4096 * 8, dtype=torch.float16, device='cuda')          # 8.6 GB, written only where it is read
+    for K in (5, 40, 700, 3001):
+        rows = big.as_strided((2, K), (far, 1))
+        rows.copy_(torch.randn((2, K), generator=g, device='cuda'))
+        mask = torch.rand((2, K), generator=g, device='cuda') < 0.9
+        levels = mask.int().argmax(-1)
+        r = ref.Rows(host(rows.contiguous()), host(mask))
+        leaf = rows.detach().requires_grad_(True)
+        s = learner.level_logprobs(leaf, levels, mask, 1)
+        near(s.logprobs, *r.of_levels(host(levels)), K)
+        assert torch.equal(host(s.top_levels), ref.top_levels(r, 1)[0])
+        up = torch.ones(2, device='cuda')
+        near(torch.autograd.grad(s.logprobs, leaf, up)[0], *r.gradient(host(levels), host(up), torch.zeros(2), torch.float16), K)
+        want, _ = ref.choose(host(rows.contiguous()), None, host(mask))
+        assert torch.equal(host(learner.choose_levels(rows, None, mask).levels), want)
+    for shape, strides, dim in (((2, 30, 70), (far, 70, 1), 1), ((2, 600, 34), (far, 34, 1), 1), ((2, 30, 70), (far, 70, 1), 0), ((2, 3000), (far, 1), 1),
+                                ((2, 90), (far, 1), 0), ((3, 20, 8), (far // 2, 8, 1), 1)):
+        x = big.as_strided(shape, strides)
+        x.copy_(torch.randn(shape, generator=g, device='cuda'))
+        gate = torch.rand(shape, generator=g, device='cuda').half()
+        up = torch.randn(shape, generator=g, device='cuda').half()
+        leaves = x.detach().requires_grad_(True), gate.requires_grad_(True)
+        want = ref.scan(host(x.contiguous()), host(gate), None, None, dim, False, host(up))
+        h, final = learner.gated_scan(*leaves, dim=dim)
+        near(h, *want['h'], (shape, dim))
+        near(final, *want['final'], (shape, dim))
+        # and as the gradient that comes in
+        far_up = big.as_strided(shape, strides)
+        kept = x.detach().clone()
+        h2, _ = learner.gated_scan(kept.requires_grad_(True), gate, dim=dim)
+        far_up.copy_(up)
+        gx, gg = torch.autograd.grad(h2, (kept, gate), far_up)
+        near(gx, *want['grad_x'], (shape, dim))
+        near(gg, *want['grad_gate'], (shape, dim))
+    del big
+
+
+def test_one_dimension_and_no_second_derivative():
+    from sustaingym_amd import learner
+    z = torch.randn(7, device='cuda', requires_grad=True)
+    c = learner.choose_levels(z)
+    assert c.levels.shape == () and int(c.levels) == int(z.argmax())
+    s = learner.level_logprobs(z, c.levels, top=7)
+    assert s.top_levels.shape == (7,) and host(s.top_levels).tolist() == host(z).argsort(descending=True).tolist()
+    r = ref.Rows(host(z))
+    grad, = torch.autograd.grad(s.logprobs, z, create_graph=True)
+    near(grad, *r.gradient(host(c.levels), torch.ones(()), torch.zeros(()), torch.float32), 'one row')
+    with pytest.raises(RuntimeError):
+        grad.sum().backward()
+    x = torch.randn((20, 3), device='cuda', requires_grad=True)
+    gx, = torch.autograd.grad(learner.gated_scan(x, 0.5)[0].sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+def test_gradients_through_saved_tensor_hooks_and_twice():
+    """What backward reads is what was saved (here: moved and brought back), and a kept graph gives the same again."""
+    from sustaingym_amd import learner
+    g = gen(33)
+    for K in (5, 2000):
+        z = torch.randn((6, K), generator=g, device='cuda', requires_grad=True)
+        levels = torch.randint(0, K, (6,), generator=g, device='cuda')
+        x = torch.randn((50, 3), generator=g, device='cuda', requires_grad=True)
+        gate = torch.rand((50, 3), generator=g, device='cuda', requires_grad=True)
+
+        def work():
+            s = learner.level_logprobs(z * 2.0, levels)
+            return s.logprobs.sum() + s.entropy.sum() + learner.gated_scan(x * 1.0, gate * 0.5)[0].sum()
+        want = torch.autograd.grad(work(), (z, x, gate))
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.clone()):
+            loss = work()
+        trash = [torch.full((6, K), 7.0, device='cuda') for _ in range(4)]
+        first = torch.autograd.grad(loss, (z, x, gate), retain_graph=True)
+        again = torch.autograd.grad(loss, (z, x, gate))
+        del trash
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, first, again))
+
+
+def test_calls_from_two_threads_on_two_streams():
+    import threading
+    from sustaingym_amd import learner
+    g = gen(35)
+    z = torch.randn((3, 90000), generator=g, device='cuda')
+    x = torch.randn((1, 20000, 6), generator=g, device='cuda')
+    levels = torch.randint(0, 90000, (3,), generator=g, device='cuda')
+    want = (*learner.level_logprobs(z, levels, None, 5), *learner.gated_scan(x, 0.9, dim=1))
+    torch.cuda.synchronize()
+    got, wrong = {}, []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[k] = [(*learner.level_logprobs(z, levels, None, 5), *learner.gated_scan(x, 0.9, dim=1)) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+            try:
+                learner.gated_scan(x, 0.9, dim=2)
+            except ValueError:
+                wrong.append(k)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(wrong) == [0, 1]
+    assert all(torch.equal(a, b) for k in got for one in got[k] for a, b in zip(one, want))
