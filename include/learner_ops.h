@@ -32,6 +32,7 @@ extern "C" {
 #define LRN_F64  3                 /* lrn_scan only */
 
 #define LRN_MAX_TOP 64             /* alternatives per row */
+#define LRN_SHORT_ROW 1024         /* rows of up to so many levels need no workspace, and lrn_score_backward no statistics */
 
 const char* lrn_last_error(void);
 
@@ -61,9 +62,8 @@ int64_t lrn_score_workspace(const lrn_rows* rows, int32_t top);
 int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int64_t* level, float* logprob_out,
               float* entropy_out, float* stat_out, int32_t top, float* top_logprob_out, int64_t* top_level_out,
               void* workspace, int64_t workspace_bytes);
-/* 1 if lrn_score_backward reads stat and entropy for these rows, 0 if it computes them again (both may then be NULL). */
-int lrn_score_backward_needs_stat(const lrn_rows* rows);
-/* grad_out (the logits' type, contiguous [rows][levels]):
+/* stat and entropy are lrn_score's for the same rows; not read (NULL) where levels <= LRN_SHORT_ROW, whose sums are computed again.
+ * grad_out (the logits' type, contiguous [rows][levels]):
  *   g_logprob (1[j = level] - p_j) - g_entropy p_j (log p_j + entropy)
  * g_logprob / g_entropy: float32 [rows] with a stride of 1 or 0 elements (NULL = zero). */
 int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, const int64_t* level, const float* stat,

@@ -148,7 +148,7 @@ class LearnerView(C.Structure):
     _fields_ = [('data', C.c_void_p), ('st', C.c_int64), ('sb', C.c_int64), ('sc', C.c_int64)]
 
 
-LEARNER_MAX_TOP = 64
+LEARNER_MAX_TOP, LEARNER_SHORT_ROW = 64, 1024
 
 # Every symbol include/learner_ops.h declares
 _i64, _rows, _seq, _view = C.c_int64, C.POINTER(LearnerRows), C.POINTER(LearnerSeq), C.POINTER(LearnerView)
@@ -158,7 +158,6 @@ LEARNER_SIGNATURES = {
     'lrn_choose': (_i32, [_i32, _vp, _rows, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64]),
     'lrn_score_workspace': (_i64, [_rows, _i32]),
     'lrn_score': (_i32, [_i32, _vp, _rows, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64]),
-    'lrn_score_backward_needs_stat': (_i32, [_rows]),
     'lrn_score_backward': (_i32, [_i32, _vp, _rows, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
     'lrn_scan_workspace': (_i64, [_seq]),
     'lrn_scan': (_i32, [_i32, _vp, _seq, _view, _view, C.c_double, _view, _vp, _view, _vp, _vp, _i64]),

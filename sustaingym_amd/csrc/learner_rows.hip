@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T
 
 // Up to eight levels: the row itself; then eight levels to a lane (a full set of wavefronts has the registers), sixteen where
 // a row would not fit a wavefront otherwise.
-constexpr int kGroupLevels = 1024;
+constexpr int kGroupLevels = LRN_SHORT_ROW;
 #define BY_LEVELS(K, call)                                                          \
     switch (K) {                                                                    \
         case 1: { constexpr int G = 1, E = 1; call; break; }                        \
@@ -948,8 +948,6 @@ int lrn_score(int32_t device, void* hip_stream, const lrn_rows* rows, const int6
     }
     BY_TYPE(rows->dtype, return (launch_wide<T, false>(R, ChooseOut{}, O, top, workspace, (hipStream_t)hip_stream, "lrn_score")));
 }
-
-int lrn_score_backward_needs_stat(const lrn_rows* rows) { return rows && rows->levels > kGroupLevels; }
 
 int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, const int64_t* level, const float* stat,
                        const float* entropy, const float* g_logprob, int32_t g_logprob_stride, const float* g_entropy,

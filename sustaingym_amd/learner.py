@@ -13,7 +13,10 @@ Every call runs on the current torch stream of its tensors' device, does not syn
 Tensors of any strides are taken as they are where the last dimension of logits and noise is dense; anything else is copied
 first.  Wrong arguments raise ``ValueError`` before anything is launched.  There is no CPU form: CPU tensors are refused.
 
-To capture a backward pass, ask for it with ``torch.autograd.grad`` inside the capture, on a forward pass of the same capture.
+To capture a backward pass into a graph, run the forward pass inside the same capture and ask for the gradients there with
+``torch.autograd.grad``, for leaves that no eager graph holds at that time (a tensor's ``detach().requires_grad_()`` taken inside
+the capture is one): torch orders a leaf's gradient behind the stream that first used the leaf, and a capture cannot wait for a
+stream outside it.
 """
 from __future__ import annotations
 
@@ -28,6 +31,7 @@ from . import _lib
 _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SEQ_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 MAX_TOP = _lib.LEARNER_MAX_TOP
+_SHORT_ROW = _lib.LEARNER_SHORT_ROW      # up to here no workspace and no statistics for the backward pass
 
 
 class LevelChoice(NamedTuple):
@@ -156,6 +160,8 @@ def _check_rows(logits, mask, noise=None):
     shape = logits.shape
     if not shape or not 1 <= shape[-1] < 2 ** 30:
         raise ValueError(f'logits: [..., levels], got {tuple(shape)}')
+    if mask is None and noise is None:
+        return
     for name, t, kind in (('mask', mask, torch.bool), ('noise', noise, torch.float32)):
         if t is None:
             continue
@@ -185,7 +191,7 @@ def choose_levels(logits, noise=None, mask=None) -> LevelChoice:
     entropy = torch.empty(shape, dtype=torch.float32, device=device)
     rows = _Rows(logits, mask, noise)
     ref = C.byref(rows.struct)
-    nbytes = lib.lrn_choose_workspace(ref)
+    nbytes = 0 if rows.struct.levels <= _SHORT_ROW else lib.lrn_choose_workspace(ref)
     ws = _workspace(nbytes, device)
     _check(lib.lrn_choose(device.index, _stream(device), ref, _ptr(rows.noise), rows.noise_strides[0], rows.noise_strides[1],
                           levels.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(), _ptr(ws), nbytes), 'choose_levels')
@@ -200,7 +206,7 @@ def _score(rows, levels, shape, device, top, want_stat):
     stat = torch.empty((*shape, 2), dtype=torch.float32, device=device) if want_stat else None
     tl = torch.empty((*shape, top), dtype=torch.float32, device=device) if top else None
     ti = torch.empty((*shape, top), dtype=torch.int64, device=device) if top else None
-    nbytes = lib.lrn_score_workspace(ref, top)
+    nbytes = 0 if rows.struct.levels <= _SHORT_ROW else lib.lrn_score_workspace(ref, top)
     ws = _workspace(nbytes, device)
     _check(lib.lrn_score(device.index, _stream(device), ref, levels.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
                          _ptr(stat), top, _ptr(tl), _ptr(ti), _ptr(ws), nbytes), 'level_logprobs')
@@ -227,7 +233,7 @@ class _LevelLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, levels, mask, top):
         rows = _Rows(logits, mask)
-        needs = bool(_lib.load().lrn_score_backward_needs_stat(C.byref(rows.struct)))
+        needs = rows.struct.levels > _SHORT_ROW
         logprobs, entropy, stat, tl, ti = _score(rows, levels, logits.shape[:-1], logits.device, top, needs)
         ctx.save_for_backward(logits, levels, mask, stat, entropy if needs else None)
         ctx.set_materialize_grads(False)

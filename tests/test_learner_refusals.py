@@ -21,6 +21,7 @@ def test_header_binding_and_library_agree():
     assert all(hasattr(lib, name) for name in learner_symbols())
     text = open(os.path.join(os.path.dirname(_lib.HEADER_PATH), 'learner_ops.h')).read()
     assert int(re.search(r'#define\s+LRN_MAX_TOP\s+(\d+)', text).group(1)) == _lib.LEARNER_MAX_TOP == learner.MAX_TOP
+    assert int(re.search(r'#define\s+LRN_SHORT_ROW\s+(\d+)', text).group(1)) == _lib.LEARNER_SHORT_ROW
 
 
 def test_cpu_tensors_are_refused():
