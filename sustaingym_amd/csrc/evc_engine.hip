@@ -1451,7 +1451,10 @@ int evc_reset_host(evc_engine* e, const int32_t* env_ids, int32_t count, const i
 
 int evc_host_register(void* ptr, size_t bytes) {
     if (!ptr || bytes == 0) return fail(EVC_EINVAL, "evc_host_register: bad argument");
-    HIP_TRY(hipHostRegister(ptr, bytes, hipHostRegisterDefault));
+    if (const hipError_t rc = hipHostRegister(ptr, bytes, hipHostRegisterDefault); rc != hipSuccess) {
+        (void)hipGetLastError();                 // the caller goes on with pageable memory: the next launch must not report this
+        return fail(EVC_EHIP, "hipHostRegister failed: %s", hipGetErrorString(rc));
+    }
     return EVC_OK;
 }
 
