@@ -57,7 +57,8 @@ __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgc
 
 // The 64 best of what a wavefront has seen, lane i the i-th (falling, the lowest index first among equals).  Candidates go in
 // one at a time: k (1 + log(n / k)) of n values do.  What an insertion costs is latency, so nothing in it goes through LDS: the
-// candidate and the bound are scalars (v_readlane), the entries behind it move up by one lane with a whole-wavefront shift.
+// candidate and the bound are scalars (v_readlane), the entries behind it move up by one lane with a whole-wavefront shift
+// (exchanges through LDS instead: 45 us for what takes 32, both without the floor).
 struct TopList {
     float v;
     int j;
@@ -146,6 +147,11 @@ struct BackIn { const int64_t* level; const float* stat; const float* entropy; c
 // every weight is computed once; the group's sums go through DPP.  The backward pass computes the row's maximum and sums again
 // from the logits that it has to read anyway: cheaper than 12 bytes a row of saved statistics.  Its results meet in LDS, from
 // where they leave as one run of 16-byte stores.
+//
+// Bound by memory where rows are short (65 536 x 54 x 5: float32 127 MB in 25 us = 5.1 TB/s, a large copy's rate; bfloat16 with a
+// mask 110 MB in 31, backward 145 MB in 31), by the issue of some 25 instructions a level where they are not and hold two bytes
+// each (16 000 x 1000 bfloat16: 13 us forward, 19 backward).  An earlier form that brought all rows through LDS, with a division
+// of every element's index, took 28 and 37 us for the first, 16 and 30 for the last.
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -166,8 +172,8 @@ template <int G, class F> __device__ __forceinline__ void over_group(F&& f) {
 template <class V, int N> __device__ __forceinline__ void take(const V* p, V (&to)[N]) { __builtin_memcpy(to, p, sizeof(to)); }
 
 // A workgroup's rows of up to eight 16-bit logits, and their mask, through LDS: at 2 to 16 bytes a row a lane's own loads are
-// many, small and askew, the run of them is a few 16-byte loads (65 536 x 54 rows of
-// five with a mask, 110 MB: 30.6 us instead of 32.6).
+// many, small and askew, the run of them is a few 16-byte loads (65 536 x 54 rows of five bfloat16 with a mask, 110 MB: 30.6 us
+// instead of 32.6).
 template <class T, int G, int E> constexpr bool kStaged = G == 1 && sizeof(T) == 2;
 template <class T, int E> struct Stage {
     __attribute__((aligned(16))) T z[256 * E];
@@ -498,6 +504,10 @@ int group_rows(int K) { int n = 256; BY_LEVELS(K, (n = 256 / G, (void)E)); retur
 // running maximum and sums of its own, rescaled when a piece raises the maximum; the lanes join at the end.  Where there are
 // too few rows to fill the GPU a row is cut into up to 64 parts, whose sums, best level and best alternatives go through the
 // workspace to a second launch, a wavefront to a row.
+//
+// 1024 x 32768 bfloat16: 67 MB in 16 us (4.2 TB/s), bound by instructions as much as by memory: eleven a level, four of them the
+// exponential's issue.  A row in parts is bound by latency: 8 x 131 071 float32 with 20 alternatives 14 + 10.5 us for 4 MB (a
+// wavefront to a row, as it was first, took 1070).
 
 template <class T> struct Piece {
     static constexpr int N = 16 / sizeof(T);
@@ -764,7 +774,8 @@ __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut 
     }
 }
 
-// One piece of 16 bytes after the other, with the row's statistics: bound by memory.
+// One piece of 16 bytes after the other, with the row's statistics: bound by memory (1024 x 32768 bfloat16: 134 MB in 23.5 us,
+// 5.7 TB/s; the forward pass has just left the logits in the last-level cache).
 constexpr int kBackPieces = 4;       // pieces a lane
 template <class T>
 __global__ __launch_bounds__(256) void wide_backward_kernel(Rows R, BackIn I, T* grad, int parts) {

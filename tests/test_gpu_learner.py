@@ -244,7 +244,7 @@ def test_row_gradient_against_differences(K):
 
 SCANS = [((1, 1, 1), 0), ((1, 256, 512), 0), ((2, 3, 5), 0), ((5, 1, 64), 0), ((7, 2, 65), 1), ((288, 4, 3), 0), ((3, 289, 33), 1), ((2, 128, 128), 1),
          ((129, 2, 72), 0), ((1, 1000, 72), 1), ((2, 511, 4), 1), ((17, 200), 0), ((200, 17), 1), ((3, 1025), 1), ((1, 4099), 1), ((4099,), 0),
-         ((31,), 0), ((64, 64), 1), ((1, 3000, 8), 1), ((1, 9000, 1), 1), ((4000, 1, 2), 0), ((20, 33, 1), 0), ((40, 70, 1000), 0), ((9, 65540), 0), ((600, 3, 34), 0)]
+         ((31,), 0), ((64, 64), 1), ((1, 3000, 8), 1), ((1, 9000, 1), 1), ((4000, 1, 2), 0), ((20, 33, 1), 0), ((40, 70, 1000), 0), ((9, 65540), 0), ((600, 3, 34), 0), ((20, 140000), 0)]
 
 
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16', 'f64'])
@@ -413,7 +413,7 @@ def test_scan_of_any_stride():
     near(learner.gated_scan(one, 0.5)[0], *ref.scan(host(one.contiguous()), 0.5, None, None, 0, False)['h'], 'expanded')
 
 
-@pytest.mark.parametrize('T,N', [(1, 1), (288, 1), (5, 64), (100, 1000), (288, 4096), (1, 70000), (2049, 3), (20000, 2), (40, 66000), (20, 65537)])
+@pytest.mark.parametrize('T,N', [(1, 1), (288, 1), (5, 64), (100, 1000), (288, 4096), (1, 70000), (2049, 3), (20000, 2), (40, 66000), (20, 65537), (20, 140000)])
 def test_advantages_against_float64(T, N):
     from sustaingym_amd import learner
     g = gen(T + N)
@@ -679,3 +679,48 @@ def test_calls_from_two_threads_on_two_streams():
         t.join()
     assert sorted(wrong) == [0, 1]
     assert all(torch.equal(a, b) for k in got for one in got[k] for a, b in zip(one, want))
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'f64', 'bf16'])
+def test_scan_of_one_long_sequence_in_parts(dtype):
+    """70 001 steps of one sequence, written out in Python floats (float64) with the bounds of learner_reference.scan."""
+    from sustaingym_amd import learner
+    kind, T = TYPES[dtype], 70001
+    state = torch.float64 if kind == torch.float64 else torch.float32
+    u, half = (2.0 ** -53, 0.0) if kind == torch.float64 else (ref.U, ref.half_step(kind))
+    for reverse in (False, True):
+        g = gen(41)
+        x, gate = (torch.rand((1, T), generator=g, device='cuda').sub(0.3).to(kind).requires_grad_(True) for _ in range(2))
+        init = torch.ones(1, dtype=state, device='cuda', requires_grad=True)
+        resets = torch.rand((1, T), generator=g, device='cuda') < 1e-3
+        up = torch.randn((1, T), generator=g, device='cuda').to(kind)
+        h, final = learner.gated_scan(x, gate, init, resets, 1, reverse)
+        gx, gg, gi = torch.autograd.grad((h, final), (x, gate, init), (up, torch.ones_like(final)))
+        flip = (lambda v: v[::-1]) if reverse else (lambda v: v)
+        X, A, R, Up = (flip(host(t)[0].tolist()) for t in (x, gate, resets, up))
+
+        def walk(xs, gates, s):
+            out, tol, M, N = [], [], abs(s), 0.0
+            for xt, a in zip(xs, gates):
+                s = a * s + xt
+                N = abs(a) * (N + M)
+                M = abs(a) * M + abs(xt)
+                out.append(s)
+                tol.append(u * (2 * N + 16 * M) + 1e-37)
+            return out, tol
+        A = [0.0 if r else a for a, r in zip(A, R)]
+        H, Ht = walk(X, A, 1.0)
+        G, Gt = walk(Up[::-1], [1.0] + A[:0:-1], 1.0)
+        G, Gt = G[::-1], Gt[::-1]
+        prev, pt = [1.0] + H[:-1], [0.0] + Ht[:-1]
+        gate_grad = [0.0 if r else a * b for a, b, r in zip(G, prev, R)]
+        gate_tol = [abs(a) * (tb + half * abs(b)) + ta * abs(b) * 2 + 2 * u * abs(a * b) for a, ta, b, tb in zip(G, Gt, prev, pt)]
+
+        def check(got, want, tol, what, rounded=True):
+            want, tol = (torch.tensor(flip(v), dtype=torch.float64)[None] for v in (want, tol))
+            near(got, want, tol + (half * (want.abs() + tol) if rounded else 0), what)
+        check(h, H, Ht, 'h')
+        check(gx, G, Gt, 'grad_x')
+        check(gg, gate_grad, gate_tol, 'grad_gate')
+        assert abs(float(final) - H[-1]) <= Ht[-1]
+        assert abs(float(gi) - A[0] * G[0]) <= abs(A[0]) * Gt[0] + 2 * u * abs(A[0] * G[0])
