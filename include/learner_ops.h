@@ -48,7 +48,8 @@ typedef struct lrn_rows {
 
 /* The level with the largest logit + noise among the allowed ones (the lowest of equals), its log probability under
  * the logits alone and the row's entropy.  noise (NULL = none): float32, row (o, i) at o * noise_outer +
- * i * noise_inner, adjacent.  With Gumbel noise the level is a sample of the row's distribution. */
+ * i * noise_inner, adjacent.  With Gumbel noise the level is a sample of the row's distribution.  Noise of -inf or NaN puts a level
+ * behind all others of its row. */
 int64_t lrn_choose_workspace(const lrn_rows* rows);
 int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const float* noise, int64_t noise_outer,
                int64_t noise_inner, int64_t* level_out, float* logprob_out, float* entropy_out, void* workspace,

@@ -52,6 +52,10 @@ struct Best {
     __device__ __forceinline__ void add(float x, int i) { if (x > v || (x == v && i < j)) { v = x; j = i; } }
 };
 
+// A level's place in the choice.  Noise of -inf (the logarithm of a logarithm of a uniform 0) and NaN puts an allowed level last,
+// not out: the only one left is chosen all the same.
+__device__ __forceinline__ float choice_key(float z, float noise) { return fmaxf(z + noise, -3.4028234e38f); }
+
 __device__ __forceinline__ float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 __device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
@@ -299,7 +303,7 @@ __global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) 
     float chosen = 0.0f;
 #pragma unroll
     for (int k = 0; k < E; k++) {
-        const float key = O.noise ? z[k] + w[k] : z[k];
+        const float key = O.noise ? choice_key(z[k], w[k]) : z[k];
         if (z[k] > kNegInf && key > b.v) { b.v = key; b.j = g * E + k; chosen = z[k]; }
     }
     over_group<G>([&](auto from) {
@@ -454,7 +458,7 @@ __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T
             // p (g_lp + g_h (log p + H)), log p = z - m - log s; a weight of 0 has p log p = 0
             float d = -(e[k] * inv) * (gl + gh * (e[k] > 0.0f ? z[k] - m + lift : 0.0f));
             if (k == mine) d += gl;
-            if (z[k] == kNegInf) d = l >= K ? gl : 0.0f;
+            if (z[k] == kNegInf) d = 0.0f;
             if (g * E + k < K) to[k] = (T)d;
         }
     }
@@ -704,7 +708,7 @@ __global__ __launch_bounds__(256) void wide_kernel(Rows R, ChooseOut C, ScoreOut
         if constexpr (CHOOSE) {
 #pragma unroll
             for (int k = 0; k < N; k++) {                        // (a lane's levels rise)
-                const float key = ns ? z[k] + w[k] : z[k];
+                const float key = ns ? choice_key(z[k], w[k]) : z[k];
                 if (z[k] > kNegInf && key > b.v) { b.v = key; b.j = e0 + k; }
             }
         }

@@ -50,7 +50,7 @@ struct Seq {
     const void* edge;           // backward: the initial state; advantages: V behind the last step (float32)
     void* final;
     int64_t part;               // steps of a part
-    int64_t tight;              // COLUMNS: tiles of a sequence where a tile may not reach over two (else 0)
+    int64_t tight, width;       // COLUMNS: tiles of a sequence where a tile may not reach over two (else 0), and their channels
     void* pairs;                // [parts][2][cols]
 };
 
@@ -282,20 +282,20 @@ __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, 
     }
 }
 
-template <class E> __device__ __forceinline__ const char* uniform_part(const View& v, int64_t b) { return v.p ? (const char*)v.p + b * v.sb * (int64_t)sizeof(E) : nullptr; }
+template <class E> __device__ __forceinline__ const char* uniform_part(const View& v, int64_t b, int64_t c) { return v.p ? (const char*)v.p + (b * v.sb + c * v.sc) * (int64_t)sizeof(E) : nullptr; }
 template <class E> __device__ __forceinline__ uint32_t lane_part(const View& v, int64_t b, int64_t c) { return (uint32_t)((b * v.sb + c * v.sc) * (int64_t)sizeof(E)); }
 
-// Column q = (b, c) seen from sequence b0.
-template <class O> __device__ __forceinline__ Place place_of(const Seq& S, int64_t b0, int64_t b, int64_t c) {
+// Column q = (b, c) seen from the tile's first, (b0, c0).
+template <class O> __device__ __forceinline__ Place place_of(const Seq& S, int64_t b0, int64_t c0, int64_t b, int64_t c) {
     using T = typename O::T;
     using E = typename O::Out;
     Place P;
-    P.x = uniform_part<T>(S.x, b0); P.ox = lane_part<T>(S.x, b - b0, c);
-    P.gate = uniform_part<T>(S.gate, b0); P.og = lane_part<T>(S.gate, b - b0, c);
-    P.before = uniform_part<E>(S.before, b0); P.ob = lane_part<E>(S.before, b - b0, c);
-    P.resets = uniform_part<uint8_t>(S.resets, b0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
-    P.h = (char*)uniform_part<E>(S.h, b0); P.oh = lane_part<E>(S.h, b - b0, c);
-    P.second = (char*)uniform_part<E>(S.second, b0); P.oo = lane_part<E>(S.second, b - b0, c);
+    P.x = uniform_part<T>(S.x, b0, c0); P.ox = lane_part<T>(S.x, b - b0, c - c0);
+    P.gate = uniform_part<T>(S.gate, b0, c0); P.og = lane_part<T>(S.gate, b - b0, c - c0);
+    P.before = uniform_part<E>(S.before, b0, c0); P.ob = lane_part<E>(S.before, b - b0, c - c0);
+    P.resets = uniform_part<uint8_t>(S.resets, b0, 0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
+    P.h = (char*)uniform_part<E>(S.h, b0, c0); P.oh = lane_part<E>(S.h, b - b0, c - c0);
+    P.second = (char*)uniform_part<E>(S.second, b0, c0); P.oo = lane_part<E>(S.second, b - b0, c - c0);
     P.next_flags = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
     return P;
 }
@@ -346,12 +346,13 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     __shared__ Pair<W> pairs_of[2][WT > 1 ? WT : 1][WT > 1 ? 64 * V : 1];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
     const int64_t tile = (int64_t)blockIdx.x * WC + (WT > 1 ? 0 : wave);
-    int64_t b0, b, c, q;
+    int64_t b0, c0 = 0, b, c, q;
     bool there;
-    if (S.tight) {                                    // a tile has columns of one sequence
+    if (V == 1 && S.tight) {                          // a tile has columns of one sequence
         b0 = b = tile / S.tight;
-        c = (tile - b * S.tight) * 64 * V + lane * V;
-        there = c < S.channels && b < S.cols / S.channels;
+        c0 = (tile - b * S.tight) * S.width;
+        c = c0 + lane;
+        there = lane < S.width && c < S.channels && b < S.cols / S.channels;
         q = b * S.channels + c;
     } else {
         q = tile * 64 * V + lane * V;
@@ -361,11 +362,11 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
         c = q - b * S.channels;
     }
     // (a lane without a column goes along to the barriers, reads the tile's first column and writes nothing)
-    if (!there) { b = b0; c = S.tight ? 0 : tile * 64 * V - b0 * S.channels; q = b * S.channels + c; }
+    if (!there) { b = b0; c = V == 1 && S.tight ? c0 : tile * 64 * V - b0 * S.channels; q = b * S.channels + c; }
     if (q >= S.cols) return;                          // WT = 1: a whole wavefront behind the last tile
     const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
     const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Place P = place_of<O>(S, b0, b, c);
+    const Place P = place_of<O>(S, b0, c0, b, c);
     W carry[V], edge[V];
     Pair<W> all[V];
 #pragma unroll
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     if (q >= S.cols) return;                          // WT > 1: a whole workgroup, else a whole wavefront and no barrier
     const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
     const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
-    const Place P = place_of<O>(S, q, q, 0);       // (one channel: the column is the sequence)
+    const Place P = place_of<O>(S, q, 0, q, 0);       // (one channel: the column is the sequence)
     W carry = first_state<K, W>(S, q);
     const W edge[1] = {edge_of<K, W>(S, q)};
     Pair<W> all{W(1), W(0)};
@@ -673,15 +674,25 @@ template <class O> constexpr int kMany = std::is_same<typename O::T, double>::va
 
 // A lane's part of an address has 32 bits: how far the columns of one tile lie apart in a view.
 bool near(const View& v, const Seq& S, int64_t size, int tile) {
+    constexpr int64_t far = (int64_t)1 << 40;
     const int64_t over = std::min(S.cols / S.channels - 1, tile / S.channels + 1);
-    return !v.p || (v.sb <= ((int64_t)1 << 40) && over * v.sb * size + S.channels * v.sc * size < ((int64_t)1 << 32));
+    return !v.p || (v.sb <= far && v.sc <= far / S.channels && over * v.sb * size + S.channels * v.sc * size < ((int64_t)1 << 32));
+}
+template <class O> bool near(const Seq& S, int tile) {
+    constexpr int64_t n = sizeof(typename O::T);
+    return near(S.x, S, n, tile) && near(S.gate, S, n, tile) && near(S.before, S, n, tile) && near(S.resets, S, 1, tile) &&
+           near(S.h, S, n, tile) && near(S.second, S, n, tile);
 }
 
 template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
-    constexpr int64_t n = sizeof(typename O::T);
-    const bool flat = near(S.x, S, n, 64 * V) && near(S.gate, S, n, 64 * V) && near(S.before, S, n, 64 * V) && near(S.resets, S, 1, 64 * V) &&
-                      near(S.h, S, n, 64 * V) && near(S.second, S, n, 64 * V);
-    S.tight = flat ? 0 : cdiv(S.channels, 64 * V);
+    const bool flat = V > 1 || near<O>(S, 64);
+    if (!flat) {
+        // Channels that lie so far apart that 64 of them pass 32 bits (time is the fast index of a long trajectory): fewer to a tile.
+        S.width = 64;
+        for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second})
+            while (S.width > 1 && v->p && v->sc >= ((int64_t)1 << 32) / (S.width * (int64_t)sizeof(typename O::T))) S.width /= 2;
+        S.tight = cdiv(S.channels, S.width);
+    }
     const int64_t tiles = cdiv(flat ? cdiv(S.cols, 64 * V) : S.cols / S.channels * S.tight, WT == 1 ? 4 : 1);
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
@@ -715,6 +726,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
     bool runs = S.channels == 1 && S.steps > 1 && (st == 1 || st == -1);
     for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.second}) runs = runs && (!v->p || v->st == st);
     for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || v->sb != 1);
+    runs = runs && S.cols < (1 << 25);                // (a grid has fewer than 2^32 lanes)
     const Deal d = runs ? deal_runs(S.steps, S.cols) : deal_columns(S.steps, S.cols);
     if (d.parts > 65535 || S.cols > ((int64_t)1 << 31)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
     S.part = d.part;
@@ -727,7 +739,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
         // steps of 72 float32: 45 us instead of 55; float64 gains nothing), and for advantages of many sequences, whose 21 bytes
         // a step keep the memory busy with half the wavefronts (but not in parts: 2048 x 2000 float64 41 us instead of 31).
         const bool even = S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) && dense(S.gate, S.channels) &&
-                          dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels);
+                          dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels) && near<O>(S, 128);
         if constexpr (O::K == ADVANTAGES) {
             if (even && S.cols >= 65536 && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
             if (even && S.cols >= 65536 && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;

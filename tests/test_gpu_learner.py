@@ -724,3 +724,104 @@ def test_scan_of_one_long_sequence_in_parts(dtype):
         check(gg, gate_grad, gate_tol, 'grad_gate')
         assert abs(float(final) - H[-1]) <= Ht[-1]
         assert abs(float(gi) - A[0] * G[0]) <= abs(A[0]) * Gt[0] + 2 * u * abs(A[0] * G[0])
+
+
+@pytest.mark.parametrize('K', [1, 5, 40, 300, 5000])
+def test_noise_never_takes_an_allowed_level_out(K):
+    """-log(-log(0)) is -inf: a row's only allowed level, or all of them, may get it.  So may the lowest value as a mask overflow."""
+    from sustaingym_amd import learner
+    z = torch.zeros((6, K), device='cuda')
+    mask = torch.ones((6, K), dtype=torch.bool, device='cuda')
+    noise = torch.zeros((6, K), device='cuda')
+    last = K - 1
+    mask[0, :last] = False
+    noise[0] = -math.inf                                             # the only one left
+    noise[1] = -math.inf                                             # all: the lowest index
+    noise[2], noise[2, last] = -math.inf, -50.0                      # a number is ahead of -inf
+    noise[3], noise[3, last] = math.nan, -1e30                       # and of NaN
+    z[4], noise[4] = torch.finfo(torch.float32).min, -1e38           # the sum passes float32
+    mask[4, :last] = False
+    mask[5], noise[5] = False, -math.inf                             # nothing allowed
+    c = learner.choose_levels(z, noise, mask)
+    assert host(c.levels).tolist() == [last, 0, last, last, last, 0]
+    lp = host(c.logprobs)
+    assert torch.isfinite(lp).all() and lp[0] == 0.0 and lp[4] == 0.0 and lp[5] == 0.0
+    assert float((lp[1:4] + math.log(K)).abs().max()) <= 1e-5        # (17 nats at most: 64 steps of float32)
+
+
+@pytest.mark.parametrize('K', [5, 40, 3001])
+def test_gradient_of_a_level_beyond_the_row(K):
+    """NaN where the row allows something, nothing where it does not."""
+    from sustaingym_amd import learner
+    z = torch.zeros((3, K), device='cuda', requires_grad=True)
+    mask = torch.ones((3, K), dtype=torch.bool, device='cuda')
+    mask[:, 1] = False
+    s = learner.level_logprobs(z, torch.tensor([K, 0, 2 ** 40], device='cuda'), mask)
+    gr = host(torch.autograd.grad(s.logprobs, z, torch.ones(3, device='cuda'))[0])
+    assert not gr[:, 1].any() and torch.isfinite(gr[1]).all()
+    assert torch.isnan(gr[0, [0] + list(range(2, K))]).all() and torch.isnan(gr[2, 0])
+
+
+@pytest.mark.parametrize('shape,strides,dim', [((20, 3, 5), (3, 1, 2 ** 30), 0), ((600, 2, 60), (2, 1, 2 ** 26), 0), ((3, 40, 70), (64, 1, 2 ** 25 + 6), 1),
+                                               ((2, 1200, 5), (2 ** 29, 1, 2 ** 30), 1), ((9, 2, 130), (2, 1, 2 ** 25 - 2), 0)])
+def test_channels_far_apart(shape, strides, dim):
+    """Channels whose columns of one tile lie more than 2^32 bytes apart, as inputs, incoming gradients and outputs."""
+    import ctypes as C
+    from sustaingym_amd import _lib, learner
+    g = gen(41)
+    size = sum((n - 1) * s for n, s in zip(shape, strides)) + 1
+    big = torch.empty(size, dtype=torch.float16, device='cuda')                  # up to 9.4 GB, written only where it is read
+    x = big.as_strided(shape, strides)
+    x.copy_(torch.randn(shape, generator=g, device='cuda'))
+    gate = torch.rand(shape, generator=g, device='cuda').half()
+    up = torch.randn(shape, generator=g, device='cuda').half()
+    resets = torch.rand(shape[:2], generator=g, device='cuda') < 0.1
+    want = ref.scan(host(x.contiguous()), host(gate), None, host(resets), dim, False, host(up))
+    h, final = learner.gated_scan(x, gate, None, resets, dim)
+    near(h, *want['h'], 'h')
+    near(final, *want['final'], 'final')
+    # an output in that layout
+    dense = x.contiguous()
+    lib, seq = _lib.load(), learner._sequence(shape, dim, False, torch.float16)
+    ws = torch.empty(max(1, lib.lrn_scan_workspace(C.byref(seq))), dtype=torch.uint8, device='cuda')
+    state = torch.empty(shape[:dim] + shape[dim + 1:], dtype=torch.float32, device='cuda')
+    rc = lib.lrn_scan(x.device.index, learner._stream(x.device), C.byref(seq), C.byref(learner._view(dense, dim)), C.byref(learner._view(gate, dim)), 0.0,
+                      C.byref(learner._view(resets, dim)), None, C.byref(learner._view(x, dim)), state.data_ptr(), ws.data_ptr(), ws.numel())
+    assert rc == 0
+    near(x.contiguous(), *want['h'], 'h in that layout')
+    # as the gradient that comes in
+    leaves = dense.requires_grad_(True), gate.requires_grad_(True)
+    h = learner.gated_scan(*leaves, None, resets, dim)[0]
+    x.copy_(up)
+    gx, gg = torch.autograd.grad(h, leaves, x)
+    near(gx, *want['grad_x'], 'grad_x')
+    near(gg, *want['grad_gate'], 'grad_gate')
+
+
+@pytest.mark.parametrize('far', [1, 2 ** 26])
+def test_resets_whose_sequences_lie_far_apart(far):
+    """Two columns to a lane and flags that one address cannot reach for both."""
+    from sustaingym_amd import learner
+    g = gen(43)
+    T, N = 1100, 66
+    x = torch.randn((T, N), generator=g, device='cuda')
+    flags = torch.rand((T, N), generator=g, device='cuda') < 0.05
+    if far > 1:
+        store = torch.empty(far * (N - 1) + T, dtype=torch.bool, device='cuda')          # 4.4 GB
+        resets = store.as_strided((T, N), (1, far))
+        resets.copy_(flags)
+    else:
+        resets = flags
+    for reverse in (False, True):
+        want = ref.scan(host(x), 0.9, None, host(flags), 0, reverse)
+        h, final = learner.gated_scan(x, 0.9, None, resets, 0, reverse)
+        near(h, *want['h'], 'h')
+        near(final, *want['final'], 'final')
+
+
+def test_more_sequences_than_a_grid_of_wavefronts():
+    from sustaingym_amd import learner
+    x = torch.randn((2 ** 25 + 3, 2), generator=gen(44), device='cuda')
+    h, final = learner.gated_scan(x, 0.5, dim=1)
+    assert torch.equal(h[:, 0], x[:, 0]) and torch.equal(h[:, 1], torch.addcmul(x[:, 1], x[:, 0], torch.full_like(x[:, 0], 0.5)))
+    assert torch.equal(final, h[:, 1])
