@@ -50,6 +50,7 @@ struct Seq {
     const void* edge;           // backward: the initial state; advantages: V behind the last step (float32)
     void* final;
     int64_t part;               // steps of a part
+    int64_t group;              // RUNS: lanes of a column, where a wavefront has all its steps
     int64_t tight, width;       // COLUMNS: tiles of a sequence where a tile may not reach over two (else 0), and their channels
     void* pairs;                // [parts][2][cols]
 };
@@ -448,7 +449,7 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     }
 }
 
-// ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column -----------------------------------------------
+// ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column; or, of short ones, several columns ------------
 
 // COUNT steps from `from`, 16 bytes at a time (at any alignment); DIR: whether they rise or fall in memory.  Not FULL: one by
 // one, what lies outside [0, hi) is 0.
@@ -490,21 +491,31 @@ __device__ __forceinline__ void put_run(char* base, int64_t from, int64_t hi, co
     }
 }
 
+// The run's own COUNT steps, with the one before them (BEFORE) or behind them (else); 0 where there is none.
+template <class E, int DIR, bool FULL, bool BEFORE, int COUNT>
+__device__ __forceinline__ void get_shifted(const char* base, int64_t u0, int64_t end, int64_t hi, E* to) {
+    if constexpr (FULL) {
+        E own[L];
+        get_run<E, DIR, L, true>(base, u0, end, own);
+        get_run<E, DIR, 1, false>(base, BEFORE ? u0 - 1 : u0 + L, hi, BEFORE ? to : to + L - 1);
+#pragma unroll
+        for (int i = 1; i < (BEFORE ? COUNT : L); i++) to[BEFORE ? i : i - 1] = own[BEFORE ? i - 1 : i];
+    } else get_run<E, DIR, COUNT, false>(base, BEFORE ? u0 - 1 : u0 + 1, hi, to);
+}
+
 template <class O, int DIR, bool FULL, bool APPLYING>
 __device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u0, int64_t end, Raw<O, 1>& d) {
     using T = typename O::T;
-    constexpr int shift = O::K == BACKWARD ? 1 : 0;
     get_run<T, DIR, L, FULL>(P.x, u0, end, d.x);
-    if constexpr (O::GATE) get_run<T, DIR, L, FULL>(P.gate, u0 - shift, end, d.g);
-    if constexpr (O::RESETS) {
-        get_run<uint8_t, DIR, L, FULL>(P.resets, u0 - shift, end, d.r);
-        if constexpr (O::K == BACKWARD && O::SECOND) get_run<uint8_t, DIR, 1, FULL>(P.resets, u0 - 1 + L, end, d.r + L);
+    if constexpr (O::K == BACKWARD) {
+        if constexpr (O::GATE) get_shifted<T, DIR, FULL, true, L>(P.gate, u0, end, end, d.g);
+        if constexpr (O::RESETS) get_shifted<uint8_t, DIR, FULL, true, L + (O::SECOND ? 1 : 0)>(P.resets, u0, end, end, d.r);
+        if constexpr (O::SECOND && APPLYING) get_shifted<T, DIR, FULL, false, L>(P.before, u0, end, S.steps, d.before);
+    } else {
+        if constexpr (O::GATE) get_run<T, DIR, L, FULL>(P.gate, u0, end, d.g);
+        if constexpr (O::RESETS) get_run<uint8_t, DIR, L, FULL>(P.resets, u0, end, d.r);
+        if constexpr (O::K == ADVANTAGES) get_shifted<float, DIR, FULL, true, L + 1>(P.before, u0, end, end, d.v);
     }
-    if constexpr (O::K == ADVANTAGES) {
-        get_run<float, DIR, 1, FULL>(P.before, u0 - 1, end, d.v);
-        get_run<float, DIR, L, FULL>(P.before, u0, end, d.v + 1);
-    }
-    if constexpr (O::K == BACKWARD && O::SECOND && APPLYING) get_run<T, DIR, L, FULL>(P.before, u0 + 1, S.steps, d.before);
 }
 
 template <class O, int DIR, bool FULL, bool APPLYING>
@@ -529,9 +540,10 @@ __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run
 }
 
 template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
-template <class W> __device__ __forceinline__ void wave_scan(Pair<W>& p, int lane) {
+template <class W> __device__ __forceinline__ void wave_scan(Pair<W>& p, int lane, int group) {
 #pragma unroll
     for (int by = 1; by < 64; by <<= 1) {
+        if (by >= group) break;
         const Pair<W> o = up(p, by);
         if (lane >= by) p.after(o);
     }
@@ -544,38 +556,42 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
     using W = typename O::W;
     constexpr int64_t TURN = WT * 64 * L;
     __shared__ W pa[2][WT], ph[2][WT];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
-    const int64_t q = WT > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-    if (q >= S.cols) return;                          // WT > 1: a whole workgroup, else a whole wavefront and no barrier
+    const int group = WT > 1 ? 64 : (int)S.group;     // lanes of a column
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = WT > 1 ? wave : 0;
+    const int lane = WT > 1 ? threadIdx.x & 63 : threadIdx.x & (group - 1), last = (threadIdx.x & 63) | (group - 1);
+    const int64_t q = WT > 1 ? (int64_t)blockIdx.x : ((int64_t)blockIdx.x * 256 + threadIdx.x) / group;
+    if (q >= S.cols) return;                          // WT > 1: a whole workgroup, else whole groups of lanes and no barrier
     const int64_t part = PH == WHOLE ? 0 : blockIdx.y;
     const int64_t begin = part * S.part, end = PH == WHOLE ? S.steps : min(begin + S.part, S.steps);
     const Place P = place_of<O>(S, q, 0, q, 0);       // (one channel: the column is the sequence)
     W carry = first_state<K, W>(S, q);
     const W edge[1] = {edge_of<K, W>(S, q)};
     Pair<W> all{W(1), W(0)};
-    const int64_t mine = (int64_t)(wt * 64 + lane) * L;
+    const int64_t mine = (int64_t)(wt * 64 + lane) * L, turn_steps = WT > 1 ? TURN : group * L;
     if constexpr (PH == APPLY) {
         const int64_t share = (part + WT * 64 - 1) / (WT * 64), from = min((wt * 64 + lane) * share, part), to = min(from + share, part);
         Pair<W> p = joined_parts<W>(S, from, to, q);
-        wave_scan(p, lane);
+        wave_scan(p, lane, 64);
         if (lane == 63) { pa[1][wt] = p.a; ph[1][wt] = p.h; }
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < WT; w++) carry = step(pa[1][w], carry, ph[1][w]);
     }
     int turn = 0;
-    for (int64_t u = begin; u < end; u += TURN, turn ^= 1) {
-        const int64_t u0 = u + mine, first = u + (int64_t)wt * 64 * L;
-        // all lanes' steps, the ones before them and the ones behind them are there (the same for the wavefront)
-        const bool full = first + 64 * L <= end && (K == SCAN || first > 0) && (K != BACKWARD || first + 64 * L < S.steps);
+    for (int64_t u = begin; u < end; u += turn_steps, turn ^= 1) {
+        const int64_t u0 = u + mine;
         Run<O, 1> f;
-        if (full) take_run<O, DIR, true, PH != PAIRS>(S, P, edge, u0, end, f);
-        else take_run<O, DIR, false, PH != PAIRS>(S, P, edge, u0, end, f);
+        if (u0 + L <= end) take_run<O, DIR, true, PH != PAIRS>(S, P, edge, u0, end, f);
+        else if (u0 < end) take_run<O, DIR, false, PH != PAIRS>(S, P, edge, u0, end, f);
+        else {
+#pragma unroll
+            for (int i = 0; i < L; i++) { f.a[i] = W(1); f.x[i] = W(0); if constexpr (O::SECOND) f.extra[i] = 0; }
+        }
         Pair<W> p = pair_of<O, 1>(f, 0);
-        wave_scan(p, lane);
+        wave_scan(p, lane, group);
         Pair<W> front = up(p, 1);                     // of the lanes before this one
         if (lane == 0) front = Pair<W>{W(1), W(0)};
-        Pair<W> whole{__shfl(p.a, 63), __shfl(p.h, 63)};
+        Pair<W> whole{__shfl(p.a, last), __shfl(p.h, last)};
         if constexpr (WT > 1) {
             if (lane == 0) { pa[turn][wt] = whole.a; ph[turn][wt] = whole.h; }
             __syncthreads();
@@ -593,8 +609,8 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void runs_kernel(Seq S) {
         } else {
             const W h = step(front.a, carry, front.h);
             carry = step(whole.a, carry, whole.h);
-            if (full) walk_run<O, DIR, true>(S, P, f, u0, end, h);
-            else walk_run<O, DIR, false>(S, P, f, u0, end, h);
+            if (u0 + L <= end) walk_run<O, DIR, true>(S, P, f, u0, end, h);
+            else if (u0 < end) walk_run<O, DIR, false>(S, P, f, u0, end, h);
         }
     }
     if (wt || lane) return;
@@ -703,7 +719,11 @@ template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hip
     } else if constexpr (V == 1 || WT != kMany<O>) columns_kernel<O, V, WT, WHOLE><<<(unsigned)tiles, threads, 0, stream>>>(S);
 }
 template <class O, int DIR, int WT> void launch_runs(Seq& S, const Deal& d, hipStream_t stream) {
-    const int64_t blocks = WT == 1 ? cdiv(S.cols, 4) : S.cols;
+    // As many lanes to a column as it has runs, so that short sequences share a wavefront (1 048 576 of 16 float32: 23 us, 5.9 TB/s
+    // out of the last-level cache; a wavefront to each took 297, by columns 90).
+    S.group = 1;
+    while (S.group < 64 && S.group * L < S.steps) S.group *= 2;
+    const int64_t blocks = WT == 1 ? cdiv(S.cols * S.group, 256) : S.cols;
     const int threads = WT == 1 ? 256 : 64 * WT;
     if (d.parts > 1) {
         if constexpr (WT == kMany<O>) {
@@ -726,7 +746,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
     bool runs = S.channels == 1 && S.steps > 1 && (st == 1 || st == -1);
     for (const View* v : {&S.x, &S.gate, &S.resets, &S.before, &S.h, &S.second}) runs = runs && (!v->p || v->st == st);
     for (const View* v : {&S.x, &S.h}) runs = runs && (S.cols == 1 || v->sb != 1);
-    runs = runs && S.cols < (1 << 25);                // (a grid has fewer than 2^32 lanes)
+    runs = runs && S.cols < ((int64_t)1 << 26) - 4;   // (a grid has fewer than 2^32 lanes)
     const Deal d = runs ? deal_runs(S.steps, S.cols) : deal_columns(S.steps, S.cols);
     if (d.parts > 65535 || S.cols > ((int64_t)1 << 31)) return fail(-1, "%s: %lld steps of %lld columns are too many for one call", who, (long long)S.steps, (long long)S.cols);
     S.part = d.part;

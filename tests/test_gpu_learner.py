@@ -825,3 +825,33 @@ def test_more_sequences_than_a_grid_of_wavefronts():
     h, final = learner.gated_scan(x, 0.5, dim=1)
     assert torch.equal(h[:, 0], x[:, 0]) and torch.equal(h[:, 1], torch.addcmul(x[:, 1], x[:, 0], torch.full_like(x[:, 0], 0.5)))
     assert torch.equal(final, h[:, 1])
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f64'])
+@pytest.mark.parametrize('T', [2, 3, 7, 8, 9, 15, 16, 17, 33, 64, 65, 129, 256, 257, 300, 511, 512, 513])
+def test_short_sequences_with_time_the_fast_index(T, dtype):
+    """Several of them share a wavefront; 67 do not fill the last one."""
+    from sustaingym_amd import learner
+    kind = TYPES[dtype]
+    g = gen(50 + T)
+    N = 67
+    x = torch.randn((N, T), generator=g, device='cuda').to(kind)
+    gate = torch.rand((N, T), generator=g, device='cuda').to(kind)
+    resets = torch.rand((N, T), generator=g, device='cuda') < 0.1
+    up = torch.randn((N, T), generator=g, device='cuda').to(kind)
+    state = torch.float64 if dtype == 'f64' else torch.float32
+    initial, g_final = (torch.randn(N, generator=g, device='cuda').to(state) for _ in range(2))
+    for reverse in (False, True):
+        want = ref.scan(host(x), host(gate), host(initial), host(resets), 1, reverse, host(up), host(g_final))
+        leaves = [t.clone().requires_grad_(True) for t in (x, gate, initial)]
+        out = learner.gated_scan(*leaves, resets, 1, reverse)
+        near(out[0], *want['h'], 'h')
+        near(out[1], *want['final'], 'final')
+        for name, got in zip(('grad_x', 'grad_gate', 'grad_initial'), torch.autograd.grad(out, leaves, (up, g_final))):
+            near(got, *want[name], name)
+    if dtype != 'bf16':
+        ends, values, last = resets, torch.randn((N, T), generator=g, device='cuda'), torch.randn(N, generator=g, device='cuda')
+        a = learner.advantages(x.t(), values.t(), ends.t(), last)
+        want, tol = ref.advantages(host(x).t(), host(values).t(), host(ends).t(), host(last), 0.99, 0.95)
+        near(a.advantages, want, tol + ref.U * want.abs(), 'advantages')
+        assert a.targets.stride() == x.t().stride()
