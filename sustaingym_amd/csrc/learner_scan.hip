@@ -13,16 +13,15 @@
 // launch writes the parts' pairs to the workspace, a second one starts each part from the pairs before it (x and a are then
 // read twice, the second time mostly from the last-level cache).
 //
-// Two layouts.  COLUMNS: lanes lie along adjacent channels (or sequences, where time is the slow index), wavefronts of a
+// Three layouts.  COLUMNS: lanes lie along adjacent channels (or sequences, where time is the slow index), wavefronts of a
 // workgroup along time; pairs go through LDS.  RUNS: time is the fast index, so lanes lie along time, pairs go through a
-// wavefront scan.  State, pairs and products are float32 (float64 for float64 sequences) whatever the elements' type.
+// wavefront scan.  TILES: as COLUMNS, with 16 bytes to a lane's load.  State, pairs and products are float32 (float64 for
+// float64 sequences) whatever the elements' type.
 //
 // Bound by memory where there are columns for everybody: advantages of 288 x 65 536 move 397 MB in 83 us (4.8 TB/s of a large
-// copy's 5.1), returns of 288 x 16 384 float64 81 MB in 18; a memory of 16 x 2048 x 1024 bfloat16 201 MB in 54 forward and 336 MB
-// in 78 backward (256 workgroups, one to a compute unit: what waits at the barriers is not made up for).  131 073 x 72 float32,
-// in 256 parts: 17 + 28 us for 113 MB, 75 of them twice.  A thread to a column, as it was first, took 173, 153, 2075, 2648 and
-// 44 000 us for these.  Elements of the next turn kept in registers ahead of time cost more registers than they saved waiting
-// (55.6 and 104 us instead of 54 and 78), runs of 16 the same (48 and 96).
+// copy's 5.1), returns of 288 x 16 384 float64 81 MB in 18; a memory of 16 x 2048 x 1024 bfloat16 201 MB in 39 forward and 336 MB
+// in 70 backward.  131 073 x 72 float32, in 256 parts: 17 + 28 us for 113 MB, 75 of them twice.  A thread to a column, as it was
+// first, took 173, 153, 2075, 2648 and 44 000 us for these.
 //
 // A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.  For float32 that is the
 // multiplication in which 0 times anything is 0, one instruction instead of a comparison and a selection behind an fma.
@@ -449,6 +448,143 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
     }
 }
 
+// ---- TILES: as COLUMNS, where 64 adjacent channels are there for every wavefront ------------------------------------------
+//
+// A wavefront's run of 64 columns is L rows of 64 adjacent elements: it is loaded and stored 16 bytes to a lane, which takes an
+// eighth (float32: a quarter) of the instructions and registers, so that the next turn's elements can be on their way while this
+// one's are worked on.  What a lane needs, a column, it gets through its wavefront's own piece of LDS.  A tile lies in one
+// sequence, whose flags are the same for all its lanes: bits of a scalar.
+//
+// 16 x 2048 x 1024 bfloat16: 201 MB in 38 us forward, 336 MB in 69 backward (5.2 and 4.8 TB/s); one element to a lane at a time,
+// in the kernel above, 41 and 78, and 300 x 2 x 8192 12.1 backward instead of 17.5.
+
+template <class T> struct Tile {
+    static constexpr int N = 16 / sizeof(T), LANES = 64 / N, ROWS = N, LOADS = L / ROWS, BYTES = L * 64 * sizeof(T);
+    typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
+    uint4 v[LOADS];
+    // rows from .. of [0, hi), 0 outside
+    __device__ __forceinline__ void load(const char* base, int64_t stride, int64_t from, int64_t hi, int lane) {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) {
+            const int64_t row = from + l * ROWS + lane / LANES;
+            v[l] = uint4{0, 0, 0, 0};
+            if (row >= 0 && row < hi) v[l] = __builtin_bit_cast(uint4, (vec)*(const vec __attribute__((address_space(1)))*)((Global)base + (row * stride + lane % LANES * 16)));
+        }
+    }
+    __device__ __forceinline__ void store(char* base, int64_t stride, int64_t from, int64_t hi, int lane) const {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) {
+            const int64_t row = from + l * ROWS + lane / LANES;
+            if (row < hi) *(vec __attribute__((address_space(1)))*)((Global)base + (row * stride + lane % LANES * 16)) = __builtin_bit_cast(vec, v[l]);
+        }
+    }
+    __device__ __forceinline__ void to_rows(char* at, int lane) const {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) ((uint4*)at)[l * 64 + lane] = v[l];
+    }
+    __device__ __forceinline__ void from_rows(const char* at, int lane) {
+#pragma unroll
+        for (int l = 0; l < LOADS; l++) v[l] = ((const uint4*)at)[l * 64 + lane];
+    }
+};
+// What a wavefront's lanes wrote is there for its other lanes: LDS works in order, the compiler has to keep to it.
+__device__ __forceinline__ void rows_written() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+// A barrier for what went through LDS; loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+constexpr int kTileWaves = 8;    // (16 take 0.5 - 1 us longer to begin and gain nothing, 4 leave half the loads out: 61 us for 38)
+
+template <class O>
+__global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
+    constexpr Kind K = O::K;
+    constexpr int WT = kTileWaves;
+    using T = typename O::T;
+    using W = typename O::W;
+    constexpr int64_t TURN = WT * L;
+    constexpr bool back = K == BACKWARD, BEFORE = back && O::SECOND;
+    constexpr int FLAGS = L + (BEFORE ? 1 : 0), shift = back ? 1 : 0, BYTES = Tile<T>::BYTES;
+    __shared__ Pair<W> pairs_of[2][WT][64];
+    __shared__ __attribute__((aligned(16))) char rows_of[WT][BEFORE ? 3 : 2][BYTES];
+    const int lane = threadIdx.x & 63, wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t q0 = (int64_t)blockIdx.x * 64, b = q0 / S.channels, c0 = q0 - b * S.channels, q = q0 + lane;
+    const char *px = uniform_part<T>(S.x, b, c0), *pg = uniform_part<T>(S.gate, b, c0), *pb = uniform_part<T>(S.before, b, c0);
+    const char* pr = uniform_part<uint8_t>(S.resets, b, 0);
+    char *ph = (char*)uniform_part<T>(S.h, b, c0), *po = (char*)uniform_part<T>(S.second, b, c0);
+    const int64_t size = sizeof(T), sx = S.x.st * size, sg = S.gate.st * size, sb = S.before.st * size;
+    char *rx = rows_of[wt][0], *rg = rows_of[wt][1], *rb = rows_of[wt][BEFORE ? 2 : 0];
+    W carry = first_state<K, W>(S, q);
+    const W edge[1] = {edge_of<K, W>(S, q)};
+    Tile<T> x, g, before;
+    uint8_t flag = 0;
+    auto ask = [&](int64_t u0) {
+        x.load(px, sx, u0, S.steps, lane);
+        if constexpr (O::GATE) g.load(pg, sg, u0 - shift, S.steps, lane);
+        if constexpr (BEFORE) before.load(pb, sb, u0 + 1, S.steps, lane);
+        if constexpr (O::RESETS) {
+            const int64_t at = u0 - shift + lane;
+            flag = 0;
+            if (lane < FLAGS && at >= 0 && at < S.steps) flag = (uint8_t)pr[at * S.resets.st];
+        }
+    };
+    ask(wt * L);
+    int turn = 0;
+    for (int64_t u = 0; u < S.steps; u += TURN, turn ^= 1) {
+        const int64_t u0 = u + wt * L;
+        x.to_rows(rx, lane);
+        if constexpr (O::GATE) g.to_rows(rg, lane);
+        if constexpr (BEFORE) before.to_rows(rb, lane);
+        const uint64_t flags = O::RESETS ? __ballot(flag != 0) : 0;
+        rows_written();
+        if (u + TURN < S.steps) ask(u0 + TURN);
+        Raw<O, 1> raw;
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            raw.x[i] = ((const T*)rx)[i * 64 + lane];
+            if constexpr (O::GATE) raw.g[i] = ((const T*)rg)[i * 64 + lane];
+            if constexpr (BEFORE) raw.before[i] = ((const T*)rb)[i * 64 + lane];
+        }
+        if constexpr (O::RESETS) {
+#pragma unroll
+            for (int i = 0; i < FLAGS; i++) raw.r[i] = flags >> i & 1;
+        }
+        Run<O, 1> f;
+        fold<O, 1, false>(S, raw, edge, u0, S.steps, f);
+        const Pair<W> own = pair_of<O, 1>(f, 0);
+        pairs_of[turn][wt][lane] = own;
+        lds_barrier();
+        W h = carry;
+#pragma unroll
+        for (int w = 0; w < WT; w++) {
+            if (w == wt) h = carry;
+            const Pair<W> p = pairs_of[turn][w][lane];
+            carry = step(p.a, carry, p.h);
+        }
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            h = step(f.a[i], h, f.x[i]);
+            ((T*)rx)[i * 64 + lane] = (T)h;
+            if constexpr (O::SECOND) ((T*)rg)[i * 64 + lane] = second_of<O, 1>(f, i, h);
+        }
+        rows_written();
+        Tile<T> out;
+        out.from_rows(rx, lane);
+        out.store(ph, S.h.st * size, u0, S.steps, lane);
+        if constexpr (O::SECOND) {
+            out.from_rows(rg, lane);
+            out.store(po, S.second.st * size, u0, S.steps, lane);
+        }
+        rows_written();
+    }
+    if (wt == 0) put_final<K, T, W>(S, b, c0 + lane, q, carry);
+}
+
 // ---- RUNS: 64 runs of one column to a wavefront, WT wavefronts to a column; or, of short ones, several columns ------------
 
 // COUNT steps from `from`, 16 bytes at a time (at any alignment); DIR: whether they rise or fall in memory.  Not FULL: one by
@@ -765,6 +901,14 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
             if (even && S.cols >= 65536 && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
         } else if constexpr (sizeof(typename O::T) <= 4) {
             if (even && d.parts > 1 && S.cols > 64) return launch_columns<O, 2, kMany<O>>(S, d, stream), 0;
+        }
+        // Tiles where wavefronts stand behind one another, in one part, and all eight have steps where there are tiles enough
+        // (64 x 500 x 1024 bfloat16: 67.6 us backward instead of 76.7; x 32: 8.4 and 7.5).  Where a wavefront has all steps
+        // (256 x 300 x 1024) the memory is busy without: 104 us forward, with them 111.
+        if constexpr (O::K != ADVANTAGES && sizeof(typename O::T) <= 4) {
+            bool tiles = (d.wt == 16 || (d.wt == 4 && S.steps > kTileWaves * L)) && d.parts == 1 && S.channels % 64 == 0;
+            for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second}) tiles = tiles && (!v->p || v->sc == 1);
+            if (tiles) return tiles_kernel<O><<<(unsigned)(S.cols / 64), 64 * kTileWaves, 0, stream>>>(S), 0;
         }
         if (d.wt == 1) launch_columns<O, 1, 1>(S, d, stream);
         else if (d.wt == 4) launch_columns<O, 1, 4>(S, d, stream);

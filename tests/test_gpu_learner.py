@@ -855,3 +855,36 @@ def test_short_sequences_with_time_the_fast_index(T, dtype):
         want, tol = ref.advantages(host(x).t(), host(values).t(), host(ends).t(), host(last), 0.99, 0.95)
         near(a.advantages, want, tol + ref.U * want.abs(), 'advantages')
         assert a.targets.stride() == x.t().stride()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('shape,dim', [((33, 1, 64), 0), ((64, 3, 128), 0), ((65, 2, 192), 0), ((5, 127, 64), 1), ((2, 130, 320), 1), ((40, 130, 64), 0), ((2, 511, 64), 1),
+                                       ((700, 1, 8320), 0)])
+def test_channels_by_the_64(shape, dim, dtype):
+    """Whole tiles of channels, with and without what each form of the kernel has, also from views that are not aligned."""
+    from sustaingym_amd import learner
+    kind = TYPES[dtype]
+    g = gen(60 + shape[1])
+    wide = (*shape[:2], shape[2] + 3)
+    x, gate, up = (torch.rand(wide, generator=g, device='cuda').to(kind)[..., k:k + shape[2]] for k in (1, 2, 3))
+    resets = torch.rand(shape[:2], generator=g, device='cuda') < 0.05
+    rest = shape[:dim] + shape[dim + 1:]
+    initial, g_final = (torch.randn(rest, generator=g, device='cuda') for _ in range(2))
+    for reverse, a, r, i in ((False, gate, resets, initial), (True, gate, None, None), (False, 0.9, resets, initial), (True, -0.5, None, initial),
+                             (True, gate, resets, initial)):
+        want = ref.scan(host(x), a if isinstance(a, float) else host(a), host(i), host(r), dim, reverse, host(up), host(g_final))
+        leaves = {'grad_x': x, 'grad_gate': a, 'grad_initial': i}
+        leaves = {k: v.detach().requires_grad_(True) for k, v in leaves.items() if isinstance(v, torch.Tensor)}
+        out = learner.gated_scan(leaves['grad_x'], leaves.get('grad_gate', a), leaves.get('grad_initial'), r, dim, reverse)
+        near(out[0], *want['h'], 'h')
+        near(out[1], *want['final'], 'final')
+        for name, got in zip(leaves, torch.autograd.grad(out, list(leaves.values()), (up, g_final), retain_graph=True)):
+            near(got, *want[name], name)
+        if 'grad_gate' in leaves:                       # the gate as it is, and as a leaf of its own
+            only, = torch.autograd.grad(out, [leaves['grad_x']], (up, g_final))
+            near(only, *want['grad_x'], 'grad_x again')
+    # a gate that needs no gradient: the state in front is not read
+    leaf = x.detach().requires_grad_(True)
+    want = ref.scan(host(x), host(gate), None, host(resets), dim, False, host(up))
+    got, = torch.autograd.grad(learner.gated_scan(leaf, gate, None, resets, dim)[0], leaf, up)
+    near(got, *want['grad_x'], 'grad_x alone')
