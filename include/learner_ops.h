@@ -9,9 +9,10 @@
  * -2 no device, -4 HIP error.
  *
  * ROWS.  `rows = outer * inner` rows of `levels` logits; row (o, i) starts at o * stride_outer + i * stride_inner
- * ELEMENTS (strides are not negative), its logits are adjacent.  What lies between two rows may be read, and is not used.  mask (NULL = all allowed): bytes, non-zero = allowed, at
- * o * mask_outer + i * mask_inner + j * mask_level (mask_level 0 or 1; strides of 0 broadcast).  What a masked place
- * holds (infinities, NaN) is never used.  A logit of -inf is a masked one.  Per-row arrays are contiguous [rows].
+ * ELEMENTS (strides are not negative), its logits are adjacent.  What lies between two rows may be read, and is not
+ * used.  mask (NULL = all allowed): bytes, non-zero = allowed, at o * mask_outer + i * mask_inner + j * mask_level
+ * (mask_level 0 or 1; strides of 0 broadcast).  What a masked place holds (infinities, NaN) is never used.  A logit of
+ * -inf is a masked one.  Per-row arrays are contiguous [rows].
  *   m = max z_j, s = sum exp(z_j - m) over the allowed j
  *   logprob(l) = z_l - m - log s;   entropy = log s - sum exp(z_j - m) (z_j - m) / s
  * A row without an allowed level has nothing to decide: logprob 0, entropy 0, gradient 0, chosen level 0.
@@ -48,8 +49,8 @@ typedef struct lrn_rows {
 
 /* The level with the largest logit + noise among the allowed ones (the lowest of equals), its log probability under
  * the logits alone and the row's entropy.  noise (NULL = none): float32, row (o, i) at o * noise_outer +
- * i * noise_inner, adjacent.  With Gumbel noise the level is a sample of the row's distribution.  Noise of -inf or NaN puts a level
- * behind all others of its row. */
+ * i * noise_inner, adjacent.  With Gumbel noise the level is a sample of the row's distribution.  Noise of -inf or NaN
+ * puts a level behind all others of its row. */
 int64_t lrn_choose_workspace(const lrn_rows* rows);
 int lrn_choose(int32_t device, void* hip_stream, const lrn_rows* rows, const float* noise, int64_t noise_outer,
                int64_t noise_inner, int64_t* level_out, float* logprob_out, float* entropy_out, void* workspace,
@@ -78,11 +79,12 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
  * lrn_scan:  h_t = a_t h_{t-1} + x_t,  t = 0 .. steps-1  (reverse: from the last step to the first; "before" and "last"
  * below are meant in that order).  a_t = gate_t (the type of x, or gate_const where gate is NULL), and exactly 0 where
  * resets (bytes, (time, batch) strides, NULL = none) says that the sequence starts anew: nothing of what came before
- * enters, not even a NaN (nor does it where the gate itself is exactly 0; in float32
- * states a product with a factor of 0 is 0).  Meant for |gate| <= 1: the products of larger gates over a run of steps must stay
- * in range.  initial [batch][channels] contiguous (NULL = 0) is the state before the first step; final
- * (NULL = not wanted) receives the last one.  initial / final are float32, float64 for LRN_F64; the state is carried in
- * those types whatever the type of x and h.  h may not overlap an input.
+ * enters, not even a NaN (nor does it where the gate itself is exactly 0; in float32 states a product with a factor of 0
+ * is 0).  Meant for |gate| <= 1: the products of larger gates over a run of steps must stay in range.  A product of gates
+ * over many steps that underflows to 0 cuts as well: a NaN or an infinity may stay behind it.  initial [batch][channels]
+ * contiguous (NULL = 0) is the state before the first step; final (NULL = not wanted) receives the last one.
+ * initial / final are float32, float64 for LRN_F64; the state is carried in those types whatever the type of x and h.
+ * h may not overlap an input.
  */
 typedef struct lrn_seq {
     int64_t steps, batch, channels;

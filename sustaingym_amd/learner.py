@@ -177,7 +177,8 @@ def choose_levels(logits, noise=None, mask=None) -> LevelChoice:
 
     logits: ``[..., K]`` float32 / bfloat16 / float16.
     noise: float32, broadcastable to the logits; with Gumbel noise (``-log(-log(u))``) the level is a sample of
-        ``softmax(logits)`` over the allowed levels, without noise it is the most probable one.
+        ``softmax(logits)`` over the allowed levels, without noise it is the most probable one.  Noise of -inf or NaN puts a
+        level behind all others of its row.
     mask: bool, broadcastable to the logits, True = allowed (``mask[N, n, 1]``: stations without a car).
 
     Returns int64 levels — what ``EVChargingVectorEnv(discrete_bins=K).step`` takes — with their log probabilities and the
@@ -395,10 +396,10 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
 
     A gate of exactly 0 does what a reset does.  Steps are joined by the products of their gates, which are meant to be at most 1
     in size: larger ones are computed as well, but where their product over a run of steps leaves float32's range (float64's for
-    float64), so does the state.
+    float64), so does the state; and behind a product that has become 0, a NaN or an infinity of the state may be gone.
 
-    ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the state's own type, what a following
-    call takes as ``initial``.  Differentiable in x, gate and initial."""
+    ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the
+    state's own type, what a following call takes as ``initial``.  Differentiable in x, gate and initial."""
     _on_device('x', x)
     device, shape = x.device, x.shape
     if x.dtype not in _SEQ_TYPES:
