@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "lrn_common.h"
+#include "lrn_grid.h"
 
 namespace lrn {
 
@@ -17,7 +18,6 @@ char* error_text() {
 
 namespace {
 
-// Workgroups are numbered over two dimensions of the grid: one holds fewer than 2^32 lanes.
 __device__ __forceinline__ int64_t block_number() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
 struct Rows {
@@ -193,9 +193,9 @@ __device__ __forceinline__ void copy_run(const void* from, void* to, int bytes) 
             for (int k = at; k < bytes; k++) ((char*)to)[k] = ((const char*)from)[k];
     }
 }
-template <class T, int G, int E> __device__ __forceinline__ void stage(const Rows& R, int64_t r0, StageOf<T, G, E>& S) {
+template <class T, int G, int E> __device__ __forceinline__ void stage(const Rows& R, int64_t r0, int here, StageOf<T, G, E>& S) {
     if constexpr (kStaged<T, G, E>) {
-        const int n = (int)min((int64_t)256, R.rows - r0) * E;
+        const int n = here * E;
         if (R.dense) copy_run((const T*)R.logits + r0 * E, S.z, n * 2);
         if (R.mask && R.mask_dense) copy_run(R.mask + r0 * E, S.mask, n);
         __syncthreads();
@@ -278,9 +278,11 @@ __device__ __forceinline__ Sums group_sums(const float (&z)[E], float (&e)[E]) {
 template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_choose_kernel(Rows R, ChooseOut O) {
     const int g = threadIdx.x % G;
-    const int64_t r = block_number() * (256 / G) + threadIdx.x / G;
+    const int64_t r0 = block_number() * (256 / G), r = r0 + threadIdx.x / G;
+    const int here = rows_here(R.rows, r0, 256 / G);
+    if (!here) return;                          // a whole workgroup behind the last row, before any barrier
     __shared__ StageOf<T, G, E> S;
-    stage<T, G, E>(R, block_number() * (256 / G), S);
+    stage<T, G, E>(R, r0, here, S);
     if (r >= R.rows) return;                    // whole groups: no lane of a group leaves alone
     int64_t off, moff, noff;
     offsets(R, r, off, moff, &O, &noff);
@@ -388,9 +390,11 @@ template <int N> struct Network {
 template <class T, int G, int E>
 __global__ __launch_bounds__(256) void group_score_kernel(Rows R, ScoreOut O) {
     const int g = threadIdx.x % G;
-    const int64_t r = block_number() * (256 / G) + threadIdx.x / G;
+    const int64_t r0 = block_number() * (256 / G), r = r0 + threadIdx.x / G;
+    const int here = rows_here(R.rows, r0, 256 / G);
+    if (!here) return;
     __shared__ StageOf<T, G, E> S;
-    stage<T, G, E>(R, block_number() * (256 / G), S);
+    stage<T, G, E>(R, r0, here, S);
     if (r >= R.rows) return;
     int64_t off, moff;
     offsets(R, r, off, moff);
@@ -439,8 +443,10 @@ __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T
     __shared__ __attribute__((aligned(16))) T out[256 * E];
     const int row = threadIdx.x / G, g = threadIdx.x % G, K = R.levels;
     const int64_t r0 = block_number() * (256 / G), r = r0 + row;
+    const int here = rows_here(R.rows, r0, 256 / G);
+    if (!here) return;
     __shared__ StageOf<T, G, E> S;
-    stage<T, G, E>(R, r0, S);
+    stage<T, G, E>(R, r0, here, S);
     if (r < R.rows) {
         int64_t off, moff;
         offsets(R, r, off, moff);
@@ -465,7 +471,7 @@ __global__ __launch_bounds__(256) void group_backward_kernel(Rows R, BackIn I, T
     __syncthreads();
     constexpr int N = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-    const int n = (int)min((int64_t)(256 / G), R.rows - r0) * K;
+    const int n = here * K;
     T* to = grad + r0 * K;
     for (int e0 = threadIdx.x * N; e0 < n; e0 += 256 * N) {
         if (e0 + N <= n) *reinterpret_cast<vec*>(to + e0) = *reinterpret_cast<const vec*>(out + e0);
@@ -888,8 +894,8 @@ int checked(const lrn_rows* in, Rows* out) {
 int64_t size_of(int dtype) { return dtype == LRN_F32 ? 4 : 2; }
 int grid_of(int64_t blocks, dim3* grid) {
     if (blocks >= (int64_t)1 << 36) return fail(-1, "rows: too many for one call");
-    const int64_t x = std::min<int64_t>(blocks, 1 << 20);
-    *grid = dim3((unsigned)x, (unsigned)cdiv(blocks, x));
+    const RowGrid g = row_grid(blocks);
+    *grid = dim3((unsigned)g.x, (unsigned)g.y);
     return 0;
 }
 
