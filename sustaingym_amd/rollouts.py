@@ -197,6 +197,10 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
         raise ValueError(f'steps: at least 1, got {steps}')
     rows: dict[str, list] = {key: [] for key in ('levels', 'logprobs', 'entropy', 'mask', 'rewards', 'values', 'ends')}
     seen: list[dict] = []
+
+    def kept(values):                                # (a policy may answer in the same tensor every time)
+        return values.to(torch.float32, copy=True)
+
     with torch.no_grad():
         if obs is None:
             obs, _ = venv.reset()
@@ -207,12 +211,12 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
                 generator=generator).clamp_(min=1e-30).log_().neg_()         # Gumbel
             choice = learner.choose_levels(logits, noise, mask)
             obs, rewards, ends, _, _ = venv.step(choice.levels)
-            for key, val in (*zip(('levels', 'logprobs', 'entropy'), choice), ('values', values.float()), ('rewards', rewards.clone()),
+            for key, val in (*zip(('levels', 'logprobs', 'entropy'), choice), ('values', kept(values)), ('rewards', rewards.clone()),
                              ('ends', ends.clone())):
                 rows[key].append(val)
             if mask is not None:
                 rows['mask'].append(mask.expand((*logits.shape[:-1], mask.shape[-1])).clone())
-        last_values = _ask(policy, obs)[1].float()
+        last_values = kept(_ask(policy, obs)[1])
         out = {key: torch.stack(val) if val else None for key, val in rows.items()}
         adv = learner.advantages(out['rewards'], out['values'], out['ends'], last_values, gamma, lam)
         return Trajectory(obs={key: torch.stack([o[key] for o in seen]) for key in seen[0]}, last_values=last_values,
