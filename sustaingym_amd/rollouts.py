@@ -184,7 +184,8 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
 
     venv: ``EVChargingVectorEnv(..., output='torch', discrete_bins=K)``; episodes begin anew by themselves.
     policy: ``policy(obs) -> (logits [N, n, K], values [N])`` or ``(logits, values, mask)``; mask: bool, broadcastable to the
-        logits, True = allowed (a station that it leaves nothing gets level 0).
+        logits, True = allowed (a station that it leaves nothing gets level 0).  K is the environments' ``discrete_bins``; other
+        shapes raise ``ValueError`` before a step is taken on them.
     obs: the observation to begin with; None resets the environments.
     greedy: the most probable level instead of a sampled one (``generator``: the torch generator of the samples).
 
@@ -197,6 +198,7 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
         raise ValueError(f'steps: at least 1, got {steps}')
     rows: dict[str, list] = {key: [] for key in ('levels', 'logprobs', 'entropy', 'mask', 'rewards', 'values', 'ends')}
     seen: list[dict] = []
+    rows_of = (venv.num_envs, venv.num_stations, venv.discrete_bins)
 
     def kept(values):                                # (a policy may answer in the same tensor every time)
         return values.to(torch.float32, copy=True)
@@ -207,6 +209,10 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
         for _ in range(steps):
             seen.append({key: val.clone() for key, val in obs.items()})      # (the environments overwrite theirs)
             logits, values, mask = _ask(policy, seen[-1])
+            if tuple(logits.shape) != rows_of:
+                raise ValueError(f'logits: {tuple(logits.shape)}, the environments take {rows_of} (environments, stations, discrete_bins)')
+            if tuple(values.shape) != rows_of[:1]:
+                raise ValueError(f'values: {tuple(values.shape)} instead of {rows_of[:1]}')
             noise = None if greedy else torch.empty(logits.shape, dtype=torch.float32, device=logits.device).exponential_(
                 generator=generator).clamp_(min=1e-30).log_().neg_()         # Gumbel
             choice = learner.choose_levels(logits, noise, mask)
@@ -217,6 +223,8 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
             if mask is not None:
                 rows['mask'].append(mask.expand((*logits.shape[:-1], mask.shape[-1])).clone())
         last_values = kept(_ask(policy, obs)[1])
+        if tuple(last_values.shape) != rows_of[:1]:
+            raise ValueError(f'values: {tuple(last_values.shape)} instead of {rows_of[:1]}')
         out = {key: torch.stack(val) if val else None for key, val in rows.items()}
         adv = learner.advantages(out['rewards'], out['values'], out['ends'], last_values, gamma, lam)
         return Trajectory(obs={key: torch.stack([o[key] for o in seen]) for key in seen[0]}, last_values=last_values,

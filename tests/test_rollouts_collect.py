@@ -58,3 +58,12 @@ def test_a_policy_may_answer_in_the_same_tensors_every_time(plain):
     assert torch.allclose(traj.advantages.double(), want, rtol=1e-6)
     values.fill_(77.0)                                        # what the policy does later changes nothing that was returned
     assert traj.last_values.tolist() == [4.0] * N and float(obs['demands'][0, 0]) == 4.0
+
+
+@pytest.mark.parametrize('logits,values,match', [((N, STATIONS, K + 1), (N,), 'logits'), ((N, STATIONS, K - 1), (N,), 'logits'), ((N, STATIONS + 1, K), (N,), 'logits'),
+                                                 ((N * STATIONS, K), (N,), 'logits'), ((N, STATIONS, K), (N, 1), 'values'), ((N, STATIONS, K), (), 'values')])
+def test_answers_of_other_shapes_are_refused_before_a_step(plain, logits, values, match):
+    venv = Environments()
+    with pytest.raises(ValueError, match=match):
+        rollouts.collect(venv, lambda obs: (torch.zeros(logits), torch.zeros(values)), 3)
+    assert venv.steps == 0
