@@ -184,8 +184,8 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
 
     venv: ``EVChargingVectorEnv(..., output='torch', discrete_bins=K)``; episodes begin anew by themselves.
     policy: ``policy(obs) -> (logits [N, n, K], values [N])`` or ``(logits, values, mask)``; mask: bool, broadcastable to the
-        logits, True = allowed (a station that it leaves nothing gets level 0).  K is the environments' ``discrete_bins``; other
-        shapes raise ``ValueError`` before a step is taken on them.
+        logits, True = allowed (a station that it leaves nothing gets level 0), given at every step or at none.  K is the
+        environments' ``discrete_bins``; answers of other shapes raise ``ValueError`` before a step is taken on them.
     obs: the observation to begin with; None resets the environments.
     greedy: the most probable level instead of a sampled one (``generator``: the torch generator of the samples).
 
@@ -198,6 +198,7 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
         raise ValueError(f'steps: at least 1, got {steps}')
     rows: dict[str, list] = {key: [] for key in ('levels', 'logprobs', 'entropy', 'mask', 'rewards', 'values', 'ends')}
     seen: list[dict] = []
+    allowed = None
     rows_of = (venv.num_envs, venv.num_stations, venv.discrete_bins)
 
     def kept(values):                                # (a policy may answer in the same tensor every time)
@@ -213,6 +214,10 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
                 raise ValueError(f'logits: {tuple(logits.shape)}, the environments take {rows_of} (environments, stations, discrete_bins)')
             if tuple(values.shape) != rows_of[:1]:
                 raise ValueError(f'values: {tuple(values.shape)} instead of {rows_of[:1]}')
+            kind = None if mask is None else mask.shape[-1] if mask.dim() else 1
+            if len(seen) > 1 and kind != allowed:
+                raise ValueError('mask: given at every step, with the same last dimension, or at none')
+            allowed = kind
             noise = None if greedy else torch.empty(logits.shape, dtype=torch.float32, device=logits.device).exponential_(
                 generator=generator).clamp_(min=1e-30).log_().neg_()         # Gumbel
             choice = learner.choose_levels(logits, noise, mask)
@@ -221,7 +226,7 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
                              ('ends', ends.clone())):
                 rows[key].append(val)
             if mask is not None:
-                rows['mask'].append(mask.expand((*logits.shape[:-1], mask.shape[-1])).clone())
+                rows['mask'].append(mask.expand((*rows_of[:2], kind)).clone())
         last_values = kept(_ask(policy, obs)[1])
         if tuple(last_values.shape) != rows_of[:1]:
             raise ValueError(f'values: {tuple(last_values.shape)} instead of {rows_of[:1]}')

@@ -67,3 +67,22 @@ def test_answers_of_other_shapes_are_refused_before_a_step(plain, logits, values
     with pytest.raises(ValueError, match=match):
         rollouts.collect(venv, lambda obs: (torch.zeros(logits), torch.zeros(values)), 3)
     assert venv.steps == 0
+
+
+@pytest.mark.parametrize('masks', [(None, 1), (1, None), (1, K), (K, 1)])
+def test_masks_that_come_and_go_are_refused(plain, masks):
+    """Stacked, they would be those of other steps."""
+    def policy(obs):
+        last = masks[int(obs['demands'][0, 0]) % 2]
+        answer = torch.zeros(N, STATIONS, K), torch.zeros(N)
+        return answer if last is None else (*answer, torch.ones((N, STATIONS, last), dtype=torch.bool))
+    venv = Environments()
+    with pytest.raises(ValueError, match='mask'):
+        rollouts.collect(venv, policy, 4)
+    assert venv.steps == 1
+
+
+@pytest.mark.parametrize('shape', [(), (1,), (K,), (STATIONS, 1), (N, STATIONS, K)])
+def test_masks_of_any_shape_that_broadcasts_are_kept(plain, shape):
+    traj, _ = rollouts.collect(Environments(), lambda obs: (torch.zeros(N, STATIONS, K), torch.zeros(N), torch.ones(shape, dtype=torch.bool)), 2)
+    assert traj.mask.shape == (2, N, STATIONS, shape[-1] if shape else 1) and bool(traj.mask.all())
