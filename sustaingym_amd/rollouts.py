@@ -189,7 +189,8 @@ def collect(venv, policy, steps: int, obs=None, gamma: float = 0.99, lam: float 
     obs: the observation to begin with; None resets the environments.
     greedy: the most probable level instead of a sampled one (``generator``: the torch generator of the samples).
 
-    Nothing is synchronised: the steps are enqueued on the current stream, and no gradient is recorded."""
+    The steps are enqueued on the current stream and no gradient is recorded.  The host waits for the GPU where the environments do:
+    ``reset`` and a step that ends the episodes fetch the ``max_profit`` of episodes that were generated on the GPU."""
     import torch
     from . import learner
     if getattr(venv, 'output', None) != 'torch' or not venv.discrete_bins > 0:
