@@ -11,7 +11,8 @@ a batch of N environments with n stations and K levels is ``logits[N, n, K]``.
 
 Every call runs on the current torch stream of its tensors' device, does not synchronise, and may be captured into a graph.
 Tensors of any strides are taken as they are where the last dimension of logits and noise is dense; anything else is copied
-first.  Wrong arguments raise ``ValueError`` before anything is launched.  There is no CPU form: CPU tensors are refused.
+first.  Wrong arguments raise ``ValueError`` before anything is launched.  There is no CPU form: CPU tensors are refused.  Gradients are
+those of a backward pass, once: second derivatives raise, forward-mode tangents are refused.
 
 To capture a backward pass into a graph, run the forward pass inside the same capture and ask for the gradients there with
 ``torch.autograd.grad``, for leaves that no eager graph holds at that time (a tensor's ``detach().requires_grad_()`` taken inside
@@ -24,6 +25,7 @@ import ctypes as C
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -65,6 +67,14 @@ def _on_device(name: str, t, device=None) -> None:
     if not t.is_cuda:
         raise ValueError(f'{name}: a CUDA tensor is needed (there is no CPU form)')
     raise ValueError(f'{name}: on {t.device}, the first argument is on {device}')
+
+
+def _no_tangents(**inputs) -> None:
+    """A dual tensor does not require a gradient: its tangent would be dropped without a word."""
+    if forward_ad._current_level >= 0:
+        for name, t in inputs.items():
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f'{name}: there is no forward-mode derivative')
 
 
 def _broadcasts(t, shape) -> bool:
@@ -272,6 +282,7 @@ def level_logprobs(logits, levels, mask=None, top: int = 0) -> LevelScores:
 
     Log probabilities, entropies and all sums are float32 whatever the logits' type; the gradient has the logits' type."""
     _check_rows(logits, mask)
+    _no_tangents(logits=logits)
     _on_device('levels', levels, logits.device)
     if levels.shape != logits.shape[:-1]:
         raise ValueError(f'levels: {tuple(levels.shape)}, the logits have rows {tuple(logits.shape[:-1])}')
@@ -436,6 +447,7 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
         if resets.shape != shape[:2]:
             raise ValueError(f'resets: {tuple(resets.shape)} instead of {tuple(shape[:2])}')
     reverse = bool(reverse)
+    _no_tangents(x=x, gate=gate, initial=initial)
     if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad)
                                     or (initial is not None and initial.requires_grad)):
         return _GatedScan.apply(x, gate, initial, resets, const, dim, reverse)
