@@ -60,10 +60,12 @@ def _check(rc: int, what: str) -> None:
 
 
 def _on_device(name: str, t, device=None) -> None:
-    if isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device):
+    if isinstance(t, torch.Tensor) and t.is_cuda and (device is None or t.device == device) and not t.is_neg():
         return
     if not isinstance(t, torch.Tensor):
         raise ValueError(f'{name}: a tensor is needed, not {type(t).__name__}')
+    if t.is_neg():
+        raise ValueError(f'{name}: its memory holds the negated values (the imaginary part of a conjugate view): resolve_neg() it first')
     if not t.is_cuda:
         raise ValueError(f'{name}: a CUDA tensor is needed (there is no CPU form)')
     raise ValueError(f'{name}: on {t.device}, the first argument is on {device}')
