@@ -79,9 +79,10 @@ int lrn_score_backward(int32_t device, void* hip_stream, const lrn_rows* rows, c
  * lrn_scan:  h_t = a_t h_{t-1} + x_t,  t = 0 .. steps-1  (reverse: from the last step to the first; "before" and "last"
  * below are meant in that order).  a_t = gate_t (the type of x, or gate_const where gate is NULL), and exactly 0 where
  * resets (bytes, (time, batch) strides, NULL = none) says that the sequence starts anew: nothing of what came before
- * enters, not even a NaN (nor does it where the gate itself is exactly 0; in float32 states a product with a factor of 0
- * is 0).  Meant for |gate| <= 1: the products of larger gates over a run of steps must stay in range.  A product of gates
- * over many steps that underflows to 0 cuts as well: a NaN or an infinity may stay behind it.  initial [batch][channels]
+ * enters, not even a NaN (nor does it where the gate itself is exactly 0).  A gate that is not finite, where no reset
+ * stands, makes the state NaN whatever it was.  Meant for |gate| <= 1: the products of larger gates over a run of steps must
+ * stay in range.  A product of gates over many steps that underflows to 0 cuts as well: a NaN or an infinity of the state may
+ * stay behind it.  initial [batch][channels]
  * contiguous (NULL = 0) is the state before the first step; final (NULL = not wanted) receives the last one.
  * initial / final are float32, float64 for LRN_F64; the state is carried in those types whatever the type of x and h.
  * h may not overlap an input.

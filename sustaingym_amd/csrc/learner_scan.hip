@@ -24,7 +24,8 @@
 // first, took 173, 153, 2075, 2648 and 44 000 us for these.
 //
 // A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.  For float32 that is the
-// multiplication in which 0 times anything is 0, one instruction instead of a comparison and a selection behind an fma.
+// multiplication in which 0 times anything is 0, one instruction instead of a comparison and a selection behind an fma.  That
+// would also hide a gate that is not finite from a state of 0, so such a gate makes its own step's x NaN (`seen`).
 #include <algorithm>
 #include <initializer_list>
 #include <type_traits>
@@ -63,6 +64,9 @@ template <> struct State<double> { using type = double; };
 extern "C" __device__ float product_with_zero(float, float) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float times(float a, float b) { return product_with_zero(a, b); }
 __device__ __forceinline__ double times(double a, double b) { return a == 0.0 ? 0.0 : a * b; }
+// x, or NaN beside a coefficient that is not finite
+__device__ __forceinline__ float seen(float a, float x) { return __builtin_fmaf(a, 0.0f, x); }
+__device__ __forceinline__ double seen(double a, double x) { return __builtin_fma(a, 0.0, x); }
 __device__ __forceinline__ float step(float a, float h, float x) { return times(a, h) + x; }
 __device__ __forceinline__ double step(double a, double h, double x) { return a == 0.0 ? x : __builtin_fma(a, h, x); }
 
@@ -231,7 +235,7 @@ __device__ __forceinline__ void fold(const Seq& S, const Raw<O, V>& d, const typ
                 }
             }
             f.a[n] = in ? a : W(1);
-            f.x[n] = in ? x : W(0);
+            f.x[n] = in ? seen(a, x) : W(0);
         }
     }
 }
@@ -329,7 +333,8 @@ template <Kind K, class T, class W> __device__ __forceinline__ void put_final(co
         const bool cut = S.resets.p && ((const uint8_t*)S.resets.p)[(S.steps - 1) * S.resets.st + b * S.resets.sb];
         W own = (W)S.gate_const;
         if (S.gate.p) own = (W)((const T*)S.gate.p)[(S.steps - 1) * S.gate.st + b * S.gate.sb + c * S.gate.sc];
-        h = step(cut ? W(0) : own, h, W(0));
+        if (cut) own = W(0);
+        h = step(own, h, seen(own, W(0)));
     }
     ((W*)S.final)[q] = h;
 }

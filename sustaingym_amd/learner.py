@@ -407,9 +407,10 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
         not even a NaN.  Forward, that is the step AFTER an episode's end; with ``reverse`` the step of the end itself.
     reverse: from the last step to the first (``h_t = gate_t * h_{t+1} + x_t``).
 
-    A gate of exactly 0 does what a reset does.  Steps are joined by the products of their gates, which are meant to be at most 1
-    in size: larger ones are computed as well, but where their product over a run of steps leaves float32's range (float64's for
-    float64), so does the state; and behind a product that has become 0, a NaN or an infinity of the state may be gone.
+    A gate of exactly 0 does what a reset does; a NaN or infinite gate makes the state NaN, also a state of 0.  Steps are joined by
+    the products of their gates, which are meant to be at most 1 in size: larger ones are computed as well, but where their product
+    over a run of steps leaves float32's range (float64's for float64), so does the state; and behind a product that has become 0, a
+    NaN or an infinity of the state may be gone.
 
     ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the
     state's own type, what a following call takes as ``initial``.  Differentiable in x, gate and initial."""
