@@ -107,7 +107,8 @@ template <class O, int V>
 struct Run {
     using W = typename O::W;
     W a[L * V], x[L * V];
-    std::conditional_t<O::K == ADVANTAGES, float, W> extra[O::SECOND ? L * V : 1];    // BACKWARD: d h / d gate; ADVANTAGES: V
+    std::conditional_t<O::K == ADVANTAGES, float, W> extra[O::SECOND ? L * V : 1];    // BACKWARD: the state before; ADVANTAGES: V
+    uint32_t anew = 0;                                     // BACKWARD: bits of the steps that have a reset
 };
 
 // A lane's V columns in every view: the part of the address that is the same for the wavefront, and the lane's own.
@@ -230,7 +231,7 @@ __device__ __forceinline__ void fold(const Seq& S, const Raw<O, V>& d, const typ
                 if constexpr (O::SECOND) {
                     W prev = (W)d.before[n];
                     if (FULL ? i == L - 1 && final_step < L : i == final_step) prev = edge[k];
-                    if constexpr (O::RESETS) prev = d.r[n + V] ? W(0) : prev;
+                    if constexpr (O::RESETS) f.anew |= (d.r[n + V] != 0 ? 1u : 0u) << n;
                     f.extra[n] = prev;
                 }
             }
@@ -257,7 +258,7 @@ template <class O, int V> __device__ __forceinline__ Pair<typename O::W> pair_of
 // The second output of a step from the state behind it.
 template <class O, int V> __device__ __forceinline__ typename O::Out second_of(const Run<O, V>& f, int n, typename O::W h) {
     using W = typename O::W;
-    if constexpr (O::K == BACKWARD) return (typename O::Out)(h * f.extra[n]);
+    if constexpr (O::K == BACKWARD) return (typename O::Out)(O::RESETS && (f.anew >> n & 1) ? W(0) : h * f.extra[n]);
     else return (typename O::Out)(h + (W)f.extra[n]);
 }
 

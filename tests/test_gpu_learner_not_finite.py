@@ -69,3 +69,26 @@ def test_gradients_behind_a_gate_that_is_not_finite(shape, dim):
         gx, gi = torch.autograd.grad(h, (x, init), torch.zeros(shape, device='cuda'))
         gx = host(gx)
         assert torch.isnan(gx[step(slice(0, at))]).all() and not gx[step(slice(at, None))].any() and torch.isnan(host(gi)).all()
+
+
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f64'])
+@pytest.mark.parametrize('shape,dim,at', [f for f in FORMS if f[0][f[1]] > 1], ids=['x'.join(map(str, f[0])) for f in FORMS if f[0][f[1]] > 1])
+def test_the_gate_of_a_reset_has_no_gradient_whatever_comes_in(shape, dim, at, dtype):
+    """grad_gate is 0 at a reset, also where the gradient of the step, or the state before it, is NaN or infinite."""
+    from sustaingym_amd import learner
+    kind = TYPES[dtype]
+
+    def step(t):
+        return (slice(None),) * dim + (t,)
+    for reverse in (False, True):
+        before = at - 1 if not reverse else at + 1
+        resets = torch.zeros(shape[:2], dtype=torch.bool, device='cuda')
+        resets[step(at)] = True
+        x = torch.ones(shape, dtype=kind, device='cuda')
+        x[step(before)] = math.nan
+        gate = torch.full(shape, 0.5, dtype=kind, device='cuda').requires_grad_(True)
+        up = torch.zeros(shape, dtype=kind, device='cuda')
+        for bad in (math.nan, math.inf, 0.0):
+            up[step(at)] = bad
+            gg, = torch.autograd.grad(learner.gated_scan(x, gate, None, resets, dim, reverse)[0], gate, up)
+            assert not host(gg)[step(at)].any(), (bad, reverse)
