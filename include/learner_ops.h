@@ -103,11 +103,26 @@ int lrn_scan(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_vie
              void* workspace, int64_t workspace_bytes);
 /* Gradients: G_t = g_h_t + a_{t+1} G_{t+1} with g_final behind the last step;  grad_x = G, grad_gate_t = G_t h_{t-1}
  * (0 at a reset), grad_initial = a_0 G_0.  g_final NULL = zero; grad_gate (wanted only with a gate tensor; then h is read) and
- * grad_initial may be NULL.  h and g_final are not read where they are not needed. */
+ * grad_initial may be NULL.  h and g_final are not read where they are not needed.  grad_gate of LRN_BF16 / LRN_F16 is refused:
+ * their h is rounded, lrn_scan_keep_backward has it. */
 int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const,
                       const lrn_view* resets, const void* initial, const lrn_view* h, const lrn_view* g_h,
                       const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
                       void* grad_initial_out, void* workspace, int64_t workspace_bytes);
+
+/* The two for LRN_BF16 / LRN_F16 with a gate's gradient, whose states are not to be rounded.  lrn_scan_keep is lrn_scan that also
+ * writes every LRN_KEEP-th state as it is: kept, float32 with strides (element, batch, channel) that are not negative, has
+ * (steps + LRN_KEEP - 1) / LRN_KEEP elements a column, of which the j-th holds the state before the step that has
+ * (j + 1) * LRN_KEEP - 1 behind it (the last element, the first step's or none's, need not be written and is not read).
+ * lrn_scan_keep_backward walks the states in between again from x. */
+#define LRN_KEEP 8
+int lrn_scan_keep(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
+                  const lrn_view* resets, const void* initial, const lrn_view* h_out, const lrn_view* kept_out, void* final_out,
+                  void* workspace, int64_t workspace_bytes);
+int lrn_scan_keep_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
+                           const lrn_view* resets, const void* initial, const lrn_view* kept, const lrn_view* g_h,
+                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
+                           void* grad_initial_out, void* workspace, int64_t workspace_bytes);
 
 /* Generalised advantages of `steps` x `batch` (channels = 1, reverse ignored):
  *   d_t = r_t + gamma (1 - end_t) V_{t+1} - V_t,  A_t = d_t + gamma lam (1 - end_t) A_{t+1},  target_t = A_t + V_t

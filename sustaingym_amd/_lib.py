@@ -148,7 +148,7 @@ class LearnerView(C.Structure):
     _fields_ = [('data', C.c_void_p), ('st', C.c_int64), ('sb', C.c_int64), ('sc', C.c_int64)]
 
 
-LEARNER_MAX_TOP, LEARNER_SHORT_ROW = 64, 1024
+LEARNER_MAX_TOP, LEARNER_SHORT_ROW, LEARNER_KEEP = 64, 1024, 8
 
 # Every symbol include/learner_ops.h declares
 _i64, _rows, _seq, _view = C.c_int64, C.POINTER(LearnerRows), C.POINTER(LearnerSeq), C.POINTER(LearnerView)
@@ -162,6 +162,8 @@ LEARNER_SIGNATURES = {
     'lrn_scan_workspace': (_i64, [_seq]),
     'lrn_scan': (_i32, [_i32, _vp, _seq, _view, _view, C.c_double, _view, _vp, _view, _vp, _vp, _i64]),
     'lrn_scan_backward': (_i32, [_i32, _vp, _seq, _view, C.c_double, _view, _vp, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
+    'lrn_scan_keep': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
+    'lrn_scan_keep_backward': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
     'lrn_advantages_workspace': (_i64, [_seq]),
     'lrn_advantages': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, C.c_double, C.c_double, _view, _view, _vp, _i64]),
 }

@@ -6,6 +6,11 @@
 //              that g_final enters as the state), and beside h = grad_x comes grad_gate = h * (the state before the step)
 //   advantages u runs against time: x_u = d_t, a_u = gamma lam (1 - end_t), and beside h comes h + V_t
 //
+// The state before a step is h itself for float32 and float64.  For 16-bit sequences h is rounded, and a gate's gradient made of it
+// is off by half a step more than its own rounding; so the forward pass keeps every eighth state as it is (float32, half a byte an
+// element), at the places where the backward pass' runs end, and the backward pass walks the seven in between again from x and the
+// gates: the traffic of reading h.
+//
 // A run of steps acts on the state in front of it as h -> A h + H, and two runs in a row as (A2 A1, A2 H1 + H2).  So the steps
 // are dealt out in runs of L to lanes that hold them in registers: each computes its (A, H) from a state of 0, the states in
 // front of the runs come from the pairs of the runs before, and each lane walks its run again with the right state and writes.
@@ -46,6 +51,7 @@ struct Seq {
     int64_t channels;
     View x, gate, resets, before, h, second;
     double gate_const, scale;   // advantages: gamma lam, gamma
+    View keep;                  // 16-bit SCAN with a gradient to come, its BACKWARD: every L-th state, [runs of BACKWARD][cols]
     const void* initial;
     const void* edge;           // backward: the initial state; advantages: V behind the last step (float32)
     void* final;
@@ -78,14 +84,15 @@ template <class W> struct Pair {
     __device__ __forceinline__ void after(const Pair& first) { h = step(a, first.h, h); a = times(a, first.a); }
 };
 
-constexpr int L = 8;             // steps of a lane's run
+constexpr int L = LRN_KEEP;      // steps of a lane's run: 8
 
 // One of the three, for one type of elements: whether there is a gate tensor (else a constant), whether there are resets, and
-// whether the second output is wanted.  Compiled in: a condition between loads keeps them from being in flight together.
+// whether the second output (SCAN: the kept states) is wanted.  Compiled in: a condition between loads keeps them from being in flight together.
 template <Kind K_, class T_, bool GATE_, bool RESETS_, bool SECOND_>
 struct Op {
     static constexpr Kind K = K_;
-    static constexpr bool GATE = GATE_, RESETS = RESETS_, SECOND = SECOND_;
+    static constexpr bool GATE = GATE_, RESETS = RESETS_, SECOND = SECOND_ && K_ != SCAN;
+    static constexpr bool KEEP = SECOND_ && K_ == SCAN, AGAIN = SECOND_ && K_ == BACKWARD && sizeof(T_) == 2;    // writes S.keep; walks from it
     using T = T_;
     using W = typename State<T_>::type;
     using Out = std::conditional_t<K_ == ADVANTAGES, float, T_>;
@@ -95,10 +102,12 @@ struct Op {
 template <class O, int V>
 struct Raw {
     using T = typename O::T;
+    using W = typename O::W;
     static constexpr int N = L * V;
     T x[N];
-    T g[O::GATE ? N : 1];                                  // SCAN: gate of the step; BACKWARD: of the step before in this order
-    T before[O::K == BACKWARD && O::SECOND ? N : 1];       // the state before the step
+    T g[O::GATE ? N + (O::AGAIN ? V : 0) : 1];             // SCAN: gate of the step; BACKWARD: of the step before in this order
+    T before[O::K == BACKWARD && O::SECOND ? N : 1];       // the state before the step; AGAIN: the x that came with it
+    W kept[O::AGAIN ? V : 1];                              // the state before the run's last step, the first of the forward walk
     float v[O::K == ADVANTAGES ? N + V : 1];               // values of the steps u0 - 1 .. u0 + L - 1
     uint8_t r[O::RESETS ? N + V : 1];                      // flags of the steps u0 .., BACKWARD: u0 - 1 ..
 };
@@ -114,8 +123,8 @@ struct Run {
 // A lane's V columns in every view: the part of the address that is the same for the wavefront, and the lane's own.
 struct Place {
     const char *x, *gate, *before, *resets;
-    char *h, *second;
-    uint32_t ox, og, ob, orr, oh, oo;          // bytes
+    char *h, *second, *keep;
+    uint32_t ox, og, ob, orr, oh, oo, ok;      // bytes
     uint32_t next_flags;                       // from the first column's flags to the second's
 };
 
@@ -188,7 +197,7 @@ __device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t u0, i
     constexpr int shift = O::K == BACKWARD ? 1 : 0;
     constexpr bool back = O::K == BACKWARD;
     get_steps<T, V, L, FULL>(P.x, S.x.st, P.ox, u0, end, d.x);
-    if constexpr (O::GATE) get_steps<T, V, L, FULL, back>(P.gate, S.gate.st, P.og, u0 - shift, end, d.g);
+    if constexpr (O::GATE) get_steps<T, V, L + (O::AGAIN && APPLYING ? 1 : 0), FULL, back>(P.gate, S.gate.st, P.og, u0 - shift, end, d.g);
     if constexpr (O::RESETS) {
         constexpr int COUNT = L + (O::K == BACKWARD && O::SECOND ? 1 : 0);
         if constexpr (V == 1) get_steps<uint8_t, 1, COUNT, FULL, back>(P.resets, S.resets.st, P.orr, u0 - shift, end, d.r);
@@ -202,7 +211,11 @@ __device__ __forceinline__ void load(const Seq& S, const Place& P, int64_t u0, i
         }
     }
     if constexpr (O::K == ADVANTAGES) get_steps<float, V, L + 1, FULL, true>(P.before, S.before.st, P.ob, u0 - 1, end, d.v);
-    if constexpr (O::K == BACKWARD && O::SECOND && APPLYING) get_steps<T, V, L, FULL, false, true>(P.before, S.before.st, P.ob, u0 + 1, S.steps, d.before);
+    if constexpr (O::AGAIN && APPLYING) {
+        using W = typename O::W;
+        get_steps<T, V, L, FULL>(P.before, S.before.st, P.ob, u0, end, d.before);
+        if (u0 + L < S.steps) get<W, V>((Global)(P.keep + u0 / L * S.keep.st * (int64_t)sizeof(W)), kept_apart(P.ok), d.kept);
+    } else if constexpr (O::K == BACKWARD && O::SECOND && APPLYING) get_steps<T, V, L, FULL, false, true>(P.before, S.before.st, P.ob, u0 + 1, S.steps, d.before);
 }
 
 // What the steps do.  Behind the end: a = 1, x = 0, so that a run that is cut short has the pair of what it holds.
@@ -228,15 +241,29 @@ __device__ __forceinline__ void fold(const Seq& S, const Raw<O, V>& d, const typ
             if (cut) a = W(0);
             if constexpr (O::K == BACKWARD) {
                 if (i == 0 && u0 == 0) a = W(1);                        // g_final enters as it is
-                if constexpr (O::SECOND) {
+                if constexpr (O::SECOND && O::RESETS) f.anew |= (d.r[n + V] != 0 ? 1u : 0u) << n;
+                if constexpr (O::SECOND && !O::AGAIN) {
                     W prev = (W)d.before[n];
                     if (FULL ? i == L - 1 && final_step < L : i == final_step) prev = edge[k];
-                    if constexpr (O::RESETS) f.anew |= (d.r[n + V] != 0 ? 1u : 0u) << n;
                     f.extra[n] = prev;
                 }
             }
             f.a[n] = in ? a : W(1);
             f.x[n] = in ? seen(a, x) : W(0);
+        }
+    }
+    if constexpr (O::AGAIN) {
+        // the forward walk's steps, from the state in front of them (a run that is cut short has the sequence's first steps)
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            W h = u0 + L < S.steps ? d.kept[k] : edge[k];
+#pragma unroll
+            for (int i = L - 1; i >= 0; i--) {
+                const int n = i * V + k;
+                f.extra[n] = h;
+                const W a = O::RESETS && (f.anew >> n & 1) ? W(0) : (W)d.g[n + V], next = step(a, h, seen(a, (W)d.before[n]));
+                h = FULL || i < count ? next : h;
+            }
         }
     }
 }
@@ -262,6 +289,9 @@ template <class O, int V> __device__ __forceinline__ typename O::Out second_of(c
     else return (typename O::Out)(h + (W)f.extra[n]);
 }
 
+// Where the state before step `at` of SCAN is kept: BACKWARD's runs are counted from the last step.
+template <class O> __device__ __forceinline__ int64_t keep_offset(const Seq& S, int64_t at) { return ((S.steps - at) / L - 1) * S.keep.st * (int64_t)sizeof(typename O::W); }
+
 // Walks the run from the state in front of it and writes.
 template <class O, int V, bool FULL>
 __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, V>& f, int64_t u0, int64_t end, typename O::W (&h)[V]) {
@@ -269,11 +299,14 @@ __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, 
     Global ph = (Global)(P.h + u0 * S.h.st * (int64_t)sizeof(E)), po = (Global)(P.second + u0 * S.second.st * (int64_t)sizeof(E));
     const int last = FULL ? L : in_front(u0, end, L);
     const uint32_t oh = kept_apart(P.oh), oo = O::SECOND ? kept_apart(P.oo) : 0;
+    const int keep = (int)(S.steps % L);                   // of every run, the step that begins one of BACKWARD's
+    typename O::W kept[V];
 #pragma unroll
     for (int i = 0; i < L; i++) {
         E out[V], second[V];
 #pragma unroll
         for (int k = 0; k < V; k++) {
+            if (O::KEEP && i == keep) kept[k] = h[k];
             h[k] = step(f.a[i * V + k], h[k], f.x[i * V + k]);
             out[k] = (E)h[k];
             if constexpr (O::SECOND) second[k] = second_of<O, V>(f, i * V + k, h[k]);
@@ -284,6 +317,9 @@ __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, 
         }
         advance(ph, S.h.st * (int64_t)sizeof(E));
         if constexpr (O::SECOND) advance(po, S.second.st * (int64_t)sizeof(E));
+    }
+    if constexpr (O::KEEP) {
+        if (u0 < end && u0 + keep < S.steps) put<typename O::W, V>((Global)(P.keep + keep_offset<O>(S, u0 + keep)), kept_apart(P.ok), kept);
     }
 }
 
@@ -301,6 +337,7 @@ template <class O> __device__ __forceinline__ Place place_of(const Seq& S, int64
     P.resets = uniform_part<uint8_t>(S.resets, b0, 0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
     P.h = (char*)uniform_part<E>(S.h, b0, c0); P.oh = lane_part<E>(S.h, b - b0, c - c0);
     P.second = (char*)uniform_part<E>(S.second, b0, c0); P.oo = lane_part<E>(S.second, b - b0, c - c0);
+    P.keep = (char*)uniform_part<typename O::W>(S.keep, b0, c0); P.ok = lane_part<typename O::W>(S.keep, b - b0, c - c0);
     P.next_flags = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
     return P;
 }
@@ -523,17 +560,23 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
     const int64_t q0 = (int64_t)blockIdx.x * 64, b = q0 / S.channels, c0 = q0 - b * S.channels, q = q0 + lane;
     const char *px = uniform_part<T>(S.x, b, c0), *pg = uniform_part<T>(S.gate, b, c0), *pb = uniform_part<T>(S.before, b, c0);
     const char* pr = uniform_part<uint8_t>(S.resets, b, 0);
-    char *ph = (char*)uniform_part<T>(S.h, b, c0), *po = (char*)uniform_part<T>(S.second, b, c0);
+    char *ph = (char*)uniform_part<T>(S.h, b, c0), *po = (char*)uniform_part<T>(S.second, b, c0), *pk = (char*)uniform_part<W>(S.keep, b, c0);
     const int64_t size = sizeof(T), sx = S.x.st * size, sg = S.gate.st * size, sb = S.before.st * size;
     char *rx = rows_of[wt][0], *rg = rows_of[wt][1], *rb = rows_of[wt][BEFORE ? 2 : 0];
     W carry = first_state<K, W>(S, q);
     const W edge[1] = {edge_of<K, W>(S, q)};
     Tile<T> x, g, before;
     uint8_t flag = 0;
+    T own{};                                          // AGAIN: the gate of the run's last step, and the state before it
+    W kept{};
     auto ask = [&](int64_t u0) {
         x.load(px, sx, u0, S.steps, lane);
         if constexpr (O::GATE) g.load(pg, sg, u0 - shift, S.steps, lane);
-        if constexpr (BEFORE) before.load(pb, sb, u0 + 1, S.steps, lane);
+        if constexpr (BEFORE) before.load(pb, sb, u0 + (O::AGAIN ? 0 : 1), S.steps, lane);
+        if constexpr (O::AGAIN) {
+            if (u0 + L <= S.steps) own = ((const T __attribute__((address_space(1)))*)((Global)pg + (u0 + L - 1) * sg))[lane];
+            if (u0 + L < S.steps) kept = ((const W __attribute__((address_space(1)))*)((Global)pk + u0 / L * S.keep.st * (int64_t)sizeof(W)))[lane];
+        }
         if constexpr (O::RESETS) {
             const int64_t at = u0 - shift + lane;
             flag = 0;
@@ -541,6 +584,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
         }
     };
     ask(wt * L);
+    const int keep = (int)(S.steps % L);
     int turn = 0;
     for (int64_t u = 0; u < S.steps; u += TURN, turn ^= 1) {
         const int64_t u0 = u + wt * L;
@@ -548,9 +592,10 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
         if constexpr (O::GATE) g.to_rows(rg, lane);
         if constexpr (BEFORE) before.to_rows(rb, lane);
         const uint64_t flags = O::RESETS ? __ballot(flag != 0) : 0;
+        Raw<O, 1> raw;
+        if constexpr (O::AGAIN) { raw.g[L] = own; raw.kept[0] = kept; }
         rows_written();
         if (u + TURN < S.steps) ask(u0 + TURN);
-        Raw<O, 1> raw;
 #pragma unroll
         for (int i = 0; i < L; i++) {
             raw.x[i] = ((const T*)rx)[i * 64 + lane];
@@ -566,7 +611,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
         const Pair<W> own = pair_of<O, 1>(f, 0);
         pairs_of[turn][wt][lane] = own;
         lds_barrier();
-        W h = carry;
+        W h = carry, own_kept{};
 #pragma unroll
         for (int w = 0; w < WT; w++) {
             if (w == wt) h = carry;
@@ -575,6 +620,7 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
         }
 #pragma unroll
         for (int i = 0; i < L; i++) {
+            if (O::KEEP && i == keep) own_kept = h;
             h = step(f.a[i], h, f.x[i]);
             ((T*)rx)[i * 64 + lane] = (T)h;
             if constexpr (O::SECOND) ((T*)rg)[i * 64 + lane] = second_of<O, 1>(f, i, h);
@@ -586,6 +632,9 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
         if constexpr (O::SECOND) {
             out.from_rows(rg, lane);
             out.store(po, S.second.st * size, u0, S.steps, lane);
+        }
+        if constexpr (O::KEEP) {
+            if (u0 + keep < S.steps) ((W __attribute__((address_space(1)))*)((Global)pk + keep_offset<O>(S, u0 + keep)))[lane] = own_kept;
         }
         rows_written();
     }
@@ -651,9 +700,12 @@ __device__ __forceinline__ void load_run(const Seq& S, const Place& P, int64_t u
     using T = typename O::T;
     get_run<T, DIR, L, FULL>(P.x, u0, end, d.x);
     if constexpr (O::K == BACKWARD) {
-        if constexpr (O::GATE) get_shifted<T, DIR, FULL, true, L>(P.gate, u0, end, end, d.g);
+        if constexpr (O::GATE) get_shifted<T, DIR, FULL, true, L + (O::AGAIN && APPLYING ? 1 : 0)>(P.gate, u0, end, end, d.g);
         if constexpr (O::RESETS) get_shifted<uint8_t, DIR, FULL, true, L + (O::SECOND ? 1 : 0)>(P.resets, u0, end, end, d.r);
-        if constexpr (O::SECOND && APPLYING) get_shifted<T, DIR, FULL, false, L>(P.before, u0, end, S.steps, d.before);
+        if constexpr (O::AGAIN && APPLYING) {
+            get_run<T, DIR, L, FULL>(P.before, u0, end, d.before);
+            if (u0 + L < S.steps) d.kept[0] = ((const typename O::W*)P.keep)[u0 / L * S.keep.st];
+        } else if constexpr (O::SECOND && APPLYING) get_shifted<T, DIR, FULL, false, L>(P.before, u0, end, S.steps, d.before);
     } else {
         if constexpr (O::GATE) get_run<T, DIR, L, FULL>(P.gate, u0, end, d.g);
         if constexpr (O::RESETS) get_run<uint8_t, DIR, L, FULL>(P.resets, u0, end, d.r);
@@ -672,14 +724,20 @@ template <class O, int DIR, bool FULL>
 __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<O, 1>& f, int64_t u0, int64_t end, typename O::W h) {
     using E = typename O::Out;
     E out[L], second[O::SECOND ? L : 1];
+    const int keep = (int)(S.steps % L);
+    typename O::W kept{};
 #pragma unroll
     for (int i = 0; i < L; i++) {
+        if (O::KEEP && i == keep) kept = h;
         h = step(f.a[i], h, f.x[i]);
         out[i] = (E)h;
         if constexpr (O::SECOND) second[i] = second_of<O, 1>(f, i, h);
     }
     put_run<E, DIR, FULL>(P.h, u0, end, out);
     if constexpr (O::SECOND) put_run<E, DIR, FULL>(P.second, u0, end, second);
+    if constexpr (O::KEEP) {
+        if (u0 + keep < S.steps) *(typename O::W*)(P.keep + keep_offset<O>(S, u0 + keep)) = kept;
+    }
 }
 
 template <class W> __device__ __forceinline__ Pair<W> up(const Pair<W>& p, int by) { return Pair<W>{__shfl_up(p.a, by), __shfl_up(p.h, by)}; }
@@ -839,7 +897,7 @@ bool near(const View& v, const Seq& S, int64_t size, int tile) {
 }
 template <class O> bool near(const Seq& S, int tile) {
     constexpr int64_t n = sizeof(typename O::T);
-    return near(S.x, S, n, tile) && near(S.gate, S, n, tile) && near(S.before, S, n, tile) && near(S.resets, S, 1, tile) &&
+    return near(S.keep, S, sizeof(typename O::W), tile) && near(S.x, S, n, tile) && near(S.gate, S, n, tile) && near(S.before, S, n, tile) && near(S.resets, S, 1, tile) &&
            near(S.h, S, n, tile) && near(S.second, S, n, tile);
 }
 
@@ -848,8 +906,8 @@ template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hip
     if (!flat) {
         // Channels that lie so far apart that 64 of them pass 32 bits (time is the fast index of a long trajectory): fewer to a tile.
         S.width = 64;
-        for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second})
-            while (S.width > 1 && v->p && v->sc >= ((int64_t)1 << 32) / (S.width * (int64_t)sizeof(typename O::T))) S.width /= 2;
+        for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second, &S.keep})
+            while (S.width > 1 && v->p && v->sc >= ((int64_t)1 << 32) / (S.width * (int64_t)sizeof(typename O::W))) S.width /= 2;
         S.tight = cdiv(S.channels, S.width);
     }
     const int64_t tiles = cdiv(flat ? cdiv(S.cols, 64 * V) : S.cols / S.channels * S.tight, WT == 1 ? 4 : 1);
@@ -902,7 +960,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
         // steps of 72 float32: 45 us instead of 55; float64 gains nothing), and for advantages of many sequences, whose 21 bytes
         // a step keep the memory busy with half the wavefronts (but not in parts: 2048 x 2000 float64 41 us instead of 31).
         const bool even = S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) && dense(S.gate, S.channels) &&
-                          dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels) && near<O>(S, 128);
+                          dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels) && dense(S.keep, S.channels) && near<O>(S, 128);
         if constexpr (O::K == ADVANTAGES) {
             if (even && S.cols >= 65536 && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
             if (even && S.cols >= 65536 && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
@@ -914,7 +972,7 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
         // (256 x 300 x 1024) the memory is busy without: 104 us forward, with them 111.
         if constexpr (O::K != ADVANTAGES && sizeof(typename O::T) <= 4) {
             bool tiles = (d.wt == 16 || (d.wt == 4 && S.steps > kTileWaves * L)) && d.parts == 1 && S.channels % 64 == 0;
-            for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second}) tiles = tiles && (!v->p || v->sc == 1);
+            for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second, &S.keep}) tiles = tiles && (!v->p || v->sc == 1);
             if (tiles) return tiles_kernel<O><<<(unsigned)(S.cols / 64), 64 * kTileWaves, 0, stream>>>(S), 0;
         }
         if (d.wt == 1) launch_columns<O, 1, 1>(S, d, stream);
@@ -929,7 +987,10 @@ template <Kind K, class T> int run(const Seq& S, void* workspace, hipStream_t st
     if constexpr (K == ADVANTAGES) rc = launch<Op<K, T, false, true, true>>(S, workspace, stream, who);
     else {
         const bool resets = S.resets.p;
-        if (K == BACKWARD && S.second.p) {
+        if (S.keep.p && K == SCAN) {
+            if constexpr (sizeof(T) == 2) rc = resets ? launch<Op<K, T, true, true, true>>(S, workspace, stream, who) : launch<Op<K, T, true, false, true>>(S, workspace, stream, who);
+            else rc = fail(-1, "%s: 16-bit sequences only", who);
+        } else if (K == BACKWARD && S.second.p) {
             if (resets) rc = launch<Op<K, T, true, true, K == BACKWARD>>(S, workspace, stream, who);
             else rc = launch<Op<K, T, true, false, K == BACKWARD>>(S, workspace, stream, who);
         } else if (S.gate.p) {
@@ -961,6 +1022,57 @@ int check_workspace(const lrn_seq* q, const void* workspace, int64_t bytes, cons
     return 0;
 }
 
+int scan(const char* who, int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate, double gate_const,
+         const lrn_view* resets, const void* initial, const lrn_view* h_out, const lrn_view* kept_out, void* final_out, void* workspace,
+         int64_t workspace_bytes) {
+    if (int rc = checked(seq, who)) return rc;
+    if (seq->batch * seq->channels == 0) return 0;
+    if (seq->steps && (!x || !x->data || !h_out || !h_out->data)) return fail(-1, "%s: null x or h", who);
+    if (int rc = check_views(who, {x, gate, resets, h_out, kept_out})) return rc;
+    if (int rc = check_workspace(seq, workspace, workspace_bytes, who)) return rc;
+    LRN_ON_DEVICE(device);
+    const bool rev = seq->reverse != 0;
+    const int64_t n = bytes_of(seq->dtype);
+    Seq S{};
+    S.steps = seq->steps; S.cols = seq->batch * seq->channels; S.channels = seq->channels;
+    S.x = ordered(x, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
+    S.resets = ordered(resets, seq->steps, 1, rev); S.h = ordered(h_out, seq->steps, n, rev);
+    S.keep = ordered(seq->steps ? kept_out : nullptr, 0, 4, false);
+    S.gate_const = gate_const; S.initial = initial; S.final = final_out;
+    return run<SCAN>(S, seq->dtype, workspace, (hipStream_t)hip_stream, who);
+}
+
+// `states`: h, or x beside `kept`
+int backward(const char* who, int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const, const lrn_view* resets,
+             const void* initial, const lrn_view* states, const lrn_view* kept, const lrn_view* g_h, const void* g_final, const lrn_view* grad_x_out,
+             const lrn_view* grad_gate_out, void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
+    if (int rc = checked(seq, who)) return rc;
+    if (seq->batch * seq->channels == 0) return 0;
+    if (seq->steps && (!g_h || !g_h->data || !grad_x_out || !grad_x_out->data)) return fail(-1, "%s: null g_h or grad_x", who);
+    const bool want_gate = seq->steps && grad_gate_out && grad_gate_out->data;
+    if (want_gate && (!states || !states->data || !gate || !gate->data)) return fail(-1, "%s: null %s or gate", who, kept ? "x" : "h");
+    if (int rc = check_views(who, {gate, resets, states, kept, g_h, grad_x_out, grad_gate_out})) return rc;
+    if (int rc = check_workspace(seq, workspace, workspace_bytes, who)) return rc;
+    LRN_ON_DEVICE(device);
+    const bool rev = seq->reverse == 0;
+    const int64_t n = bytes_of(seq->dtype);
+    Seq S{};
+    S.steps = seq->steps; S.cols = seq->batch * seq->channels; S.channels = seq->channels;
+    S.x = ordered(g_h, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
+    S.resets = ordered(resets, seq->steps, 1, rev); S.before = ordered(want_gate ? states : nullptr, seq->steps, n, rev);
+    S.keep = ordered(want_gate ? kept : nullptr, 0, 4, false);
+    S.h = ordered(grad_x_out, seq->steps, n, rev); S.second = ordered(want_gate ? grad_gate_out : nullptr, seq->steps, n, rev);
+    S.gate_const = gate_const; S.initial = g_final; S.edge = initial; S.final = grad_initial_out;
+    return run<BACKWARD>(S, seq->dtype, workspace, (hipStream_t)hip_stream, who);
+}
+
+int keeping(const lrn_seq* seq, const lrn_view* gate, const lrn_view* kept, const char* who) {
+    if (int rc = checked(seq, who)) return rc;
+    if (seq->dtype != LRN_BF16 && seq->dtype != LRN_F16) return fail(-1, "%s: dtype %d: 16-bit sequences only (h holds the states of the others)", who, seq->dtype);
+    if (seq->steps && seq->batch * seq->channels && (!gate || !gate->data || !kept || !kept->data)) return fail(-1, "%s: null gate or kept states", who);
+    return 0;
+}
+
 int64_t workspace_of(const lrn_seq* q) { return q && checked(q, "workspace") == 0 ? pair_bytes(q) : 0; }
 
 }  // namespace
@@ -975,43 +1087,34 @@ int64_t lrn_scan_workspace(const lrn_seq* seq) { return workspace_of(seq); }
 int lrn_scan(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
              double gate_const, const lrn_view* resets, const void* initial, const lrn_view* h_out, void* final_out, void* workspace,
              int64_t workspace_bytes) {
-    if (int rc = checked(seq, "lrn_scan")) return rc;
-    if (seq->batch * seq->channels == 0) return 0;
-    if (seq->steps && (!x || !x->data || !h_out || !h_out->data)) return fail(-1, "lrn_scan: null x or h");
-    if (int rc = check_views("lrn_scan", {x, gate, resets, h_out})) return rc;
-    if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_scan")) return rc;
-    LRN_ON_DEVICE(device);
-    const bool rev = seq->reverse != 0;
-    const int64_t n = bytes_of(seq->dtype);
-    Seq S{};
-    S.steps = seq->steps; S.cols = seq->batch * seq->channels; S.channels = seq->channels;
-    S.x = ordered(x, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
-    S.resets = ordered(resets, seq->steps, 1, rev); S.h = ordered(h_out, seq->steps, n, rev);
-    S.gate_const = gate_const; S.initial = initial; S.final = final_out;
-    return run<SCAN>(S, seq->dtype, workspace, (hipStream_t)hip_stream, "lrn_scan");
+    return scan("lrn_scan", device, hip_stream, seq, x, gate, gate_const, resets, initial, h_out, nullptr, final_out, workspace, workspace_bytes);
+}
+
+int lrn_scan_keep(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
+                  const lrn_view* resets, const void* initial, const lrn_view* h_out, const lrn_view* kept_out, void* final_out,
+                  void* workspace, int64_t workspace_bytes) {
+    if (int rc = keeping(seq, gate, kept_out, "lrn_scan_keep")) return rc;
+    return scan("lrn_scan_keep", device, hip_stream, seq, x, gate, 0.0, resets, initial, h_out, kept_out, final_out, workspace, workspace_bytes);
 }
 
 int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const,
                       const lrn_view* resets, const void* initial, const lrn_view* h, const lrn_view* g_h,
                       const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
                       void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
-    if (int rc = checked(seq, "lrn_scan_backward")) return rc;
-    if (seq->batch * seq->channels == 0) return 0;
-    if (seq->steps && (!g_h || !g_h->data || !grad_x_out || !grad_x_out->data)) return fail(-1, "lrn_scan_backward: null g_h or grad_x");
-    const bool want_gate = seq->steps && grad_gate_out && grad_gate_out->data;
-    if (want_gate && (!h || !h->data || !gate || !gate->data)) return fail(-1, "lrn_scan_backward: null h or gate");
-    if (int rc = check_views("lrn_scan_backward", {gate, resets, h, g_h, grad_x_out, grad_gate_out})) return rc;
-    if (int rc = check_workspace(seq, workspace, workspace_bytes, "lrn_scan_backward")) return rc;
-    LRN_ON_DEVICE(device);
-    const bool rev = seq->reverse == 0;
-    const int64_t n = bytes_of(seq->dtype);
-    Seq S{};
-    S.steps = seq->steps; S.cols = seq->batch * seq->channels; S.channels = seq->channels;
-    S.x = ordered(g_h, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
-    S.resets = ordered(resets, seq->steps, 1, rev); S.before = ordered(want_gate ? h : nullptr, seq->steps, n, rev);
-    S.h = ordered(grad_x_out, seq->steps, n, rev); S.second = ordered(want_gate ? grad_gate_out : nullptr, seq->steps, n, rev);
-    S.gate_const = gate_const; S.initial = g_final; S.edge = initial; S.final = grad_initial_out;
-    return run<BACKWARD>(S, seq->dtype, workspace, (hipStream_t)hip_stream, "lrn_scan_backward");
+    if (seq && (seq->dtype == LRN_BF16 || seq->dtype == LRN_F16) && grad_gate_out && grad_gate_out->data)
+        return fail(-1, "lrn_scan_backward: h holds rounded states: lrn_scan_keep_backward has the gate's gradient of 16-bit sequences");
+    return backward("lrn_scan_backward", device, hip_stream, seq, gate, gate_const, resets, initial, h, nullptr, g_h, g_final, grad_x_out, grad_gate_out,
+                    grad_initial_out, workspace, workspace_bytes);
+}
+
+int lrn_scan_keep_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
+                           const lrn_view* resets, const void* initial, const lrn_view* kept, const lrn_view* g_h,
+                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
+                           void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
+    if (int rc = keeping(seq, gate, kept, "lrn_scan_keep_backward")) return rc;
+    if (seq->steps && (!grad_gate_out || !grad_gate_out->data)) return fail(-1, "lrn_scan_keep_backward: null grad_gate");
+    return backward("lrn_scan_keep_backward", device, hip_stream, seq, gate, 0.0, resets, initial, x, kept, g_h, g_final, grad_x_out, grad_gate_out,
+                    grad_initial_out, workspace, workspace_bytes);
 }
 
 int64_t lrn_advantages_workspace(const lrn_seq* seq) { return workspace_of(seq); }

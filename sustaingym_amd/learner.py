@@ -34,6 +34,7 @@ _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _SEQ_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}
 MAX_TOP = _lib.LEARNER_MAX_TOP
 _SHORT_ROW = _lib.LEARNER_SHORT_ROW      # up to here no workspace and no statistics for the backward pass
+_KEEP = _lib.LEARNER_KEEP                # of 16-bit sequences every so many steps' state is kept for the backward pass
 
 
 class LevelChoice(NamedTuple):
@@ -341,7 +342,16 @@ def _laid_out(shape, stride, dtype, device):
     return torch.empty_strided(shape, stride, dtype=dtype, device=device)
 
 
-def _scan(x, gate, gate_const, initial, resets, dim, reverse):
+def _kept(h, dim):
+    """Room for every eighth state of 16-bit ``h``, ``[elements, N, C]``: along time where h is, by columns otherwise."""
+    steps, N = h.shape[dim], h.shape[1 - dim] if h.dim() > 1 else 1
+    C_, n = h.shape[2] if h.dim() > 2 else 1, -(-steps // _KEEP)
+    if C_ == 1 and steps > 1 and h.stride(dim) == 1:
+        return torch.empty((N, n, 1), dtype=torch.float32, device=h.device).transpose(0, 1)
+    return torch.empty((n, N, C_), dtype=torch.float32, device=h.device)
+
+
+def _scan(x, gate, gate_const, initial, resets, dim, reverse, keep=False):
     lib, device = _lib.load(), x.device
     h = torch.empty(x.shape, dtype=x.dtype, device=device) if x.is_contiguous() else _laid_out(x.shape, x.stride(), x.dtype, device)
     final = torch.empty(x.shape[:dim] + x.shape[dim + 1:], dtype=_state_type(x.dtype), device=device)
@@ -349,19 +359,25 @@ def _scan(x, gate, gate_const, initial, resets, dim, reverse):
     ref = C.byref(seq)
     nbytes = lib.lrn_scan_workspace(ref)
     ws = _workspace(nbytes, device)
-    _check(lib.lrn_scan(device.index, _stream(device), ref, _ref(_view(x, dim)), _ref(_view(gate, dim)), gate_const,
-                        _ref(_view(resets, dim)), _ptr(initial), _ref(_view(h, dim)), final.data_ptr(), _ptr(ws), nbytes),
-           'gated_scan')
+    stream, views = _stream(device), (_ref(_view(x, dim)), _ref(_view(gate, dim)), _ref(_view(resets, dim)), _ref(_view(h, dim)))
+    if keep:
+        kept = _kept(h, dim)
+        _check(lib.lrn_scan_keep(device.index, stream, ref, views[0], views[1], views[2], _ptr(initial), views[3], _ref(_view(kept, 0)),
+                                 final.data_ptr(), _ptr(ws), nbytes), 'gated_scan')
+        return h, final, kept
+    _check(lib.lrn_scan(device.index, stream, ref, views[0], views[1], gate_const, views[2], _ptr(initial), views[3],
+                        final.data_ptr(), _ptr(ws), nbytes), 'gated_scan')
     return h, final
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, resets, gate_const, dim, reverse):
-        h, final = _scan(x, gate, gate_const, initial, resets, dim, reverse)
-        # The gate's gradient needs the states; where they were rounded to 16 bits, so is their share of it (half a step of h),
-        # for what reading x and walking forward again would cost.
-        ctx.save_for_backward(gate, resets, initial, h if ctx.needs_input_grad[1] else None)
+        # The gate's gradient needs the states.  h holds them, but rounded for 16-bit sequences: there every eighth is kept in
+        # float32, and the backward pass walks the others again from x.
+        keep = ctx.needs_input_grad[1] and x.dtype in (torch.bfloat16, torch.float16)
+        h, final, *kept = _scan(x, gate, gate_const, initial, resets, dim, reverse, keep)
+        ctx.save_for_backward(gate, resets, initial, (x if keep else h) if ctx.needs_input_grad[1] else None, *kept)
         ctx.args = (gate_const, dim, reverse, x.shape, x.stride(), x.dtype, x.device)
         ctx.set_materialize_grads(False)
         return h, final
@@ -372,7 +388,7 @@ class _GatedScan(torch.autograd.Function):
 
     @staticmethod
     def _gradient(ctx, g_h, g_final):
-        gate, resets, initial, h = ctx.saved_tensors
+        gate, resets, initial, states, *kept = ctx.saved_tensors
         gate_const, dim, reverse, shape, stride, dtype, device = ctx.args
         want_x, want_gate, want_initial = ctx.needs_input_grad[:3]
         if g_h is None and g_final is None:
@@ -388,10 +404,14 @@ class _GatedScan(torch.autograd.Function):
         ref = C.byref(seq)
         nbytes = lib.lrn_scan_workspace(ref)
         ws = _workspace(nbytes, device)
-        _check(lib.lrn_scan_backward(device.index, _stream(device), ref, _ref(_view(gate, dim)), gate_const,
-                                     _ref(_view(resets, dim)), _ptr(initial), _ref(_view(h, dim)), _ref(_view(g_h, dim)),
-                                     _ptr(g_final), _ref(_view(gx, dim)), _ref(_view(gg, dim)), _ptr(gi), _ptr(ws), nbytes),
-               'gated_scan backward')
+        stream, up, out = _stream(device), (_ref(_view(g_h, dim)), _ptr(g_final)), (_ref(_view(gx, dim)), _ref(_view(gg, dim)), _ptr(gi), _ptr(ws), nbytes)
+        if kept and want_gate:
+            _check(lib.lrn_scan_keep_backward(device.index, stream, ref, _ref(_view(states, dim)), _ref(_view(gate, dim)),
+                                              _ref(_view(resets, dim)), _ptr(initial), _ref(_view(kept[0], 0)), *up, *out),
+                   'gated_scan backward')
+        else:
+            _check(lib.lrn_scan_backward(device.index, stream, ref, _ref(_view(gate, dim)), gate_const, _ref(_view(resets, dim)),
+                                         _ptr(initial), _ref(_view(states, dim)), *up, *out), 'gated_scan backward')
         return gx if want_x else None, gg, gi, None, None, None, None
 
 
@@ -413,7 +433,8 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
     NaN or an infinity of the state may be gone.
 
     ``h`` has x's type and layout (contiguous where x has holes or is expanded); ``final`` is the last state of the walk in the
-    state's own type, what a following call takes as ``initial``.  Differentiable in x, gate and initial."""
+    state's own type, what a following call takes as ``initial``.  Differentiable in x, gate and initial; gradients are made of states
+    in the state's own type, also where h holds them rounded to 16 bits."""
     _on_device('x', x)
     device, shape = x.device, x.shape
     if x.dtype not in _SEQ_TYPES:

@@ -1,0 +1,49 @@
+"""What lrn_scan_keep and lrn_scan_keep_backward refuse, before the device is touched."""
+import ctypes as C
+import os
+import re
+
+from sustaingym_amd import _lib
+
+
+def test_keeping_refuses():
+    lib = _lib.load()
+    one = C.c_void_p(64)            # never dereferenced by a refused call
+
+    def text():
+        return lib.lrn_last_error().decode()
+
+    def seq(**kw):
+        return C.byref(_lib.LearnerSeq(**{**dict(steps=4, batch=2, channels=3, reverse=0, dtype=1), **kw}))
+
+    def forward(s, x, gate, h, kept):
+        return lib.lrn_scan_keep(0, None, s, x, gate, None, None, h, kept, one, None, 0)
+
+    def backward(s, x, gate, kept, g_h, gx, gg):
+        return lib.lrn_scan_keep_backward(0, None, s, x, gate, None, None, kept, g_h, None, gx, gg, None, None, 0)
+
+    v, back = C.byref(_lib.LearnerView(64, 6, 3, 1)), C.byref(_lib.LearnerView(64, 6, -3, 1))
+    for kw in (dict(dtype=0), dict(dtype=3), dict(dtype=4), dict(steps=-1), dict(batch=-1)):
+        assert forward(seq(**kw), v, v, v, v) == -1 and backward(seq(**kw), v, v, v, v, v, v) == -1
+    assert forward(None, v, v, v, v) == -1 and backward(None, v, v, v, v, v, v) == -1
+    for k in range(4):
+        views = [v, v, v, v]
+        views[k] = None
+        assert forward(seq(), *views) == -1 and 'null' in text(), k
+    for k in range(6):
+        views = [v] * 6
+        views[k] = None
+        assert backward(seq(), *views) == -1 and 'null' in text(), k
+    assert forward(seq(), v, v, v, back) == -1 and 'negative' in text()
+    assert backward(seq(), v, v, back, v, v, v) == -1 and 'negative' in text()
+    # the gate's gradient from rounded states
+    for dtype in (1, 2):
+        assert lib.lrn_scan_backward(0, None, seq(dtype=dtype), v, 0.0, None, None, v, v, None, v, v, None, None, 0) == -1 and 'rounded' in text()
+    long = seq(steps=10 ** 6, batch=1, channels=1)
+    need = lib.lrn_scan_workspace(long)
+    assert need and lib.lrn_scan_keep(0, None, long, v, v, None, None, v, v, one, one, need - 1) == -1 and 'workspace' in text()
+
+
+def test_the_header_and_the_binding_keep_alike():
+    text = open(os.path.join(os.path.dirname(_lib.HEADER_PATH), 'learner_ops.h')).read()
+    assert int(re.search(r'#define\s+LRN_KEEP\s+(\d+)', text).group(1)) == _lib.LEARNER_KEEP
