@@ -114,14 +114,15 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
  * writes every LRN_KEEP-th state as it is: kept, float32 with strides (element, batch, channel) that are not negative, has
  * (steps + LRN_KEEP - 1) / LRN_KEEP elements a column, of which the j-th holds the state before the step that has
  * (j + 1) * LRN_KEEP - 1 behind it (the last element, the first step's or none's, need not be written and is not read).
- * lrn_scan_keep_backward walks the states in between again from x. */
+ * lrn_scan_keep_backward walks the states in between again from x; grad_gate_dtype: the sequence's, or LRN_F32 for a gradient that
+ * is going to be summed (of a broadcast gate). */
 #define LRN_KEEP 8
 int lrn_scan_keep(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
                   const lrn_view* resets, const void* initial, const lrn_view* h_out, const lrn_view* kept_out, void* final_out,
                   void* workspace, int64_t workspace_bytes);
 int lrn_scan_keep_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
                            const lrn_view* resets, const void* initial, const lrn_view* kept, const lrn_view* g_h,
-                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
+                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out, int32_t grad_gate_dtype,
                            void* grad_initial_out, void* workspace, int64_t workspace_bytes);
 
 /* Generalised advantages of `steps` x `batch` (channels = 1, reverse ignored):

@@ -163,7 +163,7 @@ LEARNER_SIGNATURES = {
     'lrn_scan': (_i32, [_i32, _vp, _seq, _view, _view, C.c_double, _view, _vp, _view, _vp, _vp, _i64]),
     'lrn_scan_backward': (_i32, [_i32, _vp, _seq, _view, C.c_double, _view, _vp, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
     'lrn_scan_keep': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
-    'lrn_scan_keep_backward': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, _view, _view, _vp, _view, _view, _vp, _vp, _i64]),
+    'lrn_scan_keep_backward': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, _view, _view, _vp, _view, _view, _i32, _vp, _vp, _i64]),
     'lrn_advantages_workspace': (_i64, [_seq]),
     'lrn_advantages': (_i32, [_i32, _vp, _seq, _view, _view, _view, _vp, C.c_double, C.c_double, _view, _view, _vp, _i64]),
 }

@@ -59,6 +59,7 @@ struct Seq {
     int64_t group;              // RUNS: lanes of a column, where a wavefront has all its steps
     int64_t tight, width;       // COLUMNS: tiles of a sequence where a tile may not reach over two (else 0), and their channels
     void* pairs;                // [parts][2][cols]
+    bool sums;                  // BACKWARD of 16-bit sequences: the gate's gradient in float32
 };
 
 enum Kind { SCAN, BACKWARD, ADVANTAGES };
@@ -88,7 +89,7 @@ constexpr int L = LRN_KEEP;      // steps of a lane's run: 8
 
 // One of the three, for one type of elements: whether there is a gate tensor (else a constant), whether there are resets, and
 // whether the second output (SCAN: the kept states) is wanted.  Compiled in: a condition between loads keeps them from being in flight together.
-template <Kind K_, class T_, bool GATE_, bool RESETS_, bool SECOND_>
+template <Kind K_, class T_, bool GATE_, bool RESETS_, bool SECOND_, class P_ = T_>
 struct Op {
     static constexpr Kind K = K_;
     static constexpr bool GATE = GATE_, RESETS = RESETS_, SECOND = SECOND_ && K_ != SCAN;
@@ -96,6 +97,7 @@ struct Op {
     using T = T_;
     using W = typename State<T_>::type;
     using Out = std::conditional_t<K_ == ADVANTAGES, float, T_>;
+    using Second = std::conditional_t<K_ == ADVANTAGES, float, P_>;     // (P_: the gate's gradient, float32 where it is going to be summed)
 };
 
 // One lane's run, L steps of V adjacent columns: as it comes from memory ...
@@ -283,10 +285,10 @@ template <class O, int V> __device__ __forceinline__ Pair<typename O::W> pair_of
 }
 
 // The second output of a step from the state behind it.
-template <class O, int V> __device__ __forceinline__ typename O::Out second_of(const Run<O, V>& f, int n, typename O::W h) {
+template <class O, int V> __device__ __forceinline__ typename O::Second second_of(const Run<O, V>& f, int n, typename O::W h) {
     using W = typename O::W;
-    if constexpr (O::K == BACKWARD) return (typename O::Out)(O::RESETS && (f.anew >> n & 1) ? W(0) : h * f.extra[n]);
-    else return (typename O::Out)(h + (W)f.extra[n]);
+    if constexpr (O::K == BACKWARD) return (typename O::Second)(O::RESETS && (f.anew >> n & 1) ? W(0) : h * f.extra[n]);
+    else return (typename O::Second)(h + (W)f.extra[n]);
 }
 
 // Where the state before step `at` of SCAN is kept: BACKWARD's runs are counted from the last step.
@@ -296,14 +298,16 @@ template <class O> __device__ __forceinline__ int64_t keep_offset(const Seq& S, 
 template <class O, int V, bool FULL>
 __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, V>& f, int64_t u0, int64_t end, typename O::W (&h)[V]) {
     using E = typename O::Out;
-    Global ph = (Global)(P.h + u0 * S.h.st * (int64_t)sizeof(E)), po = (Global)(P.second + u0 * S.second.st * (int64_t)sizeof(E));
+    using D = typename O::Second;
+    Global ph = (Global)(P.h + u0 * S.h.st * (int64_t)sizeof(E)), po = (Global)(P.second + u0 * S.second.st * (int64_t)sizeof(D));
     const int last = FULL ? L : in_front(u0, end, L);
     const uint32_t oh = kept_apart(P.oh), oo = O::SECOND ? kept_apart(P.oo) : 0;
     const int keep = (int)(S.steps % L);                   // of every run, the step that begins one of BACKWARD's
     typename O::W kept[V];
 #pragma unroll
     for (int i = 0; i < L; i++) {
-        E out[V], second[V];
+        E out[V];
+        D second[V];
 #pragma unroll
         for (int k = 0; k < V; k++) {
             if (O::KEEP && i == keep) kept[k] = h[k];
@@ -313,10 +317,10 @@ __device__ __forceinline__ void walk(const Seq& S, const Place& P, const Run<O, 
         }
         if (FULL || i < last) {
             put<E, V>(ph, oh, out);
-            if constexpr (O::SECOND) put<E, V>(po, oo, second);
+            if constexpr (O::SECOND) put<D, V>(po, oo, second);
         }
         advance(ph, S.h.st * (int64_t)sizeof(E));
-        if constexpr (O::SECOND) advance(po, S.second.st * (int64_t)sizeof(E));
+        if constexpr (O::SECOND) advance(po, S.second.st * (int64_t)sizeof(D));
     }
     if constexpr (O::KEEP) {
         if (u0 < end && u0 + keep < S.steps) put<typename O::W, V>((Global)(P.keep + keep_offset<O>(S, u0 + keep)), kept_apart(P.ok), kept);
@@ -336,7 +340,7 @@ template <class O> __device__ __forceinline__ Place place_of(const Seq& S, int64
     P.before = uniform_part<E>(S.before, b0, c0); P.ob = lane_part<E>(S.before, b - b0, c - c0);
     P.resets = uniform_part<uint8_t>(S.resets, b0, 0); P.orr = lane_part<uint8_t>(S.resets, b - b0, 0);
     P.h = (char*)uniform_part<E>(S.h, b0, c0); P.oh = lane_part<E>(S.h, b - b0, c - c0);
-    P.second = (char*)uniform_part<E>(S.second, b0, c0); P.oo = lane_part<E>(S.second, b - b0, c - c0);
+    P.second = (char*)uniform_part<typename O::Second>(S.second, b0, c0); P.oo = lane_part<typename O::Second>(S.second, b - b0, c - c0);
     P.keep = (char*)uniform_part<typename O::W>(S.keep, b0, c0); P.ok = lane_part<typename O::W>(S.keep, b - b0, c - c0);
     P.next_flags = S.channels == 1 ? (uint32_t)S.resets.sb : 0;
     return P;
@@ -553,14 +557,15 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
     using W = typename O::W;
     constexpr int64_t TURN = WT * L;
     constexpr bool back = K == BACKWARD, BEFORE = back && O::SECOND;
-    constexpr int FLAGS = L + (BEFORE ? 1 : 0), shift = back ? 1 : 0, BYTES = Tile<T>::BYTES;
+    using D = typename O::Second;
+    constexpr int FLAGS = L + (BEFORE ? 1 : 0), shift = back ? 1 : 0, BYTES = std::max(Tile<T>::BYTES, Tile<D>::BYTES);
     __shared__ Pair<W> pairs_of[2][WT][64];
     __shared__ __attribute__((aligned(16))) char rows_of[WT][BEFORE ? 3 : 2][BYTES];
     const int lane = threadIdx.x & 63, wt = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t q0 = (int64_t)blockIdx.x * 64, b = q0 / S.channels, c0 = q0 - b * S.channels, q = q0 + lane;
     const char *px = uniform_part<T>(S.x, b, c0), *pg = uniform_part<T>(S.gate, b, c0), *pb = uniform_part<T>(S.before, b, c0);
     const char* pr = uniform_part<uint8_t>(S.resets, b, 0);
-    char *ph = (char*)uniform_part<T>(S.h, b, c0), *po = (char*)uniform_part<T>(S.second, b, c0), *pk = (char*)uniform_part<W>(S.keep, b, c0);
+    char *ph = (char*)uniform_part<T>(S.h, b, c0), *po = (char*)uniform_part<D>(S.second, b, c0), *pk = (char*)uniform_part<W>(S.keep, b, c0);
     const int64_t size = sizeof(T), sx = S.x.st * size, sg = S.gate.st * size, sb = S.before.st * size;
     char *rx = rows_of[wt][0], *rg = rows_of[wt][1], *rb = rows_of[wt][BEFORE ? 2 : 0];
     W carry = first_state<K, W>(S, q);
@@ -623,15 +628,16 @@ __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
             if (O::KEEP && i == keep) own_kept = h;
             h = step(f.a[i], h, f.x[i]);
             ((T*)rx)[i * 64 + lane] = (T)h;
-            if constexpr (O::SECOND) ((T*)rg)[i * 64 + lane] = second_of<O, 1>(f, i, h);
+            if constexpr (O::SECOND) ((D*)rg)[i * 64 + lane] = second_of<O, 1>(f, i, h);
         }
         rows_written();
         Tile<T> out;
         out.from_rows(rx, lane);
         out.store(ph, S.h.st * size, u0, S.steps, lane);
         if constexpr (O::SECOND) {
-            out.from_rows(rg, lane);
-            out.store(po, S.second.st * size, u0, S.steps, lane);
+            Tile<D> beside;
+            beside.from_rows(rg, lane);
+            beside.store(po, S.second.st * (int64_t)sizeof(D), u0, S.steps, lane);
         }
         if constexpr (O::KEEP) {
             if (u0 + keep < S.steps) ((W __attribute__((address_space(1)))*)((Global)pk + keep_offset<O>(S, u0 + keep)))[lane] = own_kept;
@@ -723,7 +729,9 @@ __device__ __forceinline__ void take_run(const Seq& S, const Place& P, const typ
 template <class O, int DIR, bool FULL>
 __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run<O, 1>& f, int64_t u0, int64_t end, typename O::W h) {
     using E = typename O::Out;
-    E out[L], second[O::SECOND ? L : 1];
+    using D = typename O::Second;
+    E out[L];
+    D second[O::SECOND ? L : 1];
     const int keep = (int)(S.steps % L);
     typename O::W kept{};
 #pragma unroll
@@ -734,7 +742,7 @@ __device__ __forceinline__ void walk_run(const Seq& S, const Place& P, const Run
         if constexpr (O::SECOND) second[i] = second_of<O, 1>(f, i, h);
     }
     put_run<E, DIR, FULL>(P.h, u0, end, out);
-    if constexpr (O::SECOND) put_run<E, DIR, FULL>(P.second, u0, end, second);
+    if constexpr (O::SECOND) put_run<D, DIR, FULL>(P.second, u0, end, second);
     if constexpr (O::KEEP) {
         if (u0 + keep < S.steps) *(typename O::W*)(P.keep + keep_offset<O>(S, u0 + keep)) = kept;
     }
@@ -898,7 +906,7 @@ bool near(const View& v, const Seq& S, int64_t size, int tile) {
 template <class O> bool near(const Seq& S, int tile) {
     constexpr int64_t n = sizeof(typename O::T);
     return near(S.keep, S, sizeof(typename O::W), tile) && near(S.x, S, n, tile) && near(S.gate, S, n, tile) && near(S.before, S, n, tile) && near(S.resets, S, 1, tile) &&
-           near(S.h, S, n, tile) && near(S.second, S, n, tile);
+           near(S.h, S, n, tile) && near(S.second, S, sizeof(typename O::Second), tile);
 }
 
 template <class O, int V, int WT> void launch_columns(Seq& S, const Deal& d, hipStream_t stream) {
@@ -990,6 +998,10 @@ template <Kind K, class T> int run(const Seq& S, void* workspace, hipStream_t st
         if (S.keep.p && K == SCAN) {
             if constexpr (sizeof(T) == 2) rc = resets ? launch<Op<K, T, true, true, true>>(S, workspace, stream, who) : launch<Op<K, T, true, false, true>>(S, workspace, stream, who);
             else rc = fail(-1, "%s: 16-bit sequences only", who);
+        } else if (sizeof(T) == 2 && K == BACKWARD && S.second.p && S.sums) {
+            using P = std::conditional_t<sizeof(T) == 2 && K == BACKWARD, float, T>;
+            if (resets) rc = launch<Op<K, T, true, true, K == BACKWARD, P>>(S, workspace, stream, who);
+            else rc = launch<Op<K, T, true, false, K == BACKWARD, P>>(S, workspace, stream, who);
         } else if (K == BACKWARD && S.second.p) {
             if (resets) rc = launch<Op<K, T, true, true, K == BACKWARD>>(S, workspace, stream, who);
             else rc = launch<Op<K, T, true, false, K == BACKWARD>>(S, workspace, stream, who);
@@ -1045,7 +1057,7 @@ int scan(const char* who, int32_t device, void* hip_stream, const lrn_seq* seq, 
 // `states`: h, or x beside `kept`
 int backward(const char* who, int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* gate, double gate_const, const lrn_view* resets,
              const void* initial, const lrn_view* states, const lrn_view* kept, const lrn_view* g_h, const void* g_final, const lrn_view* grad_x_out,
-             const lrn_view* grad_gate_out, void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
+             const lrn_view* grad_gate_out, bool sums, void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
     if (int rc = checked(seq, who)) return rc;
     if (seq->batch * seq->channels == 0) return 0;
     if (seq->steps && (!g_h || !g_h->data || !grad_x_out || !grad_x_out->data)) return fail(-1, "%s: null g_h or grad_x", who);
@@ -1061,8 +1073,8 @@ int backward(const char* who, int32_t device, void* hip_stream, const lrn_seq* s
     S.x = ordered(g_h, seq->steps, n, rev); S.gate = ordered(gate, seq->steps, n, rev);
     S.resets = ordered(resets, seq->steps, 1, rev); S.before = ordered(want_gate ? states : nullptr, seq->steps, n, rev);
     S.keep = ordered(want_gate ? kept : nullptr, 0, 4, false);
-    S.h = ordered(grad_x_out, seq->steps, n, rev); S.second = ordered(want_gate ? grad_gate_out : nullptr, seq->steps, n, rev);
-    S.gate_const = gate_const; S.initial = g_final; S.edge = initial; S.final = grad_initial_out;
+    S.h = ordered(grad_x_out, seq->steps, n, rev); S.second = ordered(want_gate ? grad_gate_out : nullptr, seq->steps, sums ? 4 : n, rev);
+    S.sums = sums; S.gate_const = gate_const; S.initial = g_final; S.edge = initial; S.final = grad_initial_out;
     return run<BACKWARD>(S, seq->dtype, workspace, (hipStream_t)hip_stream, who);
 }
 
@@ -1104,17 +1116,18 @@ int lrn_scan_backward(int32_t device, void* hip_stream, const lrn_seq* seq, cons
     if (seq && (seq->dtype == LRN_BF16 || seq->dtype == LRN_F16) && grad_gate_out && grad_gate_out->data)
         return fail(-1, "lrn_scan_backward: h holds rounded states: lrn_scan_keep_backward has the gate's gradient of 16-bit sequences");
     return backward("lrn_scan_backward", device, hip_stream, seq, gate, gate_const, resets, initial, h, nullptr, g_h, g_final, grad_x_out, grad_gate_out,
-                    grad_initial_out, workspace, workspace_bytes);
+                    false, grad_initial_out, workspace, workspace_bytes);
 }
 
 int lrn_scan_keep_backward(int32_t device, void* hip_stream, const lrn_seq* seq, const lrn_view* x, const lrn_view* gate,
                            const lrn_view* resets, const void* initial, const lrn_view* kept, const lrn_view* g_h,
-                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out,
+                           const void* g_final, const lrn_view* grad_x_out, const lrn_view* grad_gate_out, int32_t grad_gate_dtype,
                            void* grad_initial_out, void* workspace, int64_t workspace_bytes) {
     if (int rc = keeping(seq, gate, kept, "lrn_scan_keep_backward")) return rc;
     if (seq->steps && (!grad_gate_out || !grad_gate_out->data)) return fail(-1, "lrn_scan_keep_backward: null grad_gate");
+    if (grad_gate_dtype != LRN_F32 && grad_gate_dtype != seq->dtype) return fail(-1, "lrn_scan_keep_backward: grad_gate of dtype %d", grad_gate_dtype);
     return backward("lrn_scan_keep_backward", device, hip_stream, seq, gate, 0.0, resets, initial, x, kept, g_h, g_final, grad_x_out, grad_gate_out,
-                    grad_initial_out, workspace, workspace_bytes);
+                    grad_gate_dtype == LRN_F32, grad_initial_out, workspace, workspace_bytes);
 }
 
 int64_t lrn_advantages_workspace(const lrn_seq* seq) { return workspace_of(seq); }

@@ -376,7 +376,7 @@ class _GatedScan(torch.autograd.Function):
         # The gate's gradient needs the states.  h holds them, but rounded for 16-bit sequences: there every eighth is kept in
         # float32, and the backward pass walks the others again from x.
         keep = ctx.needs_input_grad[1] and x.dtype in (torch.bfloat16, torch.float16)
-        h, final, *kept = _scan(x, gate, gate_const, initial, resets, dim, reverse, keep)
+        h, final, *kept = _scan(x, gate if gate is None else gate.expand(x.shape), gate_const, initial, resets, dim, reverse, keep)
         ctx.save_for_backward(gate, resets, initial, (x if keep else h) if ctx.needs_input_grad[1] else None, *kept)
         ctx.args = (gate_const, dim, reverse, x.shape, x.stride(), x.dtype, x.device)
         ctx.set_materialize_grads(False)
@@ -398,20 +398,26 @@ class _GatedScan(torch.autograd.Function):
         if g_h is None:                                              # only the last state was used
             g_h = torch.zeros((), dtype=dtype, device=device).expand(shape)
         gx = _laid_out(shape, stride, dtype, device)
-        gg = _laid_out(shape, stride, dtype, device) if want_gate else None
+        # (of a broadcast gate: summed before it is rounded)
+        spread, kind = gate is not None and gate.shape != shape, dtype
+        if spread:
+            of, gate, kind = gate.shape, gate.expand(shape), _state_type(dtype)
+        gg = _laid_out(shape, stride, kind, device) if want_gate else None
         gi = torch.empty(initial.shape, dtype=initial.dtype, device=device) if want_initial else None
         seq = _sequence(shape, dim, reverse, dtype)
         ref = C.byref(seq)
         nbytes = lib.lrn_scan_workspace(ref)
         ws = _workspace(nbytes, device)
-        stream, up, out = _stream(device), (_ref(_view(g_h, dim)), _ptr(g_final)), (_ref(_view(gx, dim)), _ref(_view(gg, dim)), _ptr(gi), _ptr(ws), nbytes)
+        stream, up, out = _stream(device), (_ref(_view(g_h, dim)), _ptr(g_final), _ref(_view(gx, dim)), _ref(_view(gg, dim))), (_ptr(gi), _ptr(ws), nbytes)
         if kept and want_gate:
             _check(lib.lrn_scan_keep_backward(device.index, stream, ref, _ref(_view(states, dim)), _ref(_view(gate, dim)),
-                                              _ref(_view(resets, dim)), _ptr(initial), _ref(_view(kept[0], 0)), *up, *out),
+                                              _ref(_view(resets, dim)), _ptr(initial), _ref(_view(kept[0], 0)), *up, _SEQ_TYPES[kind], *out),
                    'gated_scan backward')
         else:
             _check(lib.lrn_scan_backward(device.index, stream, ref, _ref(_view(gate, dim)), gate_const, _ref(_view(resets, dim)),
                                          _ptr(initial), _ref(_view(states, dim)), *up, *out), 'gated_scan backward')
+        if spread and want_gate:
+            gg = gg.sum_to_size(of).to(dtype)
         return gx if want_x else None, gg, gi, None, None, None, None
 
 
@@ -451,7 +457,6 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
         if gate.shape != shape:
             if not _broadcasts(gate, shape):
                 raise ValueError(f'gate: {tuple(gate.shape)} does not broadcast to x\'s {tuple(shape)}')
-            gate = gate.expand(shape)
     elif isinstance(gate, (int, float)):
         const, gate = float(gate), None
     else:
@@ -475,7 +480,7 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
     if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad)
                                     or (initial is not None and initial.requires_grad)):
         return _GatedScan.apply(x, gate, initial, resets, const, dim, reverse)
-    return _scan(x.detach(), gate, const, initial, resets, dim, reverse)
+    return _scan(x.detach(), gate if gate is None else gate.expand(shape), const, initial, resets, dim, reverse)
 
 
 def advantages(rewards, values, ends, last_values, gamma: float = 0.99, lam: float = 0.95) -> Advantages:

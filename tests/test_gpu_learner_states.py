@@ -73,3 +73,41 @@ def test_kept_states_lie_where_they_are_said_to():
                     v, tol = (w[order[at - 1]] for w in want['h'])
                     near(store[1 + j], v, tol, (T, j))
             assert bool((store[0] == -7).all()) and bool((store[n + 1] == -7).all())
+
+
+BROADCAST = [((40, 2, 5), 0, (40, 1, 5)), ((70, 2, 64), 0, (70, 1, 64)), ((2, 40, 7), 1, (1, 40, 7)), ((2, 600, 64), 1, (1, 600, 64)), ((2, 300), 1, (300,)),
+             ((2, 33000), 1, (1, 33000)), ((2, 1100, 33), 1, (1100, 33)), ((1100, 2, 34), 0, (1100, 1, 34)), ((9, 2, 5), 0, (5,)), ((30, 2, 64), 0, (1, 2, 64)),
+             ((30, 2, 3), 0, (30, 2, 1)), ((20, 2), 0, ()), ((20, 2, 130), 0, (1, 1, 1)), ((1, 2, 3), 0, (3,)), ((2, 1, 64), 1, (1, 1, 64))]
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16', 'f32', 'f64'])
+@pytest.mark.parametrize('shape,dim,gshape', BROADCAST, ids=[f'{"x".join(map(str, s))}-{"x".join(map(str, b))}' for s, _, b in BROADCAST])
+def test_the_gradient_of_a_broadcast_gate_is_summed_before_it_is_rounded(shape, dim, gshape, dtype):
+    """Two sequences whose terms nearly cancel: rounded to 16 bits first, their sum would be off by more than its own size allows.
+    torch adds n float32 values up, at most n u of the sum of their sizes off."""
+    from sustaingym_amd import learner
+    kind = TYPES[dtype]
+    g = gen(sum(shape))
+    batch = 1 - dim
+    one = list(shape)
+    one[batch] = 1
+    x, gh = (torch.randn(one, generator=g, device='cuda').to(kind).expand(shape).contiguous() for _ in range(2))
+    other = (slice(None),) * batch + (1,)
+    x[other] *= 1 + 2.0 ** -6
+    gh[other] *= -1
+    gate = torch.sigmoid(torch.randn(gshape, generator=g, device='cuda') + 2).to(kind).requires_grad_(True)
+    wide = (lambda t: t.double()) if kind == torch.float64 else (lambda t: t.float())
+    for reverse in (False, True):
+        resets = torch.rand(shape[:2], generator=g, device='cuda') < 0.05 if reverse else None
+        want = ref.scan(wide(host(x)), wide(host(gate)).expand(shape), None, host(resets), dim, reverse, wide(host(gh)))
+        h, _ = learner.gated_scan(x, gate, None, resets, dim, reverse)
+        got, = torch.autograd.grad(h, gate, gh)
+        assert got.dtype == kind and got.shape == gshape
+        v, tol = want['grad_gate']
+        n = v.numel() // max(1, gate.numel())
+        u = 2.0 ** -53 if kind == torch.float64 else ref.U
+        size = v.abs().sum_to_size(gshape)
+        v, tol = v.sum_to_size(gshape), tol.sum_to_size(gshape) + n * u * size
+        if kind in (torch.bfloat16, torch.float16):
+            v, tol = widened((v, tol), kind)
+        near(got, v, tol, 'gate')

@@ -19,8 +19,8 @@ def test_keeping_refuses():
     def forward(s, x, gate, h, kept):
         return lib.lrn_scan_keep(0, None, s, x, gate, None, None, h, kept, one, None, 0)
 
-    def backward(s, x, gate, kept, g_h, gx, gg):
-        return lib.lrn_scan_keep_backward(0, None, s, x, gate, None, None, kept, g_h, None, gx, gg, None, None, 0)
+    def backward(s, x, gate, kept, g_h, gx, gg, kind=1):
+        return lib.lrn_scan_keep_backward(0, None, s, x, gate, None, None, kept, g_h, None, gx, gg, kind, None, None, 0)
 
     v, back = C.byref(_lib.LearnerView(64, 6, 3, 1)), C.byref(_lib.LearnerView(64, 6, -3, 1))
     for kw in (dict(dtype=0), dict(dtype=3), dict(dtype=4), dict(steps=-1), dict(batch=-1)):
@@ -36,6 +36,8 @@ def test_keeping_refuses():
         assert backward(seq(), *views) == -1 and 'null' in text(), k
     assert forward(seq(), v, v, v, back) == -1 and 'negative' in text()
     assert backward(seq(), v, v, back, v, v, v) == -1 and 'negative' in text()
+    for kind in (-1, 2, 3, 4):
+        assert backward(seq(), v, v, v, v, v, v, kind) == -1 and 'grad_gate' in text()
     # the gate's gradient from rounded states
     for dtype in (1, 2):
         assert lib.lrn_scan_backward(0, None, seq(dtype=dtype), v, 0.0, None, None, v, v, None, v, v, None, None, 0) == -1 and 'rounded' in text()
