@@ -51,9 +51,11 @@ template <class T> __device__ __forceinline__ float to_f32(T v) { return (float)
 constexpr float kNegInf = -__builtin_inff();
 constexpr double kLog2e = 1.4426950408889634;
 
-// exp(x) = 2^(x log2 e) on the exponential unit.  The product is rounded once (relative error of the result at most
-// |x| 2^-24 + 1 unit): the weights below are exp(z - max), where a large |x| is a small weight.
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * (float)kLog2e); }
+// exp(x) = 2^(x log2 e) on the exponential unit.  log2 e in two parts, so that only the product's rounding counts (relative error of
+// the result at most |x| 2^-24 + 1 unit; with the rounded constant alone 1.23 |x| 2^-24): the weights below are exp(z - max), where
+// a large |x| is a small weight.  (The low part is positive: -inf stays -inf.)
+constexpr float kLog2eHigh = (float)kLog2e, kLog2eLow = (float)(kLog2e - (double)kLog2eHigh);
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2eHigh, x * kLog2eLow)); }
 
 // log(s) of a sum of weights (1 <= s, or 0: -inf) on the logarithm unit, 1 unit and one rounding off; 1 / s likewise.
 __device__ __forceinline__ float fast_log(float s) { return __builtin_amdgcn_logf(s) * 0.6931471805599453f; }
