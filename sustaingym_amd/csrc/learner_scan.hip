@@ -965,13 +965,16 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
         else launch_runs<O, -1>(S, d, stream);
     } else {
         // Two columns to a lane, wider rows and half the instructions: in sequences in parts where it takes fewer tiles (131 073
-        // steps of 72 float32: 45 us instead of 55; float64 gains nothing), and for advantages of many sequences, whose 21 bytes
-        // a step keep the memory busy with half the wavefronts (but not in parts: 2048 x 2000 float64 41 us instead of 31).
+        // steps of 72 float32: 45 us instead of 55; float64 gains nothing), and for advantages where four wavefronts stand behind
+        // one another for more than a turn: 21 bytes a step keep the memory busy with half the wavefronts, and rows that start
+        // off a cache line are fetched by fewer of them (288 steps of 65 534 sequences, float64 rewards: 102 us instead of 117;
+        // 65 536: 86 instead of 90; 2000 steps 655 instead of 838 and 540 instead of 549).  Elsewhere one column is level or
+        // ahead: 32 steps of 65 536 10.9 instead of 12.0, 288 of 131 072 float32 118 instead of 129, 262 144 level; in parts 2048
+        // x 2000 float64 31 instead of 41.
         const bool even = S.cols % 2 == 0 && (S.channels == 1 || S.channels % 2 == 0) && dense(S.x, S.channels) && dense(S.gate, S.channels) &&
                           dense(S.before, S.channels) && dense(S.h, S.channels) && dense(S.second, S.channels) && dense(S.keep, S.channels) && near<O>(S, 128);
         if constexpr (O::K == ADVANTAGES) {
-            if (even && S.cols >= 65536 && d.wt == 1) return launch_columns<O, 2, 1>(S, d, stream), 0;
-            if (even && S.cols >= 65536 && d.wt == 4) return launch_columns<O, 2, 4>(S, d, stream), 0;
+            if (even && d.wt == 4 && S.steps > 4 * L) return launch_columns<O, 2, 4>(S, d, stream), 0;
         } else if constexpr (sizeof(typename O::T) <= 4) {
             if (even && d.parts > 1 && S.cols > 64) return launch_columns<O, 2, kMany<O>>(S, d, stream), 0;
         }
