@@ -74,10 +74,9 @@ def _on_device(name: str, t, device=None) -> None:
 
 def _no_tangents(**inputs) -> None:
     """A dual tensor does not require a gradient: its tangent would be dropped without a word."""
-    if forward_ad._current_level >= 0:
-        for name, t in inputs.items():
-            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
-                raise ValueError(f'{name}: there is no forward-mode derivative')
+    for name, t in inputs.items():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f'{name}: there is no forward-mode derivative')
 
 
 def _broadcasts(t, shape) -> bool:
@@ -285,7 +284,8 @@ def level_logprobs(logits, levels, mask=None, top: int = 0) -> LevelScores:
 
     Log probabilities, entropies and all sums are float32 whatever the logits' type; the gradient has the logits' type."""
     _check_rows(logits, mask)
-    _no_tangents(logits=logits)
+    if forward_ad._current_level >= 0:
+        _no_tangents(logits=logits)
     _on_device('levels', levels, logits.device)
     if levels.shape != logits.shape[:-1]:
         raise ValueError(f'levels: {tuple(levels.shape)}, the logits have rows {tuple(logits.shape[:-1])}')
@@ -342,6 +342,10 @@ def _laid_out(shape, stride, dtype, device):
     return torch.empty_strided(shape, stride, dtype=dtype, device=device)
 
 
+def _spread(gate, shape):
+    return gate if gate is None or gate.shape == shape else gate.expand(shape)
+
+
 def _kept(h, dim):
     """Room for every eighth state of 16-bit ``h``, ``[elements, N, C]``: along time where h is, by columns otherwise."""
     steps, N = h.shape[dim], h.shape[1 - dim] if h.dim() > 1 else 1
@@ -376,7 +380,7 @@ class _GatedScan(torch.autograd.Function):
         # The gate's gradient needs the states.  h holds them, but rounded for 16-bit sequences: there every eighth is kept in
         # float32, and the backward pass walks the others again from x.
         keep = ctx.needs_input_grad[1] and x.dtype in (torch.bfloat16, torch.float16)
-        h, final, *kept = _scan(x, gate if gate is None else gate.expand(x.shape), gate_const, initial, resets, dim, reverse, keep)
+        h, final, *kept = _scan(x, _spread(gate, x.shape), gate_const, initial, resets, dim, reverse, keep)
         ctx.save_for_backward(gate, resets, initial, (x if keep else h) if ctx.needs_input_grad[1] else None, *kept)
         ctx.args = (gate_const, dim, reverse, x.shape, x.stride(), x.dtype, x.device)
         ctx.set_materialize_grads(False)
@@ -476,11 +480,12 @@ def gated_scan(x, gate, initial=None, resets=None, dim: int = 0, reverse: bool =
         if resets.shape != shape[:2]:
             raise ValueError(f'resets: {tuple(resets.shape)} instead of {tuple(shape[:2])}')
     reverse = bool(reverse)
-    _no_tangents(x=x, gate=gate, initial=initial)
+    if forward_ad._current_level >= 0:
+        _no_tangents(x=x, gate=gate, initial=initial)
     if torch.is_grad_enabled() and (x.requires_grad or (gate is not None and gate.requires_grad)
                                     or (initial is not None and initial.requires_grad)):
         return _GatedScan.apply(x, gate, initial, resets, const, dim, reverse)
-    return _scan(x.detach(), gate if gate is None else gate.expand(shape), const, initial, resets, dim, reverse)
+    return _scan(x.detach(), _spread(gate, shape), const, initial, resets, dim, reverse)
 
 
 def advantages(rewards, values, ends, last_values, gamma: float = 0.99, lam: float = 0.95) -> Advantages:
