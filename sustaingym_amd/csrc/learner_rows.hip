@@ -152,10 +152,11 @@ struct BackIn { const int64_t* level; const float* stat; const float* entropy; c
 // from the logits that it has to read anyway: cheaper than 12 bytes a row of saved statistics.  Its results meet in LDS, from
 // where they leave as one run of 16-byte stores.
 //
-// Bound by memory where rows are short (65 536 x 54 x 5: float32 127 MB in 25 us = 5.1 TB/s, a large copy's rate; bfloat16 with a
-// mask 110 MB in 31, backward 145 MB in 31), by the issue of some 25 instructions a level where they are not and hold two bytes
-// each (16 000 x 1000 bfloat16: 13 us forward, 19 backward).  An earlier form that brought all rows through LDS, with a division
-// of every element's index, took 28 and 37 us for the first, 16 and 30 for the last.
+// Bound by memory where rows are short and float32 (65 536 x 54 x 5: 127 MB in 28 us = 4.5 TB/s of a large copy's 5.1, backward
+// 198 MB in 33); of two bytes a level, by trips to memory behind one another (logits, mask, then the level's own: 110 MB in 31.5
+// with a mask, backward 145 MB in 31.8); longer rows of two bytes a level by the issue of some 25 instructions a level (16 000 x
+// 1000 bfloat16: 13.6 us forward, 19.8 backward).  An earlier form that brought all rows through LDS, with a division of every
+// element's index, took 16 and 30 for the last.
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -531,8 +532,8 @@ int group_rows(int K) { int n = 256; BY_LEVELS(K, (n = 256 / G, (void)E)); retur
 // too few rows to fill the GPU a row is cut into up to 64 parts, whose sums, best level and best alternatives go through the
 // workspace to a second launch, a wavefront to a row.
 //
-// 1024 x 32768 bfloat16: 67 MB in 16 us (4.2 TB/s), bound by instructions as much as by memory: eleven a level, four of them the
-// exponential's issue.  A row in parts is bound by latency: 8 x 131 071 float32 with 20 alternatives 14 + 10.5 us for 4 MB (a
+// 1024 x 32768 bfloat16: 67 MB in 18 us (3.7 TB/s), bound by instructions as much as by memory: twelve a level, four of them the
+// exponential's issue.  A row in parts is bound by latency: 8 x 131 071 float32 with 20 alternatives 15 + 11 us for 4 MB (a
 // wavefront to a row, as it was first, took 1070).
 
 template <class T> struct Piece {
@@ -800,8 +801,8 @@ __global__ __launch_bounds__(64) void join_kernel(Rows R, ChooseOut C, ScoreOut 
     }
 }
 
-// One piece of 16 bytes after the other, with the row's statistics: bound by memory (1024 x 32768 bfloat16: 134 MB in 23.5 us,
-// 5.7 TB/s; the forward pass has just left the logits in the last-level cache).
+// One piece of 16 bytes after the other, with the row's statistics: bound by memory (1024 x 32768 bfloat16: 134 MB in 25.6 us,
+// 5.2 TB/s; the forward pass has just left the logits in the last-level cache).
 constexpr int kBackPieces = 4;       // pieces a lane
 template <class T>
 __global__ __launch_bounds__(256) void wide_backward_kernel(Rows R, BackIn I, T* grad, int parts) {

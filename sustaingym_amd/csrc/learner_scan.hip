@@ -23,10 +23,10 @@
 // wavefront scan.  TILES: as COLUMNS, with 16 bytes to a lane's load.  State, pairs and products are float32 (float64 for
 // float64 sequences) whatever the elements' type.
 //
-// Bound by memory where there are columns for everybody: advantages of 288 x 65 536 move 397 MB in 83 us (4.8 TB/s of a large
-// copy's 5.1), returns of 288 x 16 384 float64 81 MB in 18; a memory of 16 x 2048 x 1024 bfloat16 201 MB in 39 forward and 336 MB
-// in 70 backward.  131 073 x 72 float32, in 256 parts: 17 + 28 us for 113 MB, 75 of them twice.  A thread to a column, as it was
-// first, took 173, 153, 2075, 2648 and 44 000 us for these.
+// Bound by memory where there are columns for everybody (averages over three sets of inputs in turn, which no cache holds):
+// advantages of 288 x 65 536 move 397 MB in 85 us (4.7 TB/s of a large copy's 5.1), returns of 288 x 16 384 float64 81 MB in 18;
+// a memory of 16 x 2048 x 1024 bfloat16 218 MB in 50 forward and 352 MB in 75 backward.  131 073 x 72 float32, in 256 parts:
+// 19 + 30 us for 113 MB, 75 of them twice.  A thread to a column, as it was first, took 173, 153, 2075, 2648 and 44 000 us.
 //
 // A coefficient of exactly 0 cuts: nothing of the state in front enters, whatever it holds.  For float32 that is the
 // multiplication in which 0 times anything is 0, one instruction instead of a comparison and a selection behind an fma.  That
@@ -502,9 +502,9 @@ __global__ __launch_bounds__(WT == 1 ? 256 : 64 * WT) void columns_kernel(Seq S)
 // one's are worked on.  What a lane needs, a column, it gets through its wavefront's own piece of LDS.  A tile lies in one
 // sequence, whose flags are the same for all its lanes: bits of a scalar.
 //
-// 16 x 2048 x 1024 bfloat16: 201 MB in 38 us forward, 336 MB in 69 backward (5.2 and 4.8 TB/s); one element to a lane at a time,
-// in the kernel above, 41 and 78, and 300 x 2 x 8192 12.1 backward instead of 17.5.  (Elements that no cache holds yet: 47 forward;
-// two turns ahead 45, but 67 backward instead of 66.)
+// Training, from inputs that no cache holds: 16 x 2048 x 1024 bfloat16 48 us forward and 73 backward where one element to a lane at
+// a time, in the kernel above, takes 59 and 83; 4 x 300 x 8192 13.6 and 19.1 where it takes 25 and 35.  (Two turns ahead, tried
+// while no states were kept: 45 us forward instead of 47, 67 backward instead of 66.)
 
 template <class T> struct Tile {
     static constexpr int N = 16 / sizeof(T), LANES = 64 / N, ROWS = N, LOADS = L / ROWS, BYTES = L * 64 * sizeof(T);
@@ -547,7 +547,7 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-constexpr int kTileWaves = 8;    // (16 take 0.5 - 1 us longer to begin and gain nothing, 4 leave half the loads out: 61 us for 38)
+constexpr int kTileWaves = 8;    // (16 take 0.5 - 1 us longer to begin and gain nothing; 4 leave half the loads out: 61 us for what took 38)
 
 template <class O>
 __global__ __launch_bounds__(64 * kTileWaves) void tiles_kernel(Seq S) {
@@ -979,8 +979,9 @@ template <class O> int launch(Seq S, void* workspace, hipStream_t stream, const 
             if (even && d.parts > 1 && S.cols > 64) return launch_columns<O, 2, kMany<O>>(S, d, stream), 0;
         }
         // Tiles where wavefronts stand behind one another, in one part, and all eight have steps where there are tiles enough
-        // (64 x 500 x 1024 bfloat16: 67.6 us backward instead of 76.7; x 32: 8.4 and 7.5).  Where a wavefront has all steps
-        // (256 x 300 x 1024) the memory is busy without: 104 us forward, with them 111.
+        // (64 x 500 x 1024 bfloat16: 67.7 us backward instead of 75.6, 32 x 500 x 1024 33 instead of 49).  Where a wavefront has
+        // all steps the memory is busy without: 256 x 300 x 1024 bfloat16 113 us forward on both sides, 172 backward, with them
+        // 177; at half of that batch they would be ahead (59 instead of 63, 84 instead of 106).
         if constexpr (O::K != ADVANTAGES && sizeof(typename O::T) <= 4) {
             bool tiles = (d.wt == 16 || (d.wt == 4 && S.steps > kTileWaves * L)) && d.parts == 1 && S.channels % 64 == 0;
             for (const View* v : {&S.x, &S.gate, &S.before, &S.h, &S.second, &S.keep}) tiles = tiles && (!v->p || v->sc == 1);
